@@ -6,7 +6,8 @@ live in ``libwm_b200.so`` behind the C ABI of ``include/wm_b200.h``.
 
 from .cyclic import cyclic_attention
 from .cyclic_prefill import FeedbackBlock
-from .decode_step import DecodeStepGraph, KVPoolCache, document_key_mask
+from .decode_step import DecodeStepGraph, KVPoolCache, QuantKVPoolCache, document_key_mask
+from .draft_tree import DraftTree, draft_tree_attention, prepare_draft_tree
 from .metadata import (
     CyclicAttentionMetadata,
     StrictCausalMetadata,
@@ -17,6 +18,7 @@ from .metadata import (
 from .kv_pool import KVPool
 from .layer import cyclic_attention_layer, prepare_queries
 from .mixing import mix_kv_sources, mixed_pool_decode
+from .quant_pool import dequantize_kv_rows, quantized_pool_append, quantized_pool_attention
 from .strict import strict_causal_attention
 
 __all__ = [
@@ -34,6 +36,13 @@ __all__ = [
     "FeedbackBlock",
     "KVPool",
     "KVPoolCache",
+    "QuantKVPoolCache",
+    "quantized_pool_append",
+    "quantized_pool_attention",
+    "dequantize_kv_rows",
+    "DraftTree",
+    "prepare_draft_tree",
+    "draft_tree_attention",
     "DecodeStepGraph",
     "document_key_mask",
 ]

@@ -15,6 +15,7 @@ import torch
 LIBRARY_PATH = Path(__file__).resolve().parent / "libwm_b200.so"
 
 WM_F32, WM_BF16 = 0, 1
+WM_INT8, WM_E4M3 = 2, 3  # pools held in 8 bits
 WM_MASK_CYCLIC, WM_MASK_STRICT, WM_MASK_PACKED = 0, 1, 2
 WM_KERNEL_AUTO, WM_KERNEL_SIMT, WM_KERNEL_TCGEN05 = 0, 1, 2
 
@@ -212,6 +213,114 @@ class PoolFinishArgs(ctypes.Structure):
     ]
 
 
+class PoolCommitArgs(ctypes.Structure):
+    """Mirror of ``wm_pool_commit_args`` (include/wm_b200_serving.h)."""
+
+    _fields_ = [
+        ("keys", ctypes.c_void_p),
+        ("values", ctypes.c_void_p),
+        ("key_scales", ctypes.c_void_p),
+        ("value_scales", ctypes.c_void_p),
+        ("new_keys", ctypes.c_void_p),
+        ("new_values", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("index", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("key_strides", _Strides),
+        ("value_strides", _Strides),
+        ("key_scale_strides", _Strides),
+        ("value_scale_strides", _Strides),
+        ("new_key_strides", _Strides),
+        ("new_value_strides", _Strides),
+        ("storage", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("slots", ctypes.c_int32),
+        ("rows", ctypes.c_int32),
+        ("source_rows", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("lead", ctypes.c_int32),
+        ("lengths_is64", ctypes.c_int32),
+    ]
+
+
+class PoolDequantArgs(ctypes.Structure):
+    """Mirror of ``wm_pool_dequant_args``."""
+
+    _fields_ = [
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("code_strides", _Strides),
+        ("scale_strides", _Strides),
+        ("out_strides", _Strides),
+        ("storage", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("slots", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("lead", ctypes.c_int32),
+        ("lengths_is64", ctypes.c_int32),
+    ]
+
+
+class DraftTreeArgs(ctypes.Structure):
+    """Mirror of ``wm_draft_tree_args``."""
+
+    _fields_ = [
+        ("parents", ctypes.c_void_p),
+        ("ancestors", ctypes.c_void_p),
+        ("depths", ctypes.c_void_p),
+        ("batch", ctypes.c_int32),
+        ("tokens", ctypes.c_int32),
+        ("include_self", ctypes.c_int32),
+    ]
+
+
+class PoolAttnArgs(ctypes.Structure):
+    """Mirror of ``wm_pool_attn_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scales", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p),
+        ("draft_k", ctypes.c_void_p),
+        ("draft_v", ctypes.c_void_p),
+        ("ancestors", ctypes.c_void_p),
+        ("depths", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("key_mask", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("q_strides", _Strides),
+        ("k_strides", _Strides),
+        ("v_strides", _Strides),
+        ("k_scale_strides", _Strides),
+        ("v_scale_strides", _Strides),
+        ("draft_k_strides", _Strides),
+        ("draft_v_strides", _Strides),
+        ("out_strides", _Strides),
+        ("dtype", ctypes.c_int32),
+        ("storage", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("q_len", ctypes.c_int32),
+        ("k_len", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("lead", ctypes.c_int32),
+        ("lengths_is64", ctypes.c_int32),
+        ("shared_tree", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 ATTN_ENTRY_POINTS = (
     "wm_cyclic_attn_fwd",
     "wm_cyclic_attn_bwd",
@@ -226,6 +335,12 @@ ATTN_ENTRY_POINTS = (
 )
 MIX_ENTRY_POINTS = ("wm_mix_sources_fwd", "wm_mix_sources_bwd")
 QUERY_PREP_ENTRY_POINTS = ("wm_query_prepare_fwd", "wm_query_prepare_bwd")
+SERVING_ENTRY_POINTS = (  # include/wm_b200_serving.h
+    ("wm_pool_commit", PoolCommitArgs),
+    ("wm_pool_dequant", PoolDequantArgs),
+    ("wm_draft_tree", DraftTreeArgs),
+    ("wm_pool_attn", PoolAttnArgs),
+)
 QUERY_ENTRY_POINTS = (
     "wm_abi_version",
     "wm_last_error",
@@ -293,6 +408,12 @@ def load_library() -> ctypes.CDLL:
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.POINTER(AttnArgs)]
             fn.restype = ctypes.c_size_t
+        for name, struct in SERVING_ENTRY_POINTS:
+            fn = getattr(lib, name)
+            fn.argtypes = [ctypes.POINTER(struct), ctypes.c_void_p]
+            fn.restype = ctypes.c_int
+        lib.wm_pool_attn_workspace_bytes.argtypes = [ctypes.POINTER(PoolAttnArgs)]
+        lib.wm_pool_attn_workspace_bytes.restype = ctypes.c_size_t
         lib.wm_mix_workspace_bytes.argtypes = [ctypes.POINTER(MixArgs)]
         lib.wm_mix_workspace_bytes.restype = ctypes.c_size_t
         if lib.wm_abi_version() != 1:
@@ -307,6 +428,15 @@ def dtype_code(dtype: torch.dtype) -> int:
     if dtype == torch.bfloat16:
         return WM_BF16
     raise ValueError(f"sm100 kernels support float32 and bfloat16, got {dtype}")
+
+
+def storage_code(dtype: torch.dtype) -> int:
+    """Element type of a pool: the operator types, or one of the 8-bit forms."""
+    if dtype == torch.int8:
+        return WM_INT8
+    if dtype == torch.float8_e4m3fn:
+        return WM_E4M3
+    return dtype_code(dtype)
 
 
 def strides3(t: torch.Tensor) -> _Strides:

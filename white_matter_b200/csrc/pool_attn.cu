@@ -1,0 +1,328 @@
+// Attention of queries that stand behind the committed tokens of a pool -- one token per sequence, a few new ones, or a
+// tree of drafted tokens -- over fp32, bf16 and 8-bit pools.
+#include <limits.h>
+#include <math.h>
+
+#include "pool_attn_walk.cuh"
+
+namespace wm {
+namespace {
+
+using namespace pool;
+
+// ---------------------------------------------------------------- fp32 arithmetic, any type
+// Four elements per lane, LPK lanes per key, R rows per block.
+template <int kStorage>
+struct Held;  // how four elements of a row come in
+template <>
+struct Held<WM_F32> {
+  static constexpr int kBytes = 4;
+  __device__ static void load(const char* p, float (&x)[4]) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  }
+};
+template <>
+struct Held<WM_BF16> {
+  static constexpr int kBytes = 2;
+  __device__ static void load(const char* p, float (&x)[4]) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
+    x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
+  }
+};
+template <>
+struct Held<WM_INT8> {
+  static constexpr int kBytes = 1;
+  __device__ static void load(const char* p, float (&x)[4]) { codes_to_float(*reinterpret_cast<const uint32_t*>(p), true, x); }
+};
+template <>
+struct Held<WM_E4M3> {
+  static constexpr int kBytes = 1;
+  __device__ static void load(const char* p, float (&x)[4]) { codes_to_float(*reinterpret_cast<const uint32_t*>(p), false, x); }
+};
+
+template <int R>
+struct SimtState {
+  float q[R][4], m[R], l[R], acc[R][4];
+  int token[R];  // -1: no such row, or a padding node
+};
+
+// One warp takes its 32 keys of a tile: KPW keys at a time.
+template <int R, int LPK, int kStorage, bool kDraft>
+__device__ __forceinline__ void simt_keys(const wm_pool_attn_args& a, const Piece& c, int first, int limit, SimtState<R>& s) {
+  constexpr int KPW = 32 / LPK;
+  const int lane = threadIdx.x & 31, part = lane % LPK, which = lane / LPK;
+  const bool live = part * 4 < a.head_dim;
+  const int64_t* ks = kDraft ? a.draft_k_strides : a.k_strides;
+  const int64_t* vs = kDraft ? a.draft_v_strides : a.v_strides;
+  const char* k = static_cast<const char*>(kDraft ? a.draft_k : a.k) + (c.b * ks[0] + c.kv_head * ks[1] + part * 4) * Held<kStorage>::kBytes;
+  const char* v = static_cast<const char*>(kDraft ? a.draft_v : a.v) + (c.b * vs[0] + c.kv_head * vs[1] + part * 4) * Held<kStorage>::kBytes;
+  const int words = (a.q_len + 31) / 32;
+  const uint32_t* bits = kDraft ? a.ancestors + (a.shared_tree ? 0ll : static_cast<long long>(c.b) * a.q_len * words) : nullptr;
+  const int* depths = kDraft ? a.depths + (a.shared_tree ? 0ll : static_cast<long long>(c.b) * a.q_len) : nullptr;
+  for (int j0 = first; j0 < first + 32 && j0 < limit; j0 += KPW) {
+    const int j = j0 + which;
+    bool seen = j < limit;
+    if (seen && kDraft) seen = depths[j] >= 0;
+    if (seen && !kDraft && a.key_mask != nullptr) seen = a.key_mask[static_cast<long long>(c.b) * a.k_len + j] != 0;
+    float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f}, kscale = a.scale * kLog2e, vscale = 1.f;
+    if (seen) {
+      if (live) {
+        Held<kStorage>::load(k + j * ks[2] * Held<kStorage>::kBytes, x);
+        Held<kStorage>::load(v + j * vs[2] * Held<kStorage>::kBytes, y);
+      }
+      if (kStorage == WM_INT8 || kStorage == WM_E4M3) {
+        kscale *= a.k_scales[c.b * a.k_scale_strides[0] + c.kv_head * a.k_scale_strides[1] + j * a.k_scale_strides[2]];
+        vscale = a.v_scales[c.b * a.v_scale_strides[0] + c.kv_head * a.v_scale_strides[1] + j * a.v_scale_strides[2]];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float d = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d = fmaf(s.q[r][e], x[e], d);
+#pragma unroll
+      for (int o = LPK / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+      bool use = seen && s.token[r] >= 0;
+      if (kDraft && use) use = (bits[static_cast<long long>(s.token[r]) * words + (j >> 5)] >> (j & 31)) & 1u;
+      if (!use) continue;
+      d *= kscale;
+      const float top = fmaxf(s.m[r], d);
+      const float ref = top == -INFINITY ? 0.f : top;
+      const float keep = exp2f(s.m[r] - ref), p = exp2f(d - ref);
+      s.m[r] = top;
+      s.l[r] = fmaf(s.l[r], keep, p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s.acc[r][e] = fmaf(p * vscale, y[e], s.acc[r][e] * keep);
+    }
+  }
+}
+
+template <typename T, int kStorage, int LPK, int R>
+__global__ void __launch_bounds__(kThreads) pool_attn_simt_kernel(const wm_pool_attn_args a, const Plan plan) {
+  __shared__ float sm_m[kWarps][R], sm_l[kWarps][R], sm_acc[kWarps][R][LPK * 4];
+  constexpr int kOwn = sizeof(T) == 4 ? WM_F32 : WM_BF16;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = lane % LPK;
+  Share share = find_share(a, plan, blockIdx.x, gridDim.x);
+  for (long long at = share.begin; at < share.end;) {
+    const Piece c = next_piece(a, plan, at, share.end, share.b, share.b_begin);
+    at += c.stop - c.tile;
+    SimtState<R> s;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      int token, head;
+      row_place(a, c, plan, r, token, head);
+      s.token[r] = token < a.q_len ? token : -1;
+      s.m[r] = -INFINITY;
+      s.l[r] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s.q[r][e] = s.acc[r][e] = 0.f;
+      if (s.token[r] >= 0) {
+        if (part * 4 < a.head_dim)
+          Held<kOwn>::load(static_cast<const char*>(a.q) + (c.b * a.q_strides[0] + head * a.q_strides[1] + token * a.q_strides[2] + part * 4) * static_cast<int>(sizeof(T)), s.q[r]);
+        if (a.depths != nullptr && a.depths[(a.shared_tree ? 0ll : static_cast<long long>(c.b) * a.q_len) + token] < 0) s.token[r] = -1;
+      }
+    }
+    for (int tile = c.tile; tile < c.stop; ++tile) {
+      if (tile < c.past_tiles)
+        simt_keys<R, LPK, kStorage, false>(a, c, tile * kTileKeys + warp * 32, c.slots, s);
+      else if (a.ancestors != nullptr)
+        simt_keys<R, LPK, kOwn, true>(a, c, (tile - c.past_tiles) * kTileKeys + warp * 32, a.q_len, s);
+    }
+    // join the lane groups of the warp, then the warps
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int o = LPK; o < 32; o <<= 1) {
+        const float m = __shfl_xor_sync(0xffffffffu, s.m[r], o), l = __shfl_xor_sync(0xffffffffu, s.l[r], o);
+        const float top = fmaxf(s.m[r], m), ref = top == -INFINITY ? 0.f : top;
+        const float f = exp2f(s.m[r] - ref), g = exp2f(m - ref);
+        s.l[r] = s.l[r] * f + l * g;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s.acc[r][e] = s.acc[r][e] * f + __shfl_xor_sync(0xffffffffu, s.acc[r][e], o) * g;
+        s.m[r] = top;
+      }
+      if (lane < LPK) {
+        if (lane == 0) sm_m[warp][r] = s.m[r], sm_l[warp][r] = s.l[r];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sm_acc[warp][r][part * 4 + e] = s.acc[r][e];
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < R * a.head_dim; i += kThreads) {
+      const int r = i / a.head_dim, d = i - r * a.head_dim;
+      int token, head;
+      row_place(a, c, plan, r, token, head);
+      if (token >= a.q_len) continue;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w][r]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      float l = 0.f, acc = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = exp2f(sm_m[w][r] - ref);
+        l += sm_l[w][r] * f;
+        acc += sm_acc[w][r][d] * f;
+      }
+      if (whole(c)) {
+        static_cast<T*>(a.out)[c.b * a.out_strides[0] + head * a.out_strides[1] + token * a.out_strides[2] + d] = from_float<T>(l == 0.f ? 0.f : acc / l);
+      } else {
+        float* row = partial_row(static_cast<float*>(a.workspace), a, plan, blockIdx.x, c.tile == 0, r);
+        if (d == 0) row[0] = top, row[1] = l;
+        row[2 + d] = acc;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------- joining the pieces of a segment
+// Block i joins the segment that share i leaves unfinished, if share i also began it.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) pool_attn_join_kernel(const wm_pool_attn_args a, const Plan plan) {
+  const int shares = gridDim.x;
+  Share share = find_share(a, plan, blockIdx.x, shares);
+  if (share.begin >= share.end || share.end >= share.total) return;
+  int b = share.b;
+  long long b_begin = share.b_begin;
+  const Piece c = next_piece(a, plan, share.end, share.total, b, b_begin);  // the segment that the next share goes on with
+  if (c.tile == 0 || share.end - c.tile < share.begin) return;
+  const long long stop = share.end + (c.tiles - c.tile);
+  int last = blockIdx.x + 1;
+  while (share_begin(share.total, last + 1, shares) < stop) ++last;
+  float* workspace = static_cast<float*>(a.workspace);
+  for (int i = threadIdx.x; i < plan.rows_per_block * a.head_dim; i += kThreads) {
+    const int r = i / a.head_dim, d = i - r * a.head_dim;
+    int token, head;
+    row_place(a, c, plan, r, token, head);
+    if (token >= a.q_len) continue;
+    const float* row = partial_row(workspace, a, plan, blockIdx.x, 1, r);
+    float top = row[0], l = row[1], acc = row[2 + d];
+    for (int s = blockIdx.x + 1; s <= last; ++s) {
+      if (share_begin(share.total, s, shares) == share_begin(share.total, s + 1, shares)) continue;  // an empty share
+      row = partial_row(workspace, a, plan, s, 0, r);
+      const float m = row[0], both = fmaxf(top, m), ref = both == -INFINITY ? 0.f : both;
+      const float f = exp2f(top - ref), g = exp2f(m - ref);
+      l = l * f + row[1] * g;
+      acc = acc * f + row[2 + d] * g;
+      top = both;
+    }
+    static_cast<T*>(a.out)[c.b * a.out_strides[0] + head * a.out_strides[1] + token * a.out_strides[2] + d] = from_float<T>(l == 0.f ? 0.f : acc / l);
+  }
+}
+
+// ---------------------------------------------------------------- host
+constexpr int kMaxTreeNodes = 512;
+
+int rows_per_block(const wm_pool_attn_args& a) {
+  const long long rows = static_cast<long long>(a.q_heads / a.kv_heads) * a.q_len;
+  return rows == 1 ? 1 : 4;
+}
+
+bool make_plan(const wm_pool_attn_args& a, Plan& p) {
+  const long long rows = static_cast<long long>(a.q_heads / a.kv_heads) * a.q_len;
+  p.rows_per_block = rows_per_block(a);
+  const long long blocks = (rows + p.rows_per_block - 1) / p.rows_per_block;
+  p.draft_tiles = a.ancestors != nullptr ? (a.q_len + kTileKeys - 1) / kTileKeys : 0;
+  if (blocks * a.kv_heads > INT_MAX || rows > INT_MAX) return false;
+  p.row_blocks = static_cast<int>(blocks);
+  return true;
+}
+
+// One wave: as many shares as blocks fit the GPU, and no more than there can be tiles.
+int count_shares(const wm_pool_attn_args& a, const Plan& p) {
+  const double tiles = static_cast<double>((a.k_len + kTileKeys - 1) / kTileKeys + p.draft_tiles) * a.batch * a.kv_heads * p.row_blocks;
+  const int wave = 148 * 6;
+  return tiles < wave ? (tiles < 1 ? 1 : static_cast<int>(tiles)) : wave;
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool aligned16(const int64_t* strides, int esize) {
+  return strides[0] * esize % 16 == 0 && strides[1] * esize % 16 == 0 && strides[2] * esize % 16 == 0;
+}
+
+int validate(const wm_pool_attn_args& a, Plan& plan) {
+  const char* who = "wm_pool_attn";
+  if (a.q == nullptr || a.k == nullptr || a.v == nullptr || a.out == nullptr) return fail(WM_EINVAL, "%s: q, k, v and out are required", who);
+  if (a.dtype != WM_F32 && a.dtype != WM_BF16) return fail(WM_EINVAL, "%s: dtype must be WM_F32 or WM_BF16", who);
+  const bool quantised = a.storage == WM_INT8 || a.storage == WM_E4M3;
+  if (!quantised && a.storage != a.dtype) return fail(WM_EINVAL, "%s: the pool must be WM_INT8, WM_E4M3 or of the queries' type", who);
+  if (quantised && (a.k_scales == nullptr || a.v_scales == nullptr)) return fail(WM_EINVAL, "%s: an 8-bit pool needs its scales", who);
+  if (a.batch < 1 || a.q_heads < 1 || a.kv_heads < 1 || a.q_len < 1 || a.k_len < 1 || a.head_dim < 1) return fail(WM_EINVAL, "%s: sizes must be positive", who);
+  if (a.q_heads % a.kv_heads) return fail(WM_EINVAL, "%s: q_heads must be a multiple of kv_heads", who);
+  if (a.lead != 0 && a.lead != 1) return fail(WM_EINVAL, "%s: lead must be 0 or 1", who);
+  const int have = (a.draft_k != nullptr) + (a.draft_v != nullptr) + (a.ancestors != nullptr) + (a.depths != nullptr);
+  if (have != 0 && have != 4) return fail(WM_EINVAL, "%s: drafted tokens need their keys, values and both tree tables", who);
+  if (have != 0 && a.q_len > kMaxTreeNodes) return fail(WM_EUNSUPPORTED, "%s: at most %d drafted tokens", who, kMaxTreeNodes);
+  const int wide = a.dtype == WM_F32 ? 4 : 2, held = quantised ? 1 : wide;
+  if (a.head_dim > 128 || a.head_dim * held % 16 || a.head_dim * wide % 16) return fail(WM_EUNSUPPORTED, "%s: head_dim rows must be a multiple of 16 bytes, head_dim at most 128", who);
+  if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.q_strides, wide) || !aligned16(a.k_strides, held) || !aligned16(a.v_strides, held) ||
+      (have != 0 && (!aligned16(a.draft_k) || !aligned16(a.draft_v) || !aligned16(a.draft_k_strides, wide) || !aligned16(a.draft_v_strides, wide))))
+    return fail(WM_EUNSUPPORTED, "%s: rows must be 16-byte aligned", who);
+  if (!make_plan(a, plan)) return fail(WM_EUNSUPPORTED, "%s: too many query rows", who);
+  return WM_OK;
+}
+
+template <typename T, int kStorage, int LPK>
+void launch_rows(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream) {
+  if (plan.rows_per_block == 1)
+    pool_attn_simt_kernel<T, kStorage, LPK, 1><<<shares, kThreads, 0, stream>>>(a, plan);
+  else
+    pool_attn_simt_kernel<T, kStorage, LPK, 4><<<shares, kThreads, 0, stream>>>(a, plan);
+}
+
+template <typename T, int kStorage>
+int launch(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream) {
+  if (a.head_dim <= 32)
+    launch_rows<T, kStorage, 8>(a, plan, shares, stream);
+  else if (a.head_dim <= 64)
+    launch_rows<T, kStorage, 16>(a, plan, shares, stream);
+  else
+    launch_rows<T, kStorage, 32>(a, plan, shares, stream);
+  count_launch();
+  WM_CUDA(cudaGetLastError());
+  if (shares == 1) return WM_OK;
+  pool_attn_join_kernel<T><<<shares, kThreads, 0, stream>>>(a, plan);
+  count_launch();
+  return cuda_check(cudaGetLastError(), "pool_attn_join_kernel");
+}
+
+}  // namespace
+
+size_t pool_attn_workspace(const wm_pool_attn_args& a) {
+  Plan plan;
+  if (a.batch < 1 || a.kv_heads < 1 || a.q_heads < a.kv_heads || a.q_len < 1 || a.k_len < 1 || !make_plan(a, plan)) return 0;
+  return static_cast<size_t>(count_shares(a, plan)) * 2 * plan.rows_per_block * (a.head_dim + 2) * sizeof(float);
+}
+
+int pool_attn_launch(const wm_pool_attn_args& a, cudaStream_t stream) {
+  Plan plan;
+  const int status = validate(a, plan);
+  if (status != WM_OK) return status;
+  const size_t need = pool_attn_workspace(a);
+  if (a.workspace == nullptr || a.workspace_bytes < need) return fail(WM_EWORKSPACE, "wm_pool_attn needs %zu workspace bytes, got %zu", need, a.workspace_bytes);
+  const int shares = count_shares(a, plan);
+  if (a.dtype == WM_F32) {
+    if (a.storage == WM_INT8) return launch<float, WM_INT8>(a, plan, shares, stream);
+    if (a.storage == WM_E4M3) return launch<float, WM_E4M3>(a, plan, shares, stream);
+    return launch<float, WM_F32>(a, plan, shares, stream);
+  }
+  if (a.storage == WM_INT8) return launch<__nv_bfloat16, WM_INT8>(a, plan, shares, stream);
+  if (a.storage == WM_E4M3) return launch<__nv_bfloat16, WM_E4M3>(a, plan, shares, stream);
+  return launch<__nv_bfloat16, WM_BF16>(a, plan, shares, stream);
+}
+
+}  // namespace wm
+
+extern "C" {
+
+size_t wm_pool_attn_workspace_bytes(const wm_pool_attn_args* a) { return a ? wm::pool_attn_workspace(*a) : 0; }
+
+int wm_pool_attn(const wm_pool_attn_args* a, void* stream) {
+  if (a == nullptr) return wm::fail(WM_EINVAL, "wm_pool_attn: null arguments");
+  return wm::pool_attn_launch(*a, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,327 @@
+// Commit of rows to a pool held in 8 bits, the way back, and the tables of trees of drafted tokens.
+#include <limits.h>
+
+#include "serving.cuh"
+
+namespace wm {
+namespace {
+
+constexpr int kThreads = 256;
+
+// ---------------------------------------------------------------- commit
+// 16 bytes of a source row as fp32 values
+template <typename T>
+struct Piece;
+template <>
+struct Piece<float> {
+  static constexpr int N = 4;
+  __device__ static void unpack(const uint4& raw, float (&x)[4]) {
+    x[0] = __uint_as_float(raw.x), x[1] = __uint_as_float(raw.y), x[2] = __uint_as_float(raw.z), x[3] = __uint_as_float(raw.w);
+  }
+};
+template <>
+struct Piece<__nv_bfloat16> {
+  static constexpr int N = 8;
+  __device__ static void unpack(const uint4& raw, float (&x)[8]) {
+    const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
+
+// four codes in a word, element 0 in the low byte
+__device__ __forceinline__ uint32_t int8_codes(const float* x, float inverse) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w |= (static_cast<uint32_t>(__float2int_rn(__fmul_rn(x[i], inverse))) & 0xffu) << (8 * i);
+  return w;
+}
+__device__ __forceinline__ uint32_t e4m3_codes(const float* x, float inverse) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x[1] * inverse), "f"(x[0] * inverse));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(x[3] * inverse), "f"(x[2] * inverse));
+  return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
+}
+
+// What a row is multiplied by before it is rounded, and the scale that is kept, from the bits of its largest magnitude
+// (as integers these order like the magnitudes, with infinity and NaN above every number).
+__device__ __forceinline__ void row_scale(uint32_t top, int storage, float& inverse, float& scale) {
+  inverse = 0.f;
+  scale = 0.f;
+  if (top >= 0x7f800000u) {
+    scale = __uint_as_float(0x7fffffffu);
+  } else if (top >= (27u << 23)) {  // 2^-100; below it the quotients would leave the normal range
+    if (storage == WM_INT8) {  // the correctly rounded quotients are part of the format
+      inverse = __fdiv_rn(127.f, __uint_as_float(top));
+      scale = __fdiv_rn(__uint_as_float(top), 127.f);
+    } else {  // 448 = 1.75 * 2^8
+      const int e = static_cast<int>(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u);
+      scale = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      inverse = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    }
+  }
+}
+
+// LPR lanes hold one row, 16 source bytes each.  grid: (row groups of a plane, planes = (b, head), K or V).
+template <typename T, int LPR, bool kCopy>
+__global__ void __launch_bounds__(kThreads) pool_commit_kernel(const wm_pool_commit_args a) {
+  constexpr int N = Piece<T>::N;
+  const bool values = blockIdx.z != 0;
+  const int64_t* pool_strides = values ? a.value_strides : a.key_strides;
+  const int64_t* scale_strides = values ? a.value_scale_strides : a.key_scale_strides;
+  const int64_t* src_strides = values ? a.new_value_strides : a.new_key_strides;
+  char* pool = static_cast<char*>(values ? a.values : a.keys);
+  float* scales = values ? a.value_scales : a.key_scales;
+  const T* src = static_cast<const T*>(values ? a.new_values : a.new_keys);
+  const int lane = threadIdx.x % LPR;
+  const int row = blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR;
+  const bool live = lane * N < a.head_dim;
+  for (int plane = blockIdx.y; plane < a.batch * a.heads; plane += gridDim.y) {
+    const int b = plane / a.heads, h = plane - b * a.heads;
+    const long long slot = load_index(a.lengths, a.lengths_is64, b) + a.lead + row;
+    long long from = row;
+    bool keep = row < a.rows && slot >= 0 && slot < a.slots;
+    if (keep && a.counts != nullptr) keep = row < a.counts[b];
+    if (keep && a.index != nullptr) {
+      from = a.index[static_cast<long long>(b) * a.rows + row];
+      keep = from >= 0 && from < a.source_rows;
+    }
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (keep && live) raw = *reinterpret_cast<const uint4*>(src + b * src_strides[0] + h * src_strides[1] + from * src_strides[2] + lane * N);
+    if (kCopy) {
+      if (keep && live)
+        *reinterpret_cast<uint4*>(pool + (b * pool_strides[0] + h * pool_strides[1] + slot * pool_strides[2] + lane * N) * static_cast<int>(sizeof(T))) = raw;
+      continue;
+    }
+    float x[N];
+    Piece<T>::unpack(raw, x);
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float inverse, scale;
+    row_scale(top, a.storage, inverse, scale);
+    if (!keep) continue;
+    if (inverse == 0.f) {  // codes of a row of zeros, and of a row that is not finite
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = 0.f;
+    }
+    if (live) {
+      uint32_t w[N / 4];
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) w[i] = a.storage == WM_INT8 ? int8_codes(x + 4 * i, inverse) : e4m3_codes(x + 4 * i, inverse);
+      char* dst = pool + b * pool_strides[0] + h * pool_strides[1] + slot * pool_strides[2] + lane * N;
+      if (N == 8)
+        *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[N / 4 - 1]);
+      else
+        *reinterpret_cast<uint32_t*>(dst) = w[0];
+    }
+    if (lane == 0) scales[b * scale_strides[0] + h * scale_strides[1] + slot * scale_strides[2]] = scale;
+  }
+}
+
+template <typename T, int LPR>
+int commit(const wm_pool_commit_args& a, cudaStream_t stream) {
+  const int per_block = kThreads / LPR;
+  const long long planes = static_cast<long long>(a.batch) * a.heads;
+  const dim3 grid(static_cast<unsigned>((static_cast<long long>(a.rows) + per_block - 1) / per_block), static_cast<unsigned>(planes < 65535 ? planes : 65535), 2);
+  if (a.storage == a.dtype)
+    pool_commit_kernel<T, LPR, true><<<grid, kThreads, 0, stream>>>(a);
+  else
+    pool_commit_kernel<T, LPR, false><<<grid, kThreads, 0, stream>>>(a);
+  count_launch();
+  return cuda_check(cudaGetLastError(), "pool_commit_kernel");
+}
+
+template <typename T>
+int commit_type(const wm_pool_commit_args& a, cudaStream_t stream) {
+  const int lanes = a.head_dim / Piece<T>::N;
+  if (lanes <= 8) return commit<T, 8>(a, stream);
+  if (lanes <= 16) return commit<T, 16>(a, stream);
+  return commit<T, 32>(a, stream);
+}
+
+// ---------------------------------------------------------------- read back
+// One thread turns 16 codes; a plane is one (b, head).
+template <typename T>
+__global__ void __launch_bounds__(kThreads) pool_dequant_kernel(const wm_pool_dequant_args a) {
+  const int per_row = a.head_dim / 16;
+  const long long unit = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x;
+  if (unit >= static_cast<long long>(a.slots) * per_row) return;
+  const int slot = static_cast<int>(unit / per_row), piece = static_cast<int>(unit - static_cast<long long>(slot) * per_row);
+  for (int plane = blockIdx.y; plane < a.batch * a.heads; plane += gridDim.y) {
+    const int b = plane / a.heads, h = plane - b * a.heads;
+    const bool live = a.lengths == nullptr || slot < load_index(a.lengths, a.lengths_is64, b) + a.lead;
+    float x[16];
+    if (live) {
+      const char* codes = static_cast<const char*>(a.codes) + b * a.code_strides[0] + h * a.code_strides[1] + slot * a.code_strides[2];
+      const uint4 raw = *reinterpret_cast<const uint4*>(codes + 16 * piece);
+      const float scale = a.scales[b * a.scale_strides[0] + h * a.scale_strides[1] + slot * a.scale_strides[2]];
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) codes_to_float(w[i], a.storage == WM_INT8, x + 4 * i);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] *= scale;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = 0.f;
+    }
+    T* dst = static_cast<T*>(a.out) + b * a.out_strides[0] + h * a.out_strides[1] + slot * a.out_strides[2] + 16 * piece;
+    constexpr int N = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 16 / N; ++i) {
+      __align__(16) T y[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) y[j] = from_float<T>(x[N * i + j]);
+      reinterpret_cast<uint4*>(dst)[i] = *reinterpret_cast<const uint4*>(y);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- tree tables
+// Pointer doubling over bit sets: after r rounds a node knows its 2^r nearest ancestors and the one 2^r steps up, and
+// takes over that one's set in the next round.  One block per tree, one thread per node; a round reads its neighbours'
+// state, meets, and writes.  Chains that have not ended after the rounds a chain of `tokens` nodes takes are cycles.
+constexpr int kMaxTreeNodes = 512;
+constexpr int kTreeWords = kMaxTreeNodes / 32;
+constexpr int kRoot = -1, kDead = -2;
+
+__global__ void draft_tree_kernel(const wm_draft_tree_args a, int rounds) {
+  __shared__ uint32_t sets[kTreeWords][kMaxTreeNodes];
+  __shared__ int jumps[kMaxTreeNodes];
+  const int node = threadIdx.x, words = (a.tokens + 31) / 32;
+  const long long row = static_cast<long long>(blockIdx.x) * a.tokens + node;
+  const bool live = node < a.tokens;
+  int jump = kDead;
+  uint32_t set[kTreeWords];
+#pragma unroll
+  for (int w = 0; w < kTreeWords; ++w) set[w] = 0;
+  if (live) {
+    const int parent = a.parents[row];
+    jump = parent == -1 ? kRoot : (parent >= 0 && parent < a.tokens && parent != node ? parent : kDead);
+#pragma unroll
+    for (int w = 0; w < kTreeWords; ++w) {
+      if (jump >= 0 && (jump >> 5) == w) set[w] = 1u << (jump & 31);
+      if (w < words) sets[w][node] = set[w];
+    }
+    jumps[node] = jump;
+  }
+  for (int r = 0; r < rounds; ++r) {
+    if (!__syncthreads_or(jump >= 0)) break;  // also: every node's state of the last round is in place
+    const int via = jump;
+    if (via >= 0) {
+#pragma unroll
+      for (int w = 0; w < kTreeWords; ++w)
+        if (w < words) set[w] |= sets[w][via];
+      jump = jumps[via];
+    }
+    __syncthreads();
+    if (via >= 0) {
+#pragma unroll
+      for (int w = 0; w < kTreeWords; ++w)
+        if (w < words) sets[w][node] = set[w];
+      jumps[node] = jump;
+    }
+  }
+  if (!live) return;
+  int depth = 0;
+#pragma unroll
+  for (int w = 0; w < kTreeWords; ++w) {
+    if (w < words) {
+      depth += __popc(set[w]);
+      uint32_t seen = jump == kRoot ? set[w] : 0u;
+      if (a.include_self && jump == kRoot && (node >> 5) == w) seen |= 1u << (node & 31);
+      a.ancestors[row * words + w] = seen;
+    }
+  }
+  a.depths[row] = jump == kRoot ? depth : -1;
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool aligned16(const int64_t* strides, int esize) {
+  return strides[0] * esize % 16 == 0 && strides[1] * esize % 16 == 0 && strides[2] * esize % 16 == 0;
+}
+
+}  // namespace
+
+int pool_commit_launch(const wm_pool_commit_args& a, cudaStream_t stream) {
+  const char* who = "wm_pool_commit";
+  if (a.keys == nullptr || a.values == nullptr || a.new_keys == nullptr || a.new_values == nullptr || a.lengths == nullptr)
+    return fail(WM_EINVAL, "%s: pool, new rows and lengths are required", who);
+  if (a.dtype != WM_F32 && a.dtype != WM_BF16) return fail(WM_EINVAL, "%s: new rows must be WM_F32 or WM_BF16", who);
+  const bool quantised = a.storage == WM_INT8 || a.storage == WM_E4M3;
+  if (!quantised && a.storage != a.dtype) return fail(WM_EINVAL, "%s: the pool must be WM_INT8, WM_E4M3 or of the rows' type", who);
+  if (quantised && (a.key_scales == nullptr || a.value_scales == nullptr)) return fail(WM_EINVAL, "%s: an 8-bit pool needs its scales", who);
+  if (a.batch < 1 || a.heads < 1 || a.slots < 1 || a.rows < 1 || a.source_rows < 1 || a.head_dim < 1)
+    return fail(WM_EINVAL, "%s: sizes must be positive", who);
+  if (a.index == nullptr && a.source_rows < a.rows) return fail(WM_EINVAL, "%s: more rows than the source has", who);
+  if (a.lead != 0 && a.lead != 1) return fail(WM_EINVAL, "%s: lead must be 0 or 1", who);
+  if (a.head_dim % 16 || a.head_dim > 128) return fail(WM_EUNSUPPORTED, "%s: head_dim must be a multiple of 16 up to 128", who);
+  if (static_cast<long long>(a.batch) * a.heads > INT_MAX) return fail(WM_EUNSUPPORTED, "%s: too many (sequence, head) planes", who);
+  const int wide = a.dtype == WM_F32 ? 4 : 2, held = quantised ? 1 : wide;
+  if (!aligned16(a.keys) || !aligned16(a.values) || !aligned16(a.new_keys) || !aligned16(a.new_values) || !aligned16(a.key_strides, held) ||
+      !aligned16(a.value_strides, held) || !aligned16(a.new_key_strides, wide) || !aligned16(a.new_value_strides, wide))
+    return fail(WM_EUNSUPPORTED, "%s: rows must be 16-byte aligned", who);
+  return a.dtype == WM_F32 ? commit_type<float>(a, stream) : commit_type<__nv_bfloat16>(a, stream);
+}
+
+int pool_dequant_launch(const wm_pool_dequant_args& a, cudaStream_t stream) {
+  const char* who = "wm_pool_dequant";
+  if (a.codes == nullptr || a.scales == nullptr || a.out == nullptr) return fail(WM_EINVAL, "%s: codes, scales and out are required", who);
+  if (a.storage != WM_INT8 && a.storage != WM_E4M3) return fail(WM_EINVAL, "%s: storage must be WM_INT8 or WM_E4M3", who);
+  if (a.dtype != WM_F32 && a.dtype != WM_BF16) return fail(WM_EINVAL, "%s: dtype must be WM_F32 or WM_BF16", who);
+  if (a.batch < 1 || a.heads < 1 || a.slots < 1 || a.head_dim < 1) return fail(WM_EINVAL, "%s: sizes must be positive", who);
+  if (a.lead != 0 && a.lead != 1) return fail(WM_EINVAL, "%s: lead must be 0 or 1", who);
+  if (a.head_dim % 16 || a.head_dim > 128) return fail(WM_EUNSUPPORTED, "%s: head_dim must be a multiple of 16 up to 128", who);
+  const long long planes = static_cast<long long>(a.batch) * a.heads;
+  if (planes > INT_MAX) return fail(WM_EUNSUPPORTED, "%s: too many (sequence, head) planes", who);
+  const int wide = a.dtype == WM_F32 ? 4 : 2;
+  if (!aligned16(a.codes) || !aligned16(a.out) || !aligned16(a.code_strides, 1) || !aligned16(a.out_strides, wide))
+    return fail(WM_EUNSUPPORTED, "%s: rows must be 16-byte aligned", who);
+  const long long units = static_cast<long long>(a.slots) * (a.head_dim / 16);
+  const dim3 grid(static_cast<unsigned>((units + kThreads - 1) / kThreads), static_cast<unsigned>(planes < 65535 ? planes : 65535));
+  if (a.dtype == WM_F32)
+    pool_dequant_kernel<float><<<grid, kThreads, 0, stream>>>(a);
+  else
+    pool_dequant_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(a);
+  count_launch();
+  return cuda_check(cudaGetLastError(), "pool_dequant_kernel");
+}
+
+int draft_tree_launch(const wm_draft_tree_args& a, cudaStream_t stream) {
+  const char* who = "wm_draft_tree";
+  if (a.parents == nullptr || a.ancestors == nullptr || a.depths == nullptr) return fail(WM_EINVAL, "%s: parents, ancestors and depths are required", who);
+  if (a.batch < 1 || a.tokens < 1) return fail(WM_EINVAL, "%s: sizes must be positive", who);
+  if (a.tokens > kMaxTreeNodes) return fail(WM_EUNSUPPORTED, "%s: at most %d drafted tokens", who, kMaxTreeNodes);
+  if (a.include_self != 0 && a.include_self != 1) return fail(WM_EINVAL, "%s: include_self must be 0 or 1", who);
+  int rounds = 0;
+  while ((1 << rounds) < a.tokens) ++rounds;
+  draft_tree_kernel<<<a.batch, (a.tokens + 31) / 32 * 32, 0, stream>>>(a, rounds);
+  count_launch();
+  return cuda_check(cudaGetLastError(), "draft_tree_kernel");
+}
+
+}  // namespace wm
+
+extern "C" {
+
+int wm_pool_commit(const wm_pool_commit_args* a, void* stream) {
+  if (a == nullptr) return wm::fail(WM_EINVAL, "wm_pool_commit: null arguments");
+  return wm::pool_commit_launch(*a, static_cast<cudaStream_t>(stream));
+}
+
+int wm_pool_dequant(const wm_pool_dequant_args* a, void* stream) {
+  if (a == nullptr) return wm::fail(WM_EINVAL, "wm_pool_dequant: null arguments");
+  return wm::pool_dequant_launch(*a, static_cast<cudaStream_t>(stream));
+}
+
+int wm_draft_tree(const wm_draft_tree_args* a, void* stream) {
+  if (a == nullptr) return wm::fail(WM_EINVAL, "wm_draft_tree: null arguments");
+  return wm::draft_tree_launch(*a, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

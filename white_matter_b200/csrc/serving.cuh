@@ -1,0 +1,30 @@
+// Shared by the serving operators: element types of a pool on the device, and the launchers behind
+// include/wm_b200_serving.h.
+#pragma once
+
+#include "common.cuh"
+#include "wm_b200_serving.h"
+
+namespace wm {
+
+int pool_commit_launch(const wm_pool_commit_args& a, cudaStream_t stream);
+int pool_dequant_launch(const wm_pool_dequant_args& a, cudaStream_t stream);
+int draft_tree_launch(const wm_draft_tree_args& a, cudaStream_t stream);
+int pool_attn_launch(const wm_pool_attn_args& a, cudaStream_t stream);
+size_t pool_attn_workspace(const wm_pool_attn_args& a);
+
+// the four codes of a word as fp32 numbers, element 0 in the low byte
+__device__ __forceinline__ void codes_to_float(uint32_t w, bool is_int8, float* x) {
+  if (is_int8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i)));
+  } else {
+    uint32_t lo, hi;  // two halves each; every e4m3 number is an fp16 number
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"(static_cast<uint16_t>(w)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"(static_cast<uint16_t>(w >> 16)));
+    asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; cvt.f32.f16 %0, l; cvt.f32.f16 %1, h;}" : "=f"(x[0]), "=f"(x[1]) : "r"(lo));
+    asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; cvt.f32.f16 %0, l; cvt.f32.f16 %1, h;}" : "=f"(x[2]), "=f"(x[3]) : "r"(hi));
+  }
+}
+
+}  // namespace wm
