@@ -3,15 +3,15 @@
 #include <limits.h>
 #include <math.h>
 
-#include "pool_attn_walk.cuh"
+#include "pool_attn_mma.cuh"
 
 namespace wm {
 namespace {
 
 using namespace pool;
 
-// ---------------------------------------------------------------- fp32 arithmetic, any type
-// Four elements per lane, LPK lanes per key, R rows per block.
+// ---------------------------------------------------------------- fp32 queries
+// Products in fp32 on the FMA pipe: four elements per lane, LPK lanes per key, R rows per block.
 template <int kStorage>
 struct Held;  // how four elements of a row come in
 template <>
@@ -20,15 +20,6 @@ struct Held<WM_F32> {
   __device__ static void load(const char* p, float (&x)[4]) {
     const float4 v = *reinterpret_cast<const float4*>(p);
     x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-  }
-};
-template <>
-struct Held<WM_BF16> {
-  static constexpr int kBytes = 2;
-  __device__ static void load(const char* p, float (&x)[4]) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
-    x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
   }
 };
 template <>
@@ -99,10 +90,9 @@ __device__ __forceinline__ void simt_keys(const wm_pool_attn_args& a, const Piec
   }
 }
 
-template <typename T, int kStorage, int LPK, int R>
+template <int kStorage, int LPK, int R>
 __global__ void __launch_bounds__(kThreads) pool_attn_simt_kernel(const wm_pool_attn_args a, const Plan plan) {
   __shared__ float sm_m[kWarps][R], sm_l[kWarps][R], sm_acc[kWarps][R][LPK * 4];
-  constexpr int kOwn = sizeof(T) == 4 ? WM_F32 : WM_BF16;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = lane % LPK;
   Share share = find_share(a, plan, blockIdx.x, gridDim.x);
   for (long long at = share.begin; at < share.end;) {
@@ -120,7 +110,7 @@ __global__ void __launch_bounds__(kThreads) pool_attn_simt_kernel(const wm_pool_
       for (int e = 0; e < 4; ++e) s.q[r][e] = s.acc[r][e] = 0.f;
       if (s.token[r] >= 0) {
         if (part * 4 < a.head_dim)
-          Held<kOwn>::load(static_cast<const char*>(a.q) + (c.b * a.q_strides[0] + head * a.q_strides[1] + token * a.q_strides[2] + part * 4) * static_cast<int>(sizeof(T)), s.q[r]);
+          Held<WM_F32>::load(static_cast<const char*>(a.q) + (c.b * a.q_strides[0] + head * a.q_strides[1] + token * a.q_strides[2] + part * 4) * 4, s.q[r]);
         if (a.depths != nullptr && a.depths[(a.shared_tree ? 0ll : static_cast<long long>(c.b) * a.q_len) + token] < 0) s.token[r] = -1;
       }
     }
@@ -128,7 +118,7 @@ __global__ void __launch_bounds__(kThreads) pool_attn_simt_kernel(const wm_pool_
       if (tile < c.past_tiles)
         simt_keys<R, LPK, kStorage, false>(a, c, tile * kTileKeys + warp * 32, c.slots, s);
       else if (a.ancestors != nullptr)
-        simt_keys<R, LPK, kOwn, true>(a, c, (tile - c.past_tiles) * kTileKeys + warp * 32, a.q_len, s);
+        simt_keys<R, LPK, WM_F32, true>(a, c, (tile - c.past_tiles) * kTileKeys + warp * 32, a.q_len, s);
     }
     // join the lane groups of the warp, then the warps
 #pragma unroll
@@ -167,7 +157,7 @@ __global__ void __launch_bounds__(kThreads) pool_attn_simt_kernel(const wm_pool_
         acc += sm_acc[w][r][d] * f;
       }
       if (whole(c)) {
-        static_cast<T*>(a.out)[c.b * a.out_strides[0] + head * a.out_strides[1] + token * a.out_strides[2] + d] = from_float<T>(l == 0.f ? 0.f : acc / l);
+        static_cast<float*>(a.out)[c.b * a.out_strides[0] + head * a.out_strides[1] + token * a.out_strides[2] + d] = l == 0.f ? 0.f : acc / l;
       } else {
         float* row = partial_row(static_cast<float*>(a.workspace), a, plan, blockIdx.x, c.tile == 0, r);
         if (d == 0) row[0] = top, row[1] = l;
@@ -215,10 +205,11 @@ __global__ void __launch_bounds__(kThreads) pool_attn_join_kernel(const wm_pool_
 
 // ---------------------------------------------------------------- host
 constexpr int kMaxTreeNodes = 512;
+constexpr int kSms = 148;
 
 int rows_per_block(const wm_pool_attn_args& a) {
   const long long rows = static_cast<long long>(a.q_heads / a.kv_heads) * a.q_len;
-  return rows == 1 ? 1 : 4;
+  return a.dtype == WM_F32 ? (rows == 1 ? 1 : 4) : mma_rows_per_block(rows, a.head_dim);
 }
 
 bool make_plan(const wm_pool_attn_args& a, Plan& p) {
@@ -234,7 +225,7 @@ bool make_plan(const wm_pool_attn_args& a, Plan& p) {
 // One wave: as many shares as blocks fit the GPU, and no more than there can be tiles.
 int count_shares(const wm_pool_attn_args& a, const Plan& p) {
   const double tiles = static_cast<double>((a.k_len + kTileKeys - 1) / kTileKeys + p.draft_tiles) * a.batch * a.kv_heads * p.row_blocks;
-  const int wave = 148 * 6;
+  const int wave = kSms * (a.dtype == WM_F32 ? 6 : mma_resident_blocks(p.rows_per_block, a.head_dim));
   return tiles < wave ? (tiles < 1 ? 1 : static_cast<int>(tiles)) : wave;
 }
 
@@ -265,28 +256,22 @@ int validate(const wm_pool_attn_args& a, Plan& plan) {
   return WM_OK;
 }
 
-template <typename T, int kStorage, int LPK>
-void launch_rows(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream) {
+template <int kStorage, int LPK>
+void launch_simt_rows(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream) {
   if (plan.rows_per_block == 1)
-    pool_attn_simt_kernel<T, kStorage, LPK, 1><<<shares, kThreads, 0, stream>>>(a, plan);
+    pool_attn_simt_kernel<kStorage, LPK, 1><<<shares, kThreads, 0, stream>>>(a, plan);
   else
-    pool_attn_simt_kernel<T, kStorage, LPK, 4><<<shares, kThreads, 0, stream>>>(a, plan);
+    pool_attn_simt_kernel<kStorage, LPK, 4><<<shares, kThreads, 0, stream>>>(a, plan);
 }
 
-template <typename T, int kStorage>
-int launch(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream) {
+template <int kStorage>
+void launch_simt(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream) {
   if (a.head_dim <= 32)
-    launch_rows<T, kStorage, 8>(a, plan, shares, stream);
+    launch_simt_rows<kStorage, 8>(a, plan, shares, stream);
   else if (a.head_dim <= 64)
-    launch_rows<T, kStorage, 16>(a, plan, shares, stream);
+    launch_simt_rows<kStorage, 16>(a, plan, shares, stream);
   else
-    launch_rows<T, kStorage, 32>(a, plan, shares, stream);
-  count_launch();
-  WM_CUDA(cudaGetLastError());
-  if (shares == 1) return WM_OK;
-  pool_attn_join_kernel<T><<<shares, kThreads, 0, stream>>>(a, plan);
-  count_launch();
-  return cuda_check(cudaGetLastError(), "pool_attn_join_kernel");
+    launch_simt_rows<kStorage, 32>(a, plan, shares, stream);
 }
 
 }  // namespace
@@ -305,13 +290,28 @@ int pool_attn_launch(const wm_pool_attn_args& a, cudaStream_t stream) {
   if (a.workspace == nullptr || a.workspace_bytes < need) return fail(WM_EWORKSPACE, "wm_pool_attn needs %zu workspace bytes, got %zu", need, a.workspace_bytes);
   const int shares = count_shares(a, plan);
   if (a.dtype == WM_F32) {
-    if (a.storage == WM_INT8) return launch<float, WM_INT8>(a, plan, shares, stream);
-    if (a.storage == WM_E4M3) return launch<float, WM_E4M3>(a, plan, shares, stream);
-    return launch<float, WM_F32>(a, plan, shares, stream);
+    if (a.storage == WM_INT8)
+      launch_simt<WM_INT8>(a, plan, shares, stream);
+    else if (a.storage == WM_E4M3)
+      launch_simt<WM_E4M3>(a, plan, shares, stream);
+    else
+      launch_simt<WM_F32>(a, plan, shares, stream);
+  } else if (a.storage == WM_INT8) {
+    launch_mma_int8(a, plan, shares, stream);
+  } else if (a.storage == WM_E4M3) {
+    launch_mma_e4m3(a, plan, shares, stream);
+  } else {
+    launch_mma_bf16(a, plan, shares, stream);
   }
-  if (a.storage == WM_INT8) return launch<__nv_bfloat16, WM_INT8>(a, plan, shares, stream);
-  if (a.storage == WM_E4M3) return launch<__nv_bfloat16, WM_E4M3>(a, plan, shares, stream);
-  return launch<__nv_bfloat16, WM_BF16>(a, plan, shares, stream);
+  count_launch();
+  WM_CUDA(cudaGetLastError());
+  if (shares == 1) return WM_OK;
+  if (a.dtype == WM_F32)
+    pool_attn_join_kernel<float><<<shares, kThreads, 0, stream>>>(a, plan);
+  else
+    pool_attn_join_kernel<__nv_bfloat16><<<shares, kThreads, 0, stream>>>(a, plan);
+  count_launch();
+  return cuda_check(cudaGetLastError(), "pool_attn_join_kernel");
 }
 
 }  // namespace wm

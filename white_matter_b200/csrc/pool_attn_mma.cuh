@@ -1,0 +1,595 @@
+// Pool attention for bf16 queries on the warp-level matrix instructions (bf16 operands, fp32 sums).
+//
+// The read is bound by HBM: a pool row is used by the few rows of its KV head and then never again, so what counts is
+// bytes in flight, and few instructions per byte.  Pool rows therefore go from global memory straight into the registers
+// of the warp that uses them, in the order the matrix instruction wants them, and the next step's rows are asked for as
+// soon as this step's have been used; shared memory only joins the warps of a block at the end of a segment.
+//
+// Both products are formed transposed, S^T = K Q^T and O^T = V^T P^T, so that the keys (or head_dim) fill the 16 rows
+// of an instruction and 8 query rows its columns: a single query wastes 7 of 8 columns instead of 15 of 16, registers
+// grow by 8 rows at a time, and the fragment of K that a lane needs is one contiguous piece of a pool row.  The order of
+// head_dim inside the instructions is free as long as Q (or the output) follows it: lane t of a row's four lanes holds
+// elements t*DP/4 .. of a key, lane g of eight holds elements g*DP/8 .. of a value row.
+//
+// Codes of 8-bit pools become bf16 in registers, which is exact; the key's scale multiplies the score in fp32, the
+// value's scale the weight before it is rounded to bf16 (2^-8 relative at most, like the weight of a bf16 pool).
+//
+// A row's weights are exponentials against a reference that moves only when a score exceeds it by 8 (in powers of two):
+// the sums are fp32 and the weights floating, so nothing is lost by weights up to 2^8, and the common step needs
+// one vote instead of a reduction over the lanes.
+#pragma once
+
+#include <math.h>
+
+#include "pool_attn_walk.cuh"
+
+namespace wm {
+namespace pool {
+
+constexpr float kNoReference = -3.0e38f;
+constexpr float kReferenceSlack = 8.f;
+
+// ---------------------------------------------------------------- instructions
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t y;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+  return y;
+}
+// kBytes (4, 8 or 16) of a pool row, zeros where `live` is false; read once, so kept out of L1
+template <int kBytes>
+__device__ __forceinline__ void load_row(uint32_t* r, const char* p, bool live) {
+#pragma unroll
+  for (int i = 0; i < kBytes / 4; ++i) r[i] = 0;
+  if (!live) return;
+  if (kBytes == 16)
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[kBytes / 4 > 1]), "=r"(r[kBytes / 4 > 2 ? 2 : 0]), "=r"(r[kBytes / 4 > 3 ? 3 : 0]) : "l"(p));
+  else if (kBytes == 8)
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[kBytes / 4 > 1]) : "l"(p));
+  else
+    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(r[0]) : "l"(p));
+}
+
+// ---------------------------------------------------------------- how rows are held
+template <int kStorage>
+struct Codes {
+  static constexpr int kBytes = kStorage == WM_BF16 ? 2 : 1;
+  // bytes 0, 2 (even) and 1, 3 (odd) of a word of codes as bf16 pairs
+  __device__ static uint32_t even(uint32_t w) {
+    if (kStorage == WM_INT8) return int8_pair(w);
+    return e4m3_pair((w << 4) & 0x07f007f0u, w << 8);
+  }
+  __device__ static uint32_t odd(uint32_t w) {
+    if (kStorage == WM_INT8) return int8_pair(w >> 8);
+    return e4m3_pair((w >> 4) & 0x07f007f0u, w);
+  }
+
+ private:
+  // low seven bits as 128 + x, the sign bit as 128 or 256: their difference is the code, exactly
+  __device__ static uint32_t int8_pair(uint32_t w) {
+    const uint32_t x = (w & 0x007f007fu) | 0x43004300u, s = (w & 0x00800080u) | 0x43004300u;
+    uint32_t y;
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(s));
+    return y;
+  }
+  // exponent and fraction in the places bf16 has them, which reads as 2^-120 of the number (subnormals too)
+  __device__ static uint32_t e4m3_pair(uint32_t magnitude, uint32_t sign) {
+    const uint32_t x = magnitude | (sign & 0x80008000u);
+    uint32_t y;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x7b807b80u));
+    return y;
+  }
+};
+
+// A lane's part of 16 pool rows: two key rows (g, g + 8) in pieces of DP/4 elements, four value rows (2t, 2t + 1, 2t + 8,
+// 2t + 9) in pieces of DP/8.
+template <int kStorage, int DP>
+struct Rows {
+  static constexpr int kBytes = Codes<kStorage>::kBytes;
+  static constexpr int kKeyBytes = DP / 4 * kBytes, kValueBytes = DP / 8 * kBytes;
+  static constexpr int kKeyWords = kKeyBytes / 4, kValueWords = kValueBytes / 4;
+  static constexpr int kKeyUnit = kKeyBytes % 16 ? 8 : 16;
+  static constexpr int kValueUnit = kValueBytes % 16 == 0 ? 16 : (kValueBytes % 8 == 0 ? 8 : 4);
+
+  // A row has row_bytes (a multiple of 16) of the DP elements; what lies behind them counts as zeros.
+  __device__ static void load_key(uint32_t (&r)[kKeyWords], const char* row, int t, int row_bytes, bool live) {
+#pragma unroll
+    for (int i = 0; i < kKeyBytes / kKeyUnit; ++i) {
+      const int at = t * kKeyBytes + i * kKeyUnit;
+      load_row<kKeyUnit>(r + i * kKeyUnit / 4, row + at, live && at < row_bytes);
+    }
+  }
+  __device__ static void load_value(uint32_t (&r)[kValueWords], const char* row, int g, int row_bytes, bool live) {
+#pragma unroll
+    for (int i = 0; i < kValueBytes / kValueUnit; ++i) {
+      const int at = g * kValueBytes + i * kValueUnit;
+      load_row<kValueUnit>(r + i * kValueUnit / 4, row + at, live && at < row_bytes);
+    }
+  }
+  // Fragment s (16 of head_dim) of K: elements 4s .. 4s + 3 of the piece.  8-bit pools take them in the order 0, 2, 1, 3,
+  // which is how a word of codes comes apart; kPermute gives bf16 rows the same order.
+  template <bool kPermute>
+  __device__ static void key_fragment(uint32_t (&a)[4], const uint32_t (&lo)[kKeyWords], const uint32_t (&hi)[kKeyWords], int s) {
+    if (kStorage == WM_BF16) {
+      const uint32_t l0 = lo[2 * s < kKeyWords ? 2 * s : 0], l1 = lo[2 * s + 1 < kKeyWords ? 2 * s + 1 : 0];
+      const uint32_t h0 = hi[2 * s < kKeyWords ? 2 * s : 0], h1 = hi[2 * s + 1 < kKeyWords ? 2 * s + 1 : 0];
+      a[0] = kPermute ? __byte_perm(l0, l1, 0x5410) : l0;
+      a[1] = kPermute ? __byte_perm(h0, h1, 0x5410) : h0;
+      a[2] = kPermute ? __byte_perm(l0, l1, 0x7632) : l1;
+      a[3] = kPermute ? __byte_perm(h0, h1, 0x7632) : h1;
+    } else {
+      a[0] = Codes<kStorage>::even(lo[s]);
+      a[1] = Codes<kStorage>::even(hi[s]);
+      a[2] = Codes<kStorage>::odd(lo[s]);
+      a[3] = Codes<kStorage>::odd(hi[s]);
+    }
+  }
+  // Fragment s of V^T: elements 2s, 2s + 1 of the piece for the four keys.
+  __device__ static void value_fragment(uint32_t (&a)[4], const uint32_t (&v)[4][kValueWords], int s) {
+    if (kStorage == WM_BF16) {
+      const int w = s < kValueWords ? s : 0;
+      a[0] = __byte_perm(v[0][w], v[1][w], 0x5410);
+      a[1] = __byte_perm(v[0][w], v[1][w], 0x7632);
+      a[2] = __byte_perm(v[2][w], v[3][w], 0x5410);
+      a[3] = __byte_perm(v[2][w], v[3][w], 0x7632);
+    } else {
+      const uint32_t pick = s & 1 ? 0x7632 : 0x5410;  // elements 2s, 2s + 1 of two keys: x0 x1 y0 y1
+      const uint32_t first = __byte_perm(v[0][s / 2], v[1][s / 2], pick), second = __byte_perm(v[2][s / 2], v[3][s / 2], pick);
+      a[0] = Codes<kStorage>::even(first);
+      a[1] = Codes<kStorage>::odd(first);
+      a[2] = Codes<kStorage>::even(second);
+      a[3] = Codes<kStorage>::odd(second);
+    }
+  }
+};
+
+// ---------------------------------------------------------------- state of a warp
+template <int DP, int RT>
+struct State {
+  float o[DP / 16][RT][4];  // O^T: head_dim g*DP/8 + 2s (+1), rows 2t, 2t + 1 of tile rt
+  float m[RT][2], l[RT][2]; // reference and this lane's part of the sum, rows 2t and 2t + 1
+};
+
+// Queries as B operands of S^T = K Q^T: rows g of tile rt, fragment s.  Few tiles stay in registers, more lie in shared memory.
+template <int DP, int RT>
+struct Queries {
+  static constexpr bool kShared = RT * DP > 128;
+  uint2 reg[kShared ? 1 : RT][kShared ? 1 : DP / 16];
+  const uint2* shared;
+  __device__ uint2 get(int rt, int s) const { return kShared ? shared[(rt * (DP / 16) + s) * 32 + (threadIdx.x & 31)] : reg[kShared ? 0 : rt][kShared ? 0 : s]; }
+};
+
+// Weights of 16 keys for tile rt, as the B operand of O^T += V^T P^T.  `x` holds the scores' products with the queries
+// (keys g: x[0], x[1]; g + 8: x[2], x[3]; rows 2t, 2t + 1), f0 / f1 what they are multiplied by, w0 / w1 the value scales;
+// seen[j] bit 0 / 1: row 2t + j sees key g / g + 8.
+template <int DP, int RT, bool kScaled>
+__device__ __forceinline__ void weights(State<DP, RT>& st, int rt, float (&x)[4], float f0, float f1, float w0, float w1, bool all, const uint32_t (&seen)[2],
+                                        uint32_t& b0, uint32_t& b1) {
+  x[0] *= f0, x[1] *= f0, x[2] *= f1, x[3] *= f1;
+  if (!all) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (!(seen[j] & 1u)) x[j] = -INFINITY;
+      if (!(seen[j] & 2u)) x[2 + j] = -INFINITY;
+    }
+  }
+  const float top0 = fmaxf(x[0], x[2]), top1 = fmaxf(x[1], x[3]);
+  if (__any_sync(0xffffffffu, top0 > st.m[rt][0] + kReferenceSlack || top1 > st.m[rt][1] + kReferenceSlack)) {
+    float top[2] = {top0, top1};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
+      const float ref = fmaxf(st.m[rt][j], top[j]);
+      const float keep = exp2_approx(st.m[rt][j] - ref);
+      st.m[rt][j] = ref;
+      st.l[rt][j] *= keep;
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) {
+        st.o[s][rt][j] *= keep;
+        st.o[s][rt][2 + j] *= keep;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = exp2_approx(x[i] - st.m[rt][i & 1]);
+  if (kScaled) {
+    st.l[rt][0] += x[0] + x[2];
+    st.l[rt][1] += x[1] + x[3];
+    x[0] *= w0, x[1] *= w0, x[2] *= w1, x[3] *= w1;
+    b0 = pack_bf16(x[0], x[1]);
+    b1 = pack_bf16(x[2], x[3]);
+  } else {  // the sum takes the weights as they are rounded, so that the result is an exact mean of value rows
+    b0 = pack_bf16(x[0], x[1]);
+    b1 = pack_bf16(x[2], x[3]);
+    st.l[rt][0] += __uint_as_float(b0 << 16) + __uint_as_float(b1 << 16);
+    st.l[rt][1] += __uint_as_float(b0 & 0xffff0000u) + __uint_as_float(b1 & 0xffff0000u);
+  }
+  b0 = transpose_8x8(b0);
+  b1 = transpose_8x8(b1);
+}
+
+// ---------------------------------------------------------------- committed slots
+// This warp's rows of the tiles [tile, stop) that lie among the visible slots, 16 at a time.
+template <int kStorage, int DP, int RT>
+__device__ __forceinline__ void past_keys(const wm_pool_attn_args& a, const Piece& c, int tile, int stop, const Queries<DP, RT>& q, State<DP, RT>& st) {
+  using R = Rows<kStorage, DP>;
+  constexpr bool kScaled = kStorage != WM_BF16;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int row_bytes = a.head_dim * R::kBytes;
+  const char* k = static_cast<const char*>(a.k) + (c.b * a.k_strides[0] + c.kv_head * a.k_strides[1]) * R::kBytes;
+  const char* v = static_cast<const char*>(a.v) + (c.b * a.v_strides[0] + c.kv_head * a.v_strides[1]) * R::kBytes;
+  const long long k_row = a.k_strides[2] * R::kBytes, v_row = a.v_strides[2] * R::kBytes;
+  const float* ks = kScaled ? a.k_scales + c.b * a.k_scale_strides[0] + c.kv_head * a.k_scale_strides[1] : nullptr;
+  const float* vs = kScaled ? a.v_scales + c.b * a.v_scale_strides[0] + c.kv_head * a.v_scale_strides[1] : nullptr;
+  const uint8_t* mask = a.key_mask != nullptr ? a.key_mask + static_cast<long long>(c.b) * a.k_len : nullptr;
+  const float factor = a.scale * kLog2e;
+
+  // step i covers the 16 slots from first(i) on
+  const int steps = (stop - tile) * 2;
+  const auto first = [&](int i) { return (tile + (i >> 1)) * kTileKeys + warp * 32 + (i & 1) * 16; };
+  uint32_t kr[2][R::kKeyWords], vr[4][R::kValueWords];
+  float kscale[2], vscale[2];
+  bool open = true;  // the mask keeps slot first(i) + lane
+
+  const auto load_k = [&](int j0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int j = j0 + g + 8 * h;
+      const bool live = j < c.slots;
+      R::load_key(kr[h], k + j * k_row, t, row_bytes, live);
+      if (kScaled) {
+        kscale[h] = live ? ks[j * a.k_scale_strides[2]] : 0.f;
+        vscale[h] = live ? vs[j * a.v_scale_strides[2]] : 0.f;
+      }
+    }
+    if (mask != nullptr) open = lane < 16 && j0 + lane < c.slots && mask[j0 + lane] != 0;
+  };
+  const auto load_v = [&](int j0) {
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const int j = j0 + 2 * t + (h & 1) + (h & 2) * 4;
+      R::load_value(vr[h], v + j * v_row, g, row_bytes, j < c.slots);
+    }
+  };
+
+  int i = 0;
+  if (steps > 0 && first(0) < c.slots) {
+    load_k(first(0));
+    load_v(first(0));
+  }
+  for (; i < steps && first(i) < c.slots; ++i) {
+    const int j0 = first(i), next = i + 1 < steps ? first(i + 1) : c.slots;
+    const int room = c.slots - j0;
+    uint32_t word = room >= 16 ? 0xffffu : (1u << room) - 1u;
+    if (mask != nullptr) word = __ballot_sync(0xffffffffu, open);
+    const bool all = word == 0xffffu;
+    const uint32_t mine = (word >> g & 1u) | (word >> (g + 8) & 1u) << 1;
+    const uint32_t seen[2] = {mine, mine};
+    float f0 = factor, f1 = factor, w0 = 1.f, w1 = 1.f;
+    if (kScaled) {
+      f0 = factor * kscale[0], f1 = factor * kscale[1], w0 = vscale[0], w1 = vscale[1];
+      if (!all) {
+        if (!(mine & 1u)) f0 = 0.f, w0 = 0.f;
+        if (!(mine & 2u)) f1 = 0.f, w1 = 0.f;
+      }
+    }
+    uint32_t ka[DP / 16][4];
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) R::template key_fragment<false>(ka[s], kr[0], kr[1], s);
+    if (next < c.slots) load_k(next);
+    uint32_t pb[RT][2];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) {
+        const uint2 b = q.get(rt, s);
+        mma_16816(x, ka[s][0], ka[s][1], ka[s][2], ka[s][3], b.x, b.y);
+      }
+      weights<DP, RT, kScaled>(st, rt, x, f0, f1, w0, w1, all, seen, pb[rt][0], pb[rt][1]);
+    }
+    if (!all) {  // what a masked slot holds must not meet its zero weight
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+        if (!(word >> (2 * t + (h & 1) + (h & 2) * 4) & 1u)) {
+#pragma unroll
+          for (int w = 0; w < R::kValueWords; ++w) vr[h][w] = 0;
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+      uint32_t va[4];
+      R::value_fragment(va, vr, s);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) mma_16816(st.o[s][rt], va[0], va[1], va[2], va[3], pb[rt][0], pb[rt][1]);
+    }
+    if (next < c.slots) load_v(next);
+  }
+}
+
+// ---------------------------------------------------------------- drafted tokens
+template <int kStorage, int DP, int RT>
+__device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Plan& plan, const Piece& c, int tile, int stop, const Queries<DP, RT>& q, State<DP, RT>& st) {
+  using R = Rows<WM_BF16, DP>;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int row_bytes = a.head_dim * 2, nodes = a.q_len, words = (nodes + 31) / 32;
+  const char* k = static_cast<const char*>(a.draft_k) + (c.b * a.draft_k_strides[0] + c.kv_head * a.draft_k_strides[1]) * 2;
+  const char* v = static_cast<const char*>(a.draft_v) + (c.b * a.draft_v_strides[0] + c.kv_head * a.draft_v_strides[1]) * 2;
+  const long long tree = a.shared_tree ? 0 : static_cast<long long>(c.b) * nodes;
+  const float factor = a.scale * kLog2e;
+#pragma unroll 1
+  for (int i = 0; i < (stop - tile) * 2; ++i) {
+    const int j0 = (tile + (i >> 1)) * kTileKeys + warp * 32 + (i & 1) * 16;
+    if (j0 >= nodes) break;
+    uint32_t kr[2][R::kKeyWords], vr[4][R::kValueWords];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int j = j0 + g + 8 * h;
+      R::load_key(kr[h], k + j * a.draft_k_strides[2] * 2, t, row_bytes, j < nodes);
+    }
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const int j = j0 + 2 * t + (h & 1) + (h & 2) * 4;
+      R::load_value(vr[h], v + j * a.draft_v_strides[2] * 2, g, row_bytes, j < nodes);
+    }
+    const bool real = lane < 16 && j0 + lane < nodes && a.depths[tree + j0 + lane] >= 0;
+    const uint32_t usable = __ballot_sync(0xffffffffu, real);  // padding nodes may hold anything
+    uint32_t special = 0;
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+#pragma unroll
+      for (int w = 0; w < R::kValueWords; ++w) {
+        if (!(usable >> (2 * t + (h & 1) + (h & 2) * 4) & 1u)) vr[h][w] = 0;
+        special |= (vr[h][w] & 0x7f80u) == 0x7f80u || (vr[h][w] & 0x7f800000u) == 0x7f800000u;
+      }
+    special = __any_sync(0xffffffffu, special);
+    uint32_t ka[DP / 16][4];
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) R::template key_fragment<kStorage != WM_BF16>(ka[s], kr[0], kr[1], s);
+    uint32_t pb[RT][2], sees[RT][2];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      uint32_t seen[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        int token, head;
+        row_place(a, c, plan, rt * 8 + 2 * t + j, token, head);
+        sees[rt][j] = token < nodes ? a.ancestors[(tree + token) * words + (j0 >> 5)] >> (j0 & 31) & usable : 0u;
+        seen[j] = (sees[rt][j] >> g & 1u) | (sees[rt][j] >> (g + 8) & 1u) << 1;
+      }
+      float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) {
+        const uint2 b = q.get(rt, s);
+        mma_16816(x, ka[s][0], ka[s][1], ka[s][2], ka[s][3], b.x, b.y);
+      }
+      weights<DP, RT, false>(st, rt, x, factor, factor, 1.f, 1.f, false, seen, pb[rt][0], pb[rt][1]);
+    }
+    if (!special) {
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) {
+        uint32_t va[4];
+        R::value_fragment(va, vr, s);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) mma_16816(st.o[s][rt], va[0], va[1], va[2], va[3], pb[rt][0], pb[rt][1]);
+      }
+    } else {  // an infinity or NaN among the values reaches the rows that see it and no others: row by row
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll 1
+        for (int r = 0; r < 8; ++r) {
+          const uint32_t row_sees = __shfl_sync(0xffffffffu, r & 1 ? sees[rt][1] : sees[rt][0], r >> 1);
+          uint32_t one[4][R::kValueWords];
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+#pragma unroll
+            for (int w = 0; w < R::kValueWords; ++w) one[h][w] = row_sees >> (2 * t + (h & 1) + (h & 2) * 4) & 1u ? vr[h][w] : 0u;
+          const uint32_t b0 = g == r ? pb[rt][0] : 0u, b1 = g == r ? pb[rt][1] : 0u;
+#pragma unroll
+          for (int s = 0; s < DP / 16; ++s) {
+            uint32_t va[4];
+            R::value_fragment(va, one, s);
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_16816(x, va[0], va[1], va[2], va[3], b0, b1);
+            // the other columns hold 0 * infinity: only this row's is taken
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st.o[s][rt][e] += 2 * t + (e & 1) == r ? x[e] : 0.f;
+          }
+        }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- kernel
+// Blocks of 128 threads that fit an SM together, from the registers that the accumulators, the rows in flight and the
+// queries take; the launch holds the compiler to it.
+template <int kStorage, int DP, int RT>
+constexpr int resident_blocks() {
+  return DP > 64 ? (RT == 1 ? 4 : RT == 2 ? 3 : 2) : (RT == 1 ? 5 : RT == 2 ? 4 : RT == 4 ? 3 : 2);
+}
+
+template <int kStorage, int DP, int RT>
+__global__ void __launch_bounds__(kThreads, resident_blocks<kStorage, DP, RT>()) pool_attn_mma_kernel(const wm_pool_attn_args a, const Plan plan) {
+  constexpr int kRows = RT * 8, kPitch = DP + 4;
+  __shared__ __align__(16) float sm_acc[kRows][kPitch];
+  __shared__ float sm_m[kWarps][kRows], sm_l[kWarps][kRows];
+  __shared__ uint2 sm_q[Queries<DP, RT>::kShared ? RT * (DP / 16) * 32 : 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  Share share = find_share(a, plan, blockIdx.x, gridDim.x);
+  for (long long at = share.begin; at < share.end;) {
+    const Piece c = next_piece(a, plan, at, share.end, share.b, share.b_begin);
+    at += c.stop - c.tile;
+
+    Queries<DP, RT> q;
+    q.shared = sm_q;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      int token, head;
+      row_place(a, c, plan, rt * 8 + g, token, head);
+      const bool live = token < a.q_len;
+      const char* row = static_cast<const char*>(a.q) + (live ? (c.b * a.q_strides[0] + head * a.q_strides[1] + token * a.q_strides[2]) * 2 : 0);
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) {
+        if (Queries<DP, RT>::kShared && ((rt * (DP / 16) + s) % kWarps) != warp) continue;
+        const int e = t * (DP / 4) + 4 * s;
+        uint2 x = make_uint2(0, 0);
+        if (live && e < a.head_dim) x = *reinterpret_cast<const uint2*>(row + 2 * e);
+        if (kStorage != WM_BF16) x = make_uint2(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632));
+        if (Queries<DP, RT>::kShared)
+          sm_q[(rt * (DP / 16) + s) * 32 + lane] = x;
+        else
+          q.reg[Queries<DP, RT>::kShared ? 0 : rt][Queries<DP, RT>::kShared ? 0 : s] = x;
+      }
+    }
+    State<DP, RT> st;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) st.m[rt][j] = kNoReference, st.l[rt][j] = 0.f;
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st.o[s][rt][e] = 0.f;
+    }
+    if (Queries<DP, RT>::kShared) __syncthreads();
+
+    if (c.tile < c.past_tiles) past_keys<kStorage, DP, RT>(a, c, c.tile, min(c.stop, c.past_tiles), q, st);
+    if (a.ancestors != nullptr && c.stop > c.past_tiles)
+      draft_keys<kStorage, DP, RT>(a, plan, c, max(c.tile - c.past_tiles, 0), c.stop - c.past_tiles, q, st);
+
+    // join the warps: the largest reference first, then the sums one warp after another
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (g == 0) sm_m[warp][rt * 8 + 2 * t + j] = st.m[rt][j];
+    __syncthreads();
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = rt * 8 + 2 * t + j;
+        float top = sm_m[0][r];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm_m[w][r]);
+        const float f = exp2_approx(st.m[rt][j] - top);
+        float l = st.l[rt][j];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (g == 0) sm_l[warp][r] = l * f;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+          st.o[s][rt][j] *= f;
+          st.o[s][rt][2 + j] *= f;
+        }
+      }
+#pragma unroll 1
+    for (int w = 0; w < kWarps; ++w) {
+      if (w == warp) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float2* p = reinterpret_cast<float2*>(&sm_acc[rt * 8 + 2 * t + j][g * (DP / 8) + 2 * s]);
+              float2 y = make_float2(st.o[s][rt][j], st.o[s][rt][2 + j]);
+              if (w > 0) {
+                const float2 z = *p;
+                y.x += z.x;
+                y.y += z.y;
+              }
+              *p = y;
+            }
+      }
+      __syncthreads();
+    }
+    const int pairs = a.head_dim / 2;
+    for (int i = threadIdx.x; i < kRows * pairs; i += kThreads) {
+      const int r = i / pairs, d = 2 * (i - r * pairs);
+      int token, head;
+      row_place(a, c, plan, r, token, head);
+      if (token >= a.q_len) continue;
+      float l = 0.f, top = sm_m[0][r];
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        l += sm_l[w][r];
+        top = fmaxf(top, sm_m[w][r]);
+      }
+      float2 y = *reinterpret_cast<const float2*>(&sm_acc[r][d]);
+      if (a.depths != nullptr && a.depths[(a.shared_tree ? 0ll : static_cast<long long>(c.b) * a.q_len) + token] < 0) {  // a padding node sees nothing
+        l = 0.f;
+        y = make_float2(0.f, 0.f);
+      }
+      if (whole(c)) {
+        const float inverse = l == 0.f ? 0.f : 1.f / l;
+        const long long place = c.b * a.out_strides[0] + head * a.out_strides[1] + token * a.out_strides[2] + d;
+        // 0 * infinity: a row without weights is zero whatever its sums are
+        *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + place) = l == 0.f ? 0u : pack_bf16(y.x * inverse, y.y * inverse);
+      } else {
+        float* row = partial_row(static_cast<float*>(a.workspace), a, plan, blockIdx.x, c.tile == 0, r);
+        if (d == 0) *reinterpret_cast<float2*>(row) = make_float2(top, l);
+        *reinterpret_cast<float2*>(row + 2 + d) = y;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <int kStorage, int DP>
+void launch_mma_rows(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream) {
+  switch (plan.rows_per_block) {
+    case 8: pool_attn_mma_kernel<kStorage, DP, 1><<<shares, kThreads, 0, stream>>>(a, plan); break;
+    case 16: pool_attn_mma_kernel<kStorage, DP, 2><<<shares, kThreads, 0, stream>>>(a, plan); break;
+    case 32: pool_attn_mma_kernel<kStorage, DP, 4><<<shares, kThreads, 0, stream>>>(a, plan); break;
+    default:
+      if constexpr (DP <= 64) pool_attn_mma_kernel<kStorage, DP, 8><<<shares, kThreads, 0, stream>>>(a, plan);
+  }
+}
+
+template <int kStorage>
+void launch_mma_storage(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream) {
+  if (a.head_dim <= 32)
+    launch_mma_rows<kStorage, 32>(a, plan, shares, stream);
+  else if (a.head_dim <= 64)
+    launch_mma_rows<kStorage, 64>(a, plan, shares, stream);
+  else if (a.head_dim <= 96)
+    launch_mma_rows<kStorage, 96>(a, plan, shares, stream);
+  else
+    launch_mma_rows<kStorage, 128>(a, plan, shares, stream);
+}
+
+// One translation unit per way of holding the pool.
+void launch_mma_bf16(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream);
+void launch_mma_int8(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream);
+void launch_mma_e4m3(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream);
+
+// Rows of a block: as many tiles of 8 as the rows of a KV head fill, up to what the registers hold.
+inline int mma_rows_per_block(long long rows, int head_dim) {
+  const int most = head_dim <= 64 ? 64 : 32;
+  int n = 8;
+  while (n < most && n < rows) n *= 2;
+  return n;
+}
+
+inline int mma_resident_blocks(int rows_per_block, int head_dim) {
+  return head_dim > 64 ? (rows_per_block == 8 ? 4 : rows_per_block == 16 ? 3 : 2) : (rows_per_block == 8 ? 5 : rows_per_block == 16 ? 4 : rows_per_block == 32 ? 3 : 2);
+}
+
+}  // namespace pool
+}  // namespace wm
