@@ -252,6 +252,8 @@ int validate(const wm_pool_attn_args& a, Plan& plan) {
   if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.q_strides, wide) || !aligned16(a.k_strides, held) || !aligned16(a.v_strides, held) ||
       (have != 0 && (!aligned16(a.draft_k) || !aligned16(a.draft_v) || !aligned16(a.draft_k_strides, wide) || !aligned16(a.draft_v_strides, wide))))
     return fail(WM_EUNSUPPORTED, "%s: rows must be 16-byte aligned", who);
+  for (const int64_t* strides : {a.k_strides, a.v_strides, a.k_scale_strides, a.v_scale_strides})
+    if (strides[2] < 0 || strides[2] >= 1 << 24) return fail(WM_EUNSUPPORTED, "%s: pool rows must be less than 2^24 elements apart", who);
   if (!make_plan(a, plan)) return fail(WM_EUNSUPPORTED, "%s: too many query rows", who);
   return WM_OK;
 }

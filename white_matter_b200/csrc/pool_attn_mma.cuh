@@ -50,12 +50,9 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
   return y;
 }
-// kBytes (4, 8 or 16) of a pool row, zeros where `live` is false; read once, so kept out of L1
+// kBytes (4, 8 or 16) of a pool row; read once, so kept out of L1
 template <int kBytes>
-__device__ __forceinline__ void load_row(uint32_t* r, const char* p, bool live) {
-#pragma unroll
-  for (int i = 0; i < kBytes / 4; ++i) r[i] = 0;
-  if (!live) return;
+__device__ __forceinline__ void load_row(uint32_t* r, const char* p) {
   if (kBytes == 16)
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[kBytes / 4 > 1]), "=r"(r[kBytes / 4 > 2 ? 2 : 0]), "=r"(r[kBytes / 4 > 3 ? 3 : 0]) : "l"(p));
   else if (kBytes == 8)
@@ -105,20 +102,19 @@ struct Rows {
   static constexpr int kKeyUnit = kKeyBytes % 16 ? 8 : 16;
   static constexpr int kValueUnit = kValueBytes % 16 == 0 ? 16 : (kValueBytes % 8 == 0 ? 8 : 4);
 
-  // A row has row_bytes (a multiple of 16) of the DP elements; what lies behind them counts as zeros.
-  __device__ static void load_key(uint32_t (&r)[kKeyWords], const char* row, int t, int row_bytes, bool live) {
+  // Where the piece of lane t (key rows) or g (value rows) starts.  A row of fewer than DP elements (row_bytes, a multiple of
+  // 16) has no whole piece for its last lanes: they read the last piece of the row instead.  What two lanes read then
+  // counts once, for the lower one: the queries are zero for it in the other lane, and its sums are not stored.
+  __device__ static int key_piece(int t, int row_bytes) { return min(t * kKeyBytes, row_bytes - kKeyBytes); }
+  __device__ static int value_piece(int g, int row_bytes) { return min(g * kValueBytes, row_bytes - kValueBytes); }
+
+  __device__ static void load_key(uint32_t (&r)[kKeyWords], const char* piece) {
 #pragma unroll
-    for (int i = 0; i < kKeyBytes / kKeyUnit; ++i) {
-      const int at = t * kKeyBytes + i * kKeyUnit;
-      load_row<kKeyUnit>(r + i * kKeyUnit / 4, row + at, live && at < row_bytes);
-    }
+    for (int i = 0; i < kKeyBytes / kKeyUnit; ++i) load_row<kKeyUnit>(r + i * kKeyUnit / 4, piece + i * kKeyUnit);
   }
-  __device__ static void load_value(uint32_t (&r)[kValueWords], const char* row, int g, int row_bytes, bool live) {
+  __device__ static void load_value(uint32_t (&r)[kValueWords], const char* piece) {
 #pragma unroll
-    for (int i = 0; i < kValueBytes / kValueUnit; ++i) {
-      const int at = g * kValueBytes + i * kValueUnit;
-      load_row<kValueUnit>(r + i * kValueUnit / 4, row + at, live && at < row_bytes);
-    }
+    for (int i = 0; i < kValueBytes / kValueUnit; ++i) load_row<kValueUnit>(r + i * kValueUnit / 4, piece + i * kValueUnit);
   }
   // Fragment s (16 of head_dim) of K: elements 4s .. 4s + 3 of the piece.  8-bit pools take them in the order 0, 2, 1, 3,
   // which is how a word of codes comes apart; kPermute gives bf16 rows the same order.
@@ -172,6 +168,23 @@ struct Queries {
   const uint2* shared;
   __device__ uint2 get(int rt, int s) const { return kShared ? shared[(rt * (DP / 16) + s) * 32 + (threadIdx.x & 31)] : reg[kShared ? 0 : rt][kShared ? 0 : s]; }
 };
+
+// Products of 16 keys with the queries of every tile: S^T, keys g and g + 8 in the rows of x.
+template <int kStorage, int DP, int RT, bool kPermute>
+__device__ __forceinline__ void scores(const uint32_t (&kr)[2][Rows<kStorage, DP>::kKeyWords], const Queries<DP, RT>& q, float (&x)[RT][4]) {
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) x[rt][0] = x[rt][1] = x[rt][2] = x[rt][3] = 0.f;
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    uint32_t ka[4];
+    Rows<kStorage, DP>::template key_fragment<kPermute>(ka, kr[0], kr[1], s);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const uint2 b = q.get(rt, s);
+      mma_16816(x[rt], ka[0], ka[1], ka[2], ka[3], b.x, b.y);
+    }
+  }
+}
 
 // Weights of 16 keys for tile rt, as the B operand of O^T += V^T P^T.  `x` holds the scores' products with the queries
 // (keys g: x[0], x[1]; g + 8: x[2], x[3]; rows 2t, 2t + 1), f0 / f1 what they are multiplied by, w0 / w1 the value scales;
@@ -231,50 +244,54 @@ __device__ __forceinline__ void past_keys(const wm_pool_attn_args& a, const Piec
   constexpr bool kScaled = kStorage != WM_BF16;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int row_bytes = a.head_dim * R::kBytes;
-  const char* k = static_cast<const char*>(a.k) + (c.b * a.k_strides[0] + c.kv_head * a.k_strides[1]) * R::kBytes;
-  const char* v = static_cast<const char*>(a.v) + (c.b * a.v_strides[0] + c.kv_head * a.v_strides[1]) * R::kBytes;
-  const long long k_row = a.k_strides[2] * R::kBytes, v_row = a.v_strides[2] * R::kBytes;
-  const float* ks = kScaled ? a.k_scales + c.b * a.k_scale_strides[0] + c.kv_head * a.k_scale_strides[1] : nullptr;
-  const float* vs = kScaled ? a.v_scales + c.b * a.v_scale_strides[0] + c.kv_head * a.v_scale_strides[1] : nullptr;
-  const uint8_t* mask = a.key_mask != nullptr ? a.key_mask + static_cast<long long>(c.b) * a.k_len : nullptr;
   const float factor = a.scale * kLog2e;
 
-  // step i covers the 16 slots from first(i) on
-  const int steps = (stop - tile) * 2;
-  const auto first = [&](int i) { return (tile + (i >> 1)) * kTileKeys + warp * 32 + (i & 1) * 16; };
+  // Step i covers the 16 slots from first + i * kStepKeys on.  Addresses are a base that moves with the steps and offsets of
+  // the lane that stay: launches refuse pools whose 16 rows would not fit 32-bit offsets.
+  constexpr int kStepKeys = 16 * kWarps;
+  int j0 = tile * kTileKeys + warp * 16;
+  const int end = min(c.slots, stop * kTileKeys);
+  if (j0 >= end) return;
+  const uint32_t k_row = static_cast<uint32_t>(a.k_strides[2]) * R::kBytes, v_row = static_cast<uint32_t>(a.v_strides[2]) * R::kBytes;
+  const uint32_t ks_row = static_cast<uint32_t>(a.k_scale_strides[2]), vs_row = static_cast<uint32_t>(a.v_scale_strides[2]);
+  const char* k = static_cast<const char*>(a.k) + (c.b * a.k_strides[0] + c.kv_head * a.k_strides[1] + j0 * a.k_strides[2]) * R::kBytes;
+  const char* v = static_cast<const char*>(a.v) + (c.b * a.v_strides[0] + c.kv_head * a.v_strides[1] + j0 * a.v_strides[2]) * R::kBytes;
+  const float* ks = kScaled ? a.k_scales + c.b * a.k_scale_strides[0] + c.kv_head * a.k_scale_strides[1] + j0 * a.k_scale_strides[2] : nullptr;
+  const float* vs = kScaled ? a.v_scales + c.b * a.v_scale_strides[0] + c.kv_head * a.v_scale_strides[1] + j0 * a.v_scale_strides[2] : nullptr;
+  const uint8_t* mask = a.key_mask != nullptr ? a.key_mask + static_cast<long long>(c.b) * a.k_len : nullptr;
+  const uint32_t k_piece = R::key_piece(t, row_bytes), v_piece = R::value_piece(g, row_bytes);
+
   uint32_t kr[2][R::kKeyWords], vr[4][R::kValueWords];
   float kscale[2], vscale[2];
-  bool open = true;  // the mask keeps slot first(i) + lane
+  bool open = true;  // the mask keeps slot lane of the step
 
-  const auto load_k = [&](int j0) {
+  // Rows behind the last visible slot are not read: the last one takes their place, with weight zero.
+  const auto load_k = [&](int j) {
+    const int last = c.slots - 1 - j;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int j = j0 + g + 8 * h;
-      const bool live = j < c.slots;
-      R::load_key(kr[h], k + j * k_row, t, row_bytes, live);
+      const uint32_t row = last >= 15 ? g + 8 * h : min(g + 8 * h, last);
+      R::load_key(kr[h], k + (row * k_row + k_piece));
       if (kScaled) {
-        kscale[h] = live ? ks[j * a.k_scale_strides[2]] : 0.f;
-        vscale[h] = live ? vs[j * a.v_scale_strides[2]] : 0.f;
+        kscale[h] = ks[row * ks_row];
+        vscale[h] = vs[row * vs_row];
       }
     }
-    if (mask != nullptr) open = lane < 16 && j0 + lane < c.slots && mask[j0 + lane] != 0;
+    if (mask != nullptr) open = lane <= min(last, 15) && mask[j + lane] != 0;
   };
-  const auto load_v = [&](int j0) {
+  const auto load_v = [&](int j) {
+    const int last = c.slots - 1 - j;
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
-      const int j = j0 + 2 * t + (h & 1) + (h & 2) * 4;
-      R::load_value(vr[h], v + j * v_row, g, row_bytes, j < c.slots);
+      const uint32_t in = 2 * t + (h & 1) + (h & 2) * 4, row = last >= 15 ? in : min(static_cast<int>(in), last);
+      R::load_value(vr[h], v + (row * v_row + v_piece));
     }
   };
 
-  int i = 0;
-  if (steps > 0 && first(0) < c.slots) {
-    load_k(first(0));
-    load_v(first(0));
-  }
-  for (; i < steps && first(i) < c.slots; ++i) {
-    const int j0 = first(i), next = i + 1 < steps ? first(i + 1) : c.slots;
-    const int room = c.slots - j0;
+  load_k(j0);
+  load_v(j0);
+  for (;;) {
+    const int next = j0 + kStepKeys, room = c.slots - j0;
     uint32_t word = room >= 16 ? 0xffffu : (1u << room) - 1u;
     if (mask != nullptr) word = __ballot_sync(0xffffffffu, open);
     const bool all = word == 0xffffu;
@@ -288,21 +305,19 @@ __device__ __forceinline__ void past_keys(const wm_pool_attn_args& a, const Piec
         if (!(mine & 2u)) f1 = 0.f, w1 = 0.f;
       }
     }
-    uint32_t ka[DP / 16][4];
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) R::template key_fragment<false>(ka[s], kr[0], kr[1], s);
-    if (next < c.slots) load_k(next);
+    float x[RT][4];
+    scores<kStorage, DP, RT, false>(kr, q, x);
+    if (next < end) {
+      k += kStepKeys * a.k_strides[2] * R::kBytes;
+      if (kScaled) {
+        ks += kStepKeys * a.k_scale_strides[2];
+        vs += kStepKeys * a.v_scale_strides[2];
+      }
+      load_k(next);
+    }
     uint32_t pb[RT][2];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < DP / 16; ++s) {
-        const uint2 b = q.get(rt, s);
-        mma_16816(x, ka[s][0], ka[s][1], ka[s][2], ka[s][3], b.x, b.y);
-      }
-      weights<DP, RT, kScaled>(st, rt, x, f0, f1, w0, w1, all, seen, pb[rt][0], pb[rt][1]);
-    }
+    for (int rt = 0; rt < RT; ++rt) weights<DP, RT, kScaled>(st, rt, x[rt], f0, f1, w0, w1, all, seen, pb[rt][0], pb[rt][1]);
     if (!all) {  // what a masked slot holds must not meet its zero weight
 #pragma unroll
       for (int h = 0; h < 4; ++h)
@@ -318,7 +333,10 @@ __device__ __forceinline__ void past_keys(const wm_pool_attn_args& a, const Piec
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) mma_16816(st.o[s][rt], va[0], va[1], va[2], va[3], pb[rt][0], pb[rt][1]);
     }
-    if (next < c.slots) load_v(next);
+    if (next >= end) break;
+    v += kStepKeys * a.v_strides[2] * R::kBytes;
+    load_v(next);
+    j0 = next;
   }
 }
 
@@ -328,25 +346,19 @@ __device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Pla
   using R = Rows<WM_BF16, DP>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int row_bytes = a.head_dim * 2, nodes = a.q_len, words = (nodes + 31) / 32;
-  const char* k = static_cast<const char*>(a.draft_k) + (c.b * a.draft_k_strides[0] + c.kv_head * a.draft_k_strides[1]) * 2;
-  const char* v = static_cast<const char*>(a.draft_v) + (c.b * a.draft_v_strides[0] + c.kv_head * a.draft_v_strides[1]) * 2;
+  const char* k = static_cast<const char*>(a.draft_k) + (c.b * a.draft_k_strides[0] + c.kv_head * a.draft_k_strides[1]) * 2 + R::key_piece(t, row_bytes);
+  const char* v = static_cast<const char*>(a.draft_v) + (c.b * a.draft_v_strides[0] + c.kv_head * a.draft_v_strides[1]) * 2 + R::value_piece(g, row_bytes);
   const long long tree = a.shared_tree ? 0 : static_cast<long long>(c.b) * nodes;
   const float factor = a.scale * kLog2e;
 #pragma unroll 1
   for (int i = 0; i < (stop - tile) * 2; ++i) {
-    const int j0 = (tile + (i >> 1)) * kTileKeys + warp * 32 + (i & 1) * 16;
+    const int j0 = (tile + (i >> 1)) * kTileKeys + (i & 1) * 16 * kWarps + warp * 16;
     if (j0 >= nodes) break;
     uint32_t kr[2][R::kKeyWords], vr[4][R::kValueWords];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int j = j0 + g + 8 * h;
-      R::load_key(kr[h], k + j * a.draft_k_strides[2] * 2, t, row_bytes, j < nodes);
-    }
+    for (int h = 0; h < 2; ++h) R::load_key(kr[h], k + min(j0 + g + 8 * h, nodes - 1) * a.draft_k_strides[2] * 2);
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      const int j = j0 + 2 * t + (h & 1) + (h & 2) * 4;
-      R::load_value(vr[h], v + j * a.draft_v_strides[2] * 2, g, row_bytes, j < nodes);
-    }
+    for (int h = 0; h < 4; ++h) R::load_value(vr[h], v + min(j0 + 2 * t + (h & 1) + (h & 2) * 4, nodes - 1) * a.draft_v_strides[2] * 2);
     const bool real = lane < 16 && j0 + lane < nodes && a.depths[tree + j0 + lane] >= 0;
     const uint32_t usable = __ballot_sync(0xffffffffu, real);  // padding nodes may hold anything
     uint32_t special = 0;
@@ -358,9 +370,8 @@ __device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Pla
         special |= (vr[h][w] & 0x7f80u) == 0x7f80u || (vr[h][w] & 0x7f800000u) == 0x7f800000u;
       }
     special = __any_sync(0xffffffffu, special);
-    uint32_t ka[DP / 16][4];
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) R::template key_fragment<kStorage != WM_BF16>(ka[s], kr[0], kr[1], s);
+    float x[RT][4];
+    scores<WM_BF16, DP, RT, kStorage != WM_BF16>(kr, q, x);
     uint32_t pb[RT][2], sees[RT][2];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -372,13 +383,7 @@ __device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Pla
         sees[rt][j] = token < nodes ? a.ancestors[(tree + token) * words + (j0 >> 5)] >> (j0 & 31) & usable : 0u;
         seen[j] = (sees[rt][j] >> g & 1u) | (sees[rt][j] >> (g + 8) & 1u) << 1;
       }
-      float x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < DP / 16; ++s) {
-        const uint2 b = q.get(rt, s);
-        mma_16816(x, ka[s][0], ka[s][1], ka[s][2], ka[s][3], b.x, b.y);
-      }
-      weights<DP, RT, false>(st, rt, x, factor, factor, 1.f, 1.f, false, seen, pb[rt][0], pb[rt][1]);
+      weights<DP, RT, false>(st, rt, x[rt], factor, factor, 1.f, 1.f, false, seen, pb[rt][0], pb[rt][1]);
     }
     if (!special) {
 #pragma unroll
@@ -394,15 +399,15 @@ __device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Pla
 #pragma unroll 1
         for (int r = 0; r < 8; ++r) {
           const uint32_t row_sees = __shfl_sync(0xffffffffu, r & 1 ? sees[rt][1] : sees[rt][0], r >> 1);
-          uint32_t one[4][R::kValueWords];
+          uint32_t keep[4];
 #pragma unroll
-          for (int h = 0; h < 4; ++h)
-#pragma unroll
-            for (int w = 0; w < R::kValueWords; ++w) one[h][w] = row_sees >> (2 * t + (h & 1) + (h & 2) * 4) & 1u ? vr[h][w] : 0u;
+          for (int h = 0; h < 4; ++h) keep[h] = 0u - (row_sees >> (2 * t + (h & 1) + (h & 2) * 4) & 1u);
           const uint32_t b0 = g == r ? pb[rt][0] : 0u, b1 = g == r ? pb[rt][1] : 0u;
 #pragma unroll
           for (int s = 0; s < DP / 16; ++s) {
-            uint32_t va[4];
+            uint32_t va[4], one[4][R::kValueWords];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) one[h][s] = vr[h][s] & keep[h];
             R::value_fragment(va, one, s);
             float x[4] = {0.f, 0.f, 0.f, 0.f};
             mma_16816(x, va[0], va[1], va[2], va[3], b0, b1);
@@ -423,7 +428,7 @@ constexpr int resident_blocks() {
   return DP > 64 ? (RT == 1 ? 4 : RT == 2 ? 3 : 2) : (RT == 1 ? 5 : RT == 2 ? 4 : RT == 4 ? 3 : 2);
 }
 
-template <int kStorage, int DP, int RT>
+template <int kStorage, int DP, int RT, bool kTree>
 __global__ void __launch_bounds__(kThreads, resident_blocks<kStorage, DP, RT>()) pool_attn_mma_kernel(const wm_pool_attn_args a, const Plan plan) {
   constexpr int kRows = RT * 8, kPitch = DP + 4;
   __shared__ __align__(16) float sm_acc[kRows][kPitch];
@@ -446,9 +451,9 @@ __global__ void __launch_bounds__(kThreads, resident_blocks<kStorage, DP, RT>())
 #pragma unroll
       for (int s = 0; s < DP / 16; ++s) {
         if (Queries<DP, RT>::kShared && ((rt * (DP / 16) + s) % kWarps) != warp) continue;
-        const int e = t * (DP / 4) + 4 * s;
+        const int e = Rows<WM_BF16, DP>::key_piece(t, a.head_dim * 2) / 2 + 4 * s;
         uint2 x = make_uint2(0, 0);
-        if (live && e < a.head_dim) x = *reinterpret_cast<const uint2*>(row + 2 * e);
+        if (live && e >= t * (DP / 4)) x = *reinterpret_cast<const uint2*>(row + 2 * e);
         if (kStorage != WM_BF16) x = make_uint2(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632));
         if (Queries<DP, RT>::kShared)
           sm_q[(rt * (DP / 16) + s) * 32 + lane] = x;
@@ -469,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, resident_blocks<kStorage, DP, RT>())
     if (Queries<DP, RT>::kShared) __syncthreads();
 
     if (c.tile < c.past_tiles) past_keys<kStorage, DP, RT>(a, c, c.tile, min(c.stop, c.past_tiles), q, st);
-    if (a.ancestors != nullptr && c.stop > c.past_tiles)
+    if (kTree && c.stop > c.past_tiles)
       draft_keys<kStorage, DP, RT>(a, plan, c, max(c.tile - c.past_tiles, 0), c.stop - c.past_tiles, q, st);
 
     // join the warps: the largest reference first, then the sums one warp after another
@@ -507,7 +512,9 @@ __global__ void __launch_bounds__(kThreads, resident_blocks<kStorage, DP, RT>())
           for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              float2* p = reinterpret_cast<float2*>(&sm_acc[rt * 8 + 2 * t + j][g * (DP / 8) + 2 * s]);
+              const int d = Rows<WM_BF16, DP>::value_piece(g, a.head_dim * 2) / 2 + 2 * s;
+              if (d < g * (DP / 8)) continue;  // a lower lane's
+              float2* p = reinterpret_cast<float2*>(&sm_acc[rt * 8 + 2 * t + j][d]);
               float2 y = make_float2(st.o[s][rt][j], st.o[s][rt][2 + j]);
               if (w > 0) {
                 const float2 z = *p;
@@ -532,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, resident_blocks<kStorage, DP, RT>())
         top = fmaxf(top, sm_m[w][r]);
       }
       float2 y = *reinterpret_cast<const float2*>(&sm_acc[r][d]);
-      if (a.depths != nullptr && a.depths[(a.shared_tree ? 0ll : static_cast<long long>(c.b) * a.q_len) + token] < 0) {  // a padding node sees nothing
+      if (kTree && a.depths[(a.shared_tree ? 0ll : static_cast<long long>(c.b) * a.q_len) + token] < 0) {  // a padding node sees nothing
         l = 0.f;
         y = make_float2(0.f, 0.f);
       }
@@ -551,14 +558,22 @@ __global__ void __launch_bounds__(kThreads, resident_blocks<kStorage, DP, RT>())
   }
 }
 
+template <int kStorage, int DP, int RT>
+void launch_mma(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream) {
+  if (a.ancestors != nullptr)
+    pool_attn_mma_kernel<kStorage, DP, RT, true><<<shares, kThreads, 0, stream>>>(a, plan);
+  else
+    pool_attn_mma_kernel<kStorage, DP, RT, false><<<shares, kThreads, 0, stream>>>(a, plan);
+}
+
 template <int kStorage, int DP>
 void launch_mma_rows(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream) {
   switch (plan.rows_per_block) {
-    case 8: pool_attn_mma_kernel<kStorage, DP, 1><<<shares, kThreads, 0, stream>>>(a, plan); break;
-    case 16: pool_attn_mma_kernel<kStorage, DP, 2><<<shares, kThreads, 0, stream>>>(a, plan); break;
-    case 32: pool_attn_mma_kernel<kStorage, DP, 4><<<shares, kThreads, 0, stream>>>(a, plan); break;
+    case 8: return launch_mma<kStorage, DP, 1>(a, plan, shares, stream);
+    case 16: return launch_mma<kStorage, DP, 2>(a, plan, shares, stream);
+    case 32: return launch_mma<kStorage, DP, 4>(a, plan, shares, stream);
     default:
-      if constexpr (DP <= 64) pool_attn_mma_kernel<kStorage, DP, 8><<<shares, kThreads, 0, stream>>>(a, plan);
+      if constexpr (DP <= 64) launch_mma<kStorage, DP, 8>(a, plan, shares, stream);
   }
 }
 
