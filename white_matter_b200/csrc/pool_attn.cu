@@ -95,14 +95,15 @@ __global__ void __launch_bounds__(kThreads) pool_attn_simt_kernel(const wm_pool_
   __shared__ float sm_m[kWarps][R], sm_l[kWarps][R], sm_acc[kWarps][R][LPK * 4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = lane % LPK;
   Share share = find_share(a, plan, blockIdx.x, gridDim.x);
-  for (long long at = share.begin; at < share.end;) {
+  if (threadIdx.x == 0) note_of(a, blockIdx.x)->last = -1;
+  for (int at = share.begin; at < share.end;) {
     const Piece c = next_piece(a, plan, at, share.end, share.b, share.b_begin);
     at += c.stop - c.tile;
     SimtState<R> s;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       int token, head;
-      row_place(a, c, plan, r, token, head);
+      row_place(a, plan, c.kv_head, c.row_block, r, token, head);
       s.token[r] = token < a.q_len ? token : -1;
       s.m[r] = -INFINITY;
       s.l[r] = 0.f;
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(kThreads) pool_attn_simt_kernel(const wm_pool_
     for (int i = threadIdx.x; i < R * a.head_dim; i += kThreads) {
       const int r = i / a.head_dim, d = i - r * a.head_dim;
       int token, head;
-      row_place(a, c, plan, r, token, head);
+      row_place(a, plan, c.kv_head, c.row_block, r, token, head);
       if (token >= a.q_len) continue;
       float top = -INFINITY;
 #pragma unroll
@@ -159,47 +160,51 @@ __global__ void __launch_bounds__(kThreads) pool_attn_simt_kernel(const wm_pool_
       if (whole(c)) {
         static_cast<float*>(a.out)[c.b * a.out_strides[0] + head * a.out_strides[1] + token * a.out_strides[2] + d] = l == 0.f ? 0.f : acc / l;
       } else {
-        float* row = partial_row(static_cast<float*>(a.workspace), a, plan, blockIdx.x, c.tile == 0, r);
+        float* row = partial_row(a, plan, gridDim.x, blockIdx.x, c.tile == 0, r);
         if (d == 0) row[0] = top, row[1] = l;
         row[2 + d] = acc;
       }
     }
+    if (threadIdx.x == 0) leave_note(a, share, c, blockIdx.x, gridDim.x);
     __syncthreads();
   }
 }
 
 // ---------------------------------------------------------------- joining the pieces of a segment
-// Block i joins the segment that share i leaves unfinished, if share i also began it.
+// Block i joins the segment that share i began and left unfinished, if its note names one.  Every thread keeps one row.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) pool_attn_join_kernel(const wm_pool_attn_args a, const Plan plan) {
-  const int shares = gridDim.x;
-  Share share = find_share(a, plan, blockIdx.x, shares);
-  if (share.begin >= share.end || share.end >= share.total) return;
-  int b = share.b;
-  long long b_begin = share.b_begin;
-  const Piece c = next_piece(a, plan, share.end, share.total, b, b_begin);  // the segment that the next share goes on with
-  if (c.tile == 0 || share.end - c.tile < share.begin) return;
-  const long long stop = share.end + (c.tiles - c.tile);
-  int last = blockIdx.x + 1;
-  while (share_begin(share.total, last + 1, shares) < stop) ++last;
-  float* workspace = static_cast<float*>(a.workspace);
-  for (int i = threadIdx.x; i < plan.rows_per_block * a.head_dim; i += kThreads) {
-    const int r = i / a.head_dim, d = i - r * a.head_dim;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched ahead of the first kernel's end
+  const int shares = gridDim.x, first = blockIdx.x;
+  const Note note = *note_of(a, first);
+  if (note.last < 0) return;
+  const int per_row = kThreads / min(plan.rows_per_block, 16), pairs = a.head_dim / 2;
+  for (int r = threadIdx.x / per_row; r < plan.rows_per_block; r += kThreads / per_row) {
     int token, head;
-    row_place(a, c, plan, r, token, head);
+    row_place(a, plan, note.kv_head, note.row_block, r, token, head);
     if (token >= a.q_len) continue;
-    const float* row = partial_row(workspace, a, plan, blockIdx.x, 1, r);
-    float top = row[0], l = row[1], acc = row[2 + d];
-    for (int s = blockIdx.x + 1; s <= last; ++s) {
-      if (share_begin(share.total, s, shares) == share_begin(share.total, s + 1, shares)) continue;  // an empty share
-      row = partial_row(workspace, a, plan, s, 0, r);
-      const float m = row[0], both = fmaxf(top, m), ref = both == -INFINITY ? 0.f : both;
-      const float f = exp2f(top - ref), g = exp2f(m - ref);
-      l = l * f + row[1] * g;
-      acc = acc * f + row[2 + d] * g;
-      top = both;
+    // the reference and the sum of the whole row first, by every thread of the row
+    float top = -INFINITY, l = 0.f;
+    for (int s = first; s <= note.last; ++s) top = fmaxf(top, *partial_row(a, plan, shares, s, s == first, r));
+    const float ref = top == -INFINITY ? 0.f : top;
+    for (int s = first; s <= note.last; ++s) {
+      const float2 x = *reinterpret_cast<const float2*>(partial_row(a, plan, shares, s, s == first, r));
+      l += x.y * exp2f(x.x - ref);
     }
-    static_cast<T*>(a.out)[c.b * a.out_strides[0] + head * a.out_strides[1] + token * a.out_strides[2] + d] = from_float<T>(l == 0.f ? 0.f : acc / l);
+    const float inverse = l == 0.f ? 0.f : 1.f / l;
+    T* out = static_cast<T*>(a.out) + note.b * a.out_strides[0] + head * a.out_strides[1] + token * a.out_strides[2];
+    for (int d = threadIdx.x % per_row; d < pairs; d += per_row) {
+      float2 sum = make_float2(0.f, 0.f);
+      for (int s = first; s <= note.last; ++s) {
+        const float* row = partial_row(a, plan, shares, s, s == first, r);
+        const float f = exp2f(row[0] - ref);
+        const float2 y = *reinterpret_cast<const float2*>(row + 2 + 2 * d);
+        sum.x = fmaf(y.x, f, sum.x);
+        sum.y = fmaf(y.y, f, sum.y);
+      }
+      out[2 * d] = from_float<T>(l == 0.f ? 0.f : sum.x * inverse);
+      out[2 * d + 1] = from_float<T>(l == 0.f ? 0.f : sum.y * inverse);
+    }
   }
 }
 
@@ -217,7 +222,9 @@ bool make_plan(const wm_pool_attn_args& a, Plan& p) {
   p.rows_per_block = rows_per_block(a);
   const long long blocks = (rows + p.rows_per_block - 1) / p.rows_per_block;
   p.draft_tiles = a.ancestors != nullptr ? (a.q_len + kTileKeys - 1) / kTileKeys : 0;
-  if (blocks * a.kv_heads > INT_MAX || rows > INT_MAX) return false;
+  p.group = a.q_heads / a.kv_heads;
+  const double units = (static_cast<double>(a.k_len) / kTileKeys + 1 + p.draft_tiles) * a.batch * a.kv_heads * blocks;
+  if (units >= INT_MAX || rows > INT_MAX) return false;  // the kernels count in 32 bits
   p.row_blocks = static_cast<int>(blocks);
   return true;
 }
@@ -225,7 +232,7 @@ bool make_plan(const wm_pool_attn_args& a, Plan& p) {
 // One wave: as many shares as blocks fit the GPU, and no more than there can be tiles.
 int count_shares(const wm_pool_attn_args& a, const Plan& p) {
   const double tiles = static_cast<double>((a.k_len + kTileKeys - 1) / kTileKeys + p.draft_tiles) * a.batch * a.kv_heads * p.row_blocks;
-  const int wave = kSms * (a.dtype == WM_F32 ? 6 : mma_resident_blocks(p.rows_per_block, a.head_dim));
+  const int wave = kSms * (a.dtype == WM_F32 ? 6 : resident_blocks(a.storage, p.rows_per_block / 8, a.head_dim));
   return tiles < wave ? (tiles < 1 ? 1 : static_cast<int>(tiles)) : wave;
 }
 
@@ -281,7 +288,7 @@ void launch_simt(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaS
 size_t pool_attn_workspace(const wm_pool_attn_args& a) {
   Plan plan;
   if (a.batch < 1 || a.kv_heads < 1 || a.q_heads < a.kv_heads || a.q_len < 1 || a.k_len < 1 || !make_plan(a, plan)) return 0;
-  return static_cast<size_t>(count_shares(a, plan)) * 2 * plan.rows_per_block * (a.head_dim + 2) * sizeof(float);
+  return static_cast<size_t>(count_shares(a, plan)) * (sizeof(Note) + 2 * plan.rows_per_block * (a.head_dim + 2) * sizeof(float));
 }
 
 int pool_attn_launch(const wm_pool_attn_args& a, cudaStream_t stream) {
@@ -308,12 +315,19 @@ int pool_attn_launch(const wm_pool_attn_args& a, cudaStream_t stream) {
   count_launch();
   WM_CUDA(cudaGetLastError());
   if (shares == 1) return WM_OK;
-  if (a.dtype == WM_F32)
-    pool_attn_join_kernel<float><<<shares, kThreads, 0, stream>>>(a, plan);
-  else
-    pool_attn_join_kernel<__nv_bfloat16><<<shares, kThreads, 0, stream>>>(a, plan);
+  cudaLaunchAttribute early = {};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(shares);
+  config.blockDim = dim3(kThreads);
+  config.stream = stream;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  const cudaError_t status_join = a.dtype == WM_F32 ? cudaLaunchKernelEx(&config, pool_attn_join_kernel<float>, a, plan)
+                                                    : cudaLaunchKernelEx(&config, pool_attn_join_kernel<__nv_bfloat16>, a, plan);
   count_launch();
-  return cuda_check(cudaGetLastError(), "pool_attn_join_kernel");
+  return cuda_check(status_join, "pool_attn_join_kernel");
 }
 
 }  // namespace wm

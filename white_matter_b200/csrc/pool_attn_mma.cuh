@@ -186,23 +186,33 @@ __device__ __forceinline__ void scores(const uint32_t (&kr)[2][Rows<kStorage, DP
   }
 }
 
-// Weights of 16 keys for tile rt, as the B operand of O^T += V^T P^T.  `x` holds the scores' products with the queries
-// (keys g: x[0], x[1]; g + 8: x[2], x[3]; rows 2t, 2t + 1), f0 / f1 what they are multiplied by, w0 / w1 the value scales;
-// seen[j] bit 0 / 1: row 2t + j sees key g / g + 8.
-template <int DP, int RT, bool kScaled>
-__device__ __forceinline__ void weights(State<DP, RT>& st, int rt, float (&x)[4], float f0, float f1, float w0, float w1, bool all, const uint32_t (&seen)[2],
-                                        uint32_t& b0, uint32_t& b1) {
-  x[0] *= f0, x[1] *= f0, x[2] *= f1, x[3] *= f1;
-  if (!all) {
+// What 16 keys bring along: factor of the score and scale of the value for keys g and g + 8, which of them the rows see
+// (bit 0 / 1 of seen[j]: row 2t + j sees key g / g + 8), and whether every row sees all 16.
+struct Keys {
+  float factor[2], scale[2];
+  uint32_t seen[2];
+  bool all;
+};
+
+// Weights of U x 16 keys for tile rt, as B operands of O^T += V^T P^T.  x holds the keys' products with the queries (keys
+// g: x[.][0], x[.][1]; g + 8: x[.][2], x[.][3]; rows 2t, 2t + 1).
+template <int DP, int RT, int U, bool kScaled>
+__device__ __forceinline__ void weights(State<DP, RT>& st, int rt, float (&x)[U][RT][4], const Keys (&keys)[U], uint32_t (&pb)[U][RT][2]) {
+  float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if (!(seen[j] & 1u)) x[j] = -INFINITY;
-      if (!(seen[j] & 2u)) x[2 + j] = -INFINITY;
+  for (int u = 0; u < U; ++u) {
+    float(&y)[4] = x[u][rt];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] *= keys[u].factor[e >> 1];
+    if (!keys[u].all) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (!(keys[u].seen[e & 1] >> (e >> 1) & 1u)) y[e] = -INFINITY;
     }
+    top[0] = fmaxf(top[0], fmaxf(y[0], y[2]));
+    top[1] = fmaxf(top[1], fmaxf(y[1], y[3]));
   }
-  const float top0 = fmaxf(x[0], x[2]), top1 = fmaxf(x[1], x[3]);
-  if (__any_sync(0xffffffffu, top0 > st.m[rt][0] + kReferenceSlack || top1 > st.m[rt][1] + kReferenceSlack)) {
-    float top[2] = {top0, top1};
+  if (__any_sync(0xffffffffu, top[0] > st.m[rt][0] + kReferenceSlack || top[1] > st.m[rt][1] + kReferenceSlack)) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -219,37 +229,46 @@ __device__ __forceinline__ void weights(State<DP, RT>& st, int rt, float (&x)[4]
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = exp2_approx(x[i] - st.m[rt][i & 1]);
-  if (kScaled) {
-    st.l[rt][0] += x[0] + x[2];
-    st.l[rt][1] += x[1] + x[3];
-    x[0] *= w0, x[1] *= w0, x[2] *= w1, x[3] *= w1;
-    b0 = pack_bf16(x[0], x[1]);
-    b1 = pack_bf16(x[2], x[3]);
-  } else {  // the sum takes the weights as they are rounded, so that the result is an exact mean of value rows
-    b0 = pack_bf16(x[0], x[1]);
-    b1 = pack_bf16(x[2], x[3]);
-    st.l[rt][0] += __uint_as_float(b0 << 16) + __uint_as_float(b1 << 16);
-    st.l[rt][1] += __uint_as_float(b0 & 0xffff0000u) + __uint_as_float(b1 & 0xffff0000u);
+  for (int u = 0; u < U; ++u) {
+    float(&y)[4] = x[u][rt];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = exp2_approx(y[e] - st.m[rt][e & 1]);
+    if (kScaled) {
+      st.l[rt][0] += y[0] + y[2];
+      st.l[rt][1] += y[1] + y[3];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] *= keys[u].scale[e >> 1];
+    }
+    const uint32_t b0 = pack_bf16(y[0], y[1]), b1 = pack_bf16(y[2], y[3]);
+    if (!kScaled) {  // the sum takes the weights as they are rounded, so that the result is an exact mean of value rows
+      st.l[rt][0] += __uint_as_float(b0 << 16) + __uint_as_float(b1 << 16);
+      st.l[rt][1] += __uint_as_float(b0 & 0xffff0000u) + __uint_as_float(b1 & 0xffff0000u);
+    }
+    pb[u][rt][0] = transpose_8x8(b0);
+    pb[u][rt][1] = transpose_8x8(b1);
   }
-  b0 = transpose_8x8(b0);
-  b1 = transpose_8x8(b1);
 }
 
 // ---------------------------------------------------------------- committed slots
-// This warp's rows of the tiles [tile, stop) that lie among the visible slots, 16 at a time.
+// Steps of 16 U keys per warp: two groups of 16 where the registers hold their rows (bytes in flight), one elsewhere.
+template <int kStorage, int DP, int RT>
+__host__ __device__ constexpr int groups_per_step() {
+  return RT <= 2 && DP * Codes<kStorage>::kBytes <= 64 ? 2 : 1;
+}
+
+// This warp's rows of the tiles [tile, stop) that lie among the visible slots.
 template <int kStorage, int DP, int RT>
 __device__ __forceinline__ void past_keys(const wm_pool_attn_args& a, const Piece& c, int tile, int stop, const Queries<DP, RT>& q, State<DP, RT>& st) {
   using R = Rows<kStorage, DP>;
   constexpr bool kScaled = kStorage != WM_BF16;
+  constexpr int U = groups_per_step<kStorage, DP, RT>(), kGroup = 16 * U, kStepKeys = kGroup * kWarps;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int row_bytes = a.head_dim * R::kBytes;
   const float factor = a.scale * kLog2e;
 
-  // Step i covers the 16 slots from first + i * kStepKeys on.  Addresses are a base that moves with the steps and offsets of
-  // the lane that stay: launches refuse pools whose 16 rows would not fit 32-bit offsets.
-  constexpr int kStepKeys = 16 * kWarps;
-  int j0 = tile * kTileKeys + warp * 16;
+  // Addresses are a base that moves with the steps and offsets of the lane that stay: launches refuse pools whose 32 rows
+  // would not fit 32-bit offsets.
+  int j0 = tile * kTileKeys + warp * kGroup;
   const int end = min(c.slots, stop * kTileKeys);
   if (j0 >= end) return;
   const uint32_t k_row = static_cast<uint32_t>(a.k_strides[2]) * R::kBytes, v_row = static_cast<uint32_t>(a.v_strides[2]) * R::kBytes;
@@ -261,52 +280,61 @@ __device__ __forceinline__ void past_keys(const wm_pool_attn_args& a, const Piec
   const uint8_t* mask = a.key_mask != nullptr ? a.key_mask + static_cast<long long>(c.b) * a.k_len : nullptr;
   const uint32_t k_piece = R::key_piece(t, row_bytes), v_piece = R::value_piece(g, row_bytes);
 
-  uint32_t kr[2][R::kKeyWords], vr[4][R::kValueWords];
-  float kscale[2], vscale[2];
-  bool open = true;  // the mask keeps slot lane of the step
+  uint32_t kr[U][2][R::kKeyWords], vr[U][4][R::kValueWords];
+  float kscale[U][2], vscale[U][2];
+  bool open = true;  // the mask keeps slot `lane` of the step
 
   // Rows behind the last visible slot are not read: the last one takes their place, with weight zero.
   const auto load_k = [&](int j) {
     const int last = c.slots - 1 - j;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t row = last >= 15 ? g + 8 * h : min(g + 8 * h, last);
-      R::load_key(kr[h], k + (row * k_row + k_piece));
-      if (kScaled) {
-        kscale[h] = ks[row * ks_row];
-        vscale[h] = vs[row * vs_row];
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int in = 16 * u + g + 8 * h;
+        const uint32_t row = last >= kGroup - 1 ? in : min(in, last);
+        R::load_key(kr[u][h], k + (row * k_row + k_piece));
+        if (kScaled) {
+          kscale[u][h] = ks[row * ks_row];
+          vscale[u][h] = vs[row * vs_row];
+        }
       }
-    }
-    if (mask != nullptr) open = lane <= min(last, 15) && mask[j + lane] != 0;
+    if (mask != nullptr) open = lane <= min(last, kGroup - 1) && mask[j + lane] != 0;
   };
   const auto load_v = [&](int j) {
     const int last = c.slots - 1 - j;
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      const uint32_t in = 2 * t + (h & 1) + (h & 2) * 4, row = last >= 15 ? in : min(static_cast<int>(in), last);
-      R::load_value(vr[h], v + (row * v_row + v_piece));
-    }
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const int in = 16 * u + 2 * t + (h & 1) + (h & 2) * 4;
+        const uint32_t row = last >= kGroup - 1 ? in : min(in, last);
+        R::load_value(vr[u][h], v + (row * v_row + v_piece));
+      }
   };
 
   load_k(j0);
   load_v(j0);
   for (;;) {
     const int next = j0 + kStepKeys, room = c.slots - j0;
-    uint32_t word = room >= 16 ? 0xffffu : (1u << room) - 1u;
+    constexpr uint32_t kFull = U == 2 ? 0xffffffffu : 0xffffu;
+    uint32_t word = room >= kGroup ? kFull : (1u << room) - 1u;
     if (mask != nullptr) word = __ballot_sync(0xffffffffu, open);
-    const bool all = word == 0xffffu;
-    const uint32_t mine = (word >> g & 1u) | (word >> (g + 8) & 1u) << 1;
-    const uint32_t seen[2] = {mine, mine};
-    float f0 = factor, f1 = factor, w0 = 1.f, w1 = 1.f;
-    if (kScaled) {
-      f0 = factor * kscale[0], f1 = factor * kscale[1], w0 = vscale[0], w1 = vscale[1];
-      if (!all) {
-        if (!(mine & 1u)) f0 = 0.f, w0 = 0.f;
-        if (!(mine & 2u)) f1 = 0.f, w1 = 0.f;
+    Keys keys[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      keys[u].all = word == kFull;
+      keys[u].seen[0] = keys[u].seen[1] = (word >> (16 * u + g) & 1u) | (word >> (16 * u + g + 8) & 1u) << 1;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        keys[u].factor[h] = kScaled ? factor * kscale[u][h] : factor;
+        keys[u].scale[h] = kScaled ? vscale[u][h] : 1.f;
+        if (kScaled && !keys[u].all && !(keys[u].seen[0] >> h & 1u)) keys[u].scale[h] = 0.f;
       }
     }
-    float x[RT][4];
-    scores<kStorage, DP, RT, false>(kr, q, x);
+    float x[U][RT][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) scores<kStorage, DP, RT, false>(kr[u], q, x[u]);
     if (next < end) {
       k += kStepKeys * a.k_strides[2] * R::kBytes;
       if (kScaled) {
@@ -315,23 +343,26 @@ __device__ __forceinline__ void past_keys(const wm_pool_attn_args& a, const Piec
       }
       load_k(next);
     }
-    uint32_t pb[RT][2];
+    uint32_t pb[U][RT][2];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) weights<DP, RT, kScaled>(st, rt, x[rt], f0, f1, w0, w1, all, seen, pb[rt][0], pb[rt][1]);
-    if (!all) {  // what a masked slot holds must not meet its zero weight
+    for (int rt = 0; rt < RT; ++rt) weights<DP, RT, U, kScaled>(st, rt, x, keys, pb);
 #pragma unroll
-      for (int h = 0; h < 4; ++h)
-        if (!(word >> (2 * t + (h & 1) + (h & 2) * 4) & 1u)) {
+    for (int u = 0; u < U; ++u) {
+      if (!keys[u].all) {  // what a masked slot holds must not meet its zero weight
 #pragma unroll
-          for (int w = 0; w < R::kValueWords; ++w) vr[h][w] = 0;
-        }
-    }
+        for (int h = 0; h < 4; ++h)
+          if (!(word >> (16 * u + 2 * t + (h & 1) + (h & 2) * 4) & 1u)) {
 #pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-      uint32_t va[4];
-      R::value_fragment(va, vr, s);
+            for (int w = 0; w < R::kValueWords; ++w) vr[u][h][w] = 0;
+          }
+      }
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) mma_16816(st.o[s][rt], va[0], va[1], va[2], va[3], pb[rt][0], pb[rt][1]);
+      for (int s = 0; s < DP / 16; ++s) {
+        uint32_t va[4];
+        R::value_fragment(va, vr[u], s);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) mma_16816(st.o[s][rt], va[0], va[1], va[2], va[3], pb[u][rt][0], pb[u][rt][1]);
+      }
     }
     if (next >= end) break;
     v += kStepKeys * a.v_strides[2] * R::kBytes;
@@ -370,20 +401,20 @@ __device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Pla
         special |= (vr[h][w] & 0x7f80u) == 0x7f80u || (vr[h][w] & 0x7f800000u) == 0x7f800000u;
       }
     special = __any_sync(0xffffffffu, special);
-    float x[RT][4];
-    scores<WM_BF16, DP, RT, kStorage != WM_BF16>(kr, q, x);
-    uint32_t pb[RT][2], sees[RT][2];
+    float x[1][RT][4];
+    scores<WM_BF16, DP, RT, kStorage != WM_BF16>(kr, q, x[0]);
+    uint32_t pb[1][RT][2], sees[RT][2];
+    Keys keys[1] = {{{factor, factor}, {1.f, 1.f}, {0u, 0u}, false}};
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      uint32_t seen[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         int token, head;
-        row_place(a, c, plan, rt * 8 + 2 * t + j, token, head);
+        row_place(a, plan, c.kv_head, c.row_block, rt * 8 + 2 * t + j, token, head);
         sees[rt][j] = token < nodes ? a.ancestors[(tree + token) * words + (j0 >> 5)] >> (j0 & 31) & usable : 0u;
-        seen[j] = (sees[rt][j] >> g & 1u) | (sees[rt][j] >> (g + 8) & 1u) << 1;
+        keys[0].seen[j] = (sees[rt][j] >> g & 1u) | (sees[rt][j] >> (g + 8) & 1u) << 1;
       }
-      weights<DP, RT, false>(st, rt, x[rt], factor, factor, 1.f, 1.f, false, seen, pb[rt][0], pb[rt][1]);
+      weights<DP, RT, 1, false>(st, rt, x, keys, pb);
     }
     if (!special) {
 #pragma unroll
@@ -391,7 +422,7 @@ __device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Pla
         uint32_t va[4];
         R::value_fragment(va, vr, s);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) mma_16816(st.o[s][rt], va[0], va[1], va[2], va[3], pb[rt][0], pb[rt][1]);
+        for (int rt = 0; rt < RT; ++rt) mma_16816(st.o[s][rt], va[0], va[1], va[2], va[3], pb[0][rt][0], pb[0][rt][1]);
       }
     } else {  // an infinity or NaN among the values reaches the rows that see it and no others: row by row
 #pragma unroll
@@ -402,7 +433,7 @@ __device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Pla
           uint32_t keep[4];
 #pragma unroll
           for (int h = 0; h < 4; ++h) keep[h] = 0u - (row_sees >> (2 * t + (h & 1) + (h & 2) * 4) & 1u);
-          const uint32_t b0 = g == r ? pb[rt][0] : 0u, b1 = g == r ? pb[rt][1] : 0u;
+          const uint32_t b0 = g == r ? pb[0][rt][0] : 0u, b1 = g == r ? pb[0][rt][1] : 0u;
 #pragma unroll
           for (int s = 0; s < DP / 16; ++s) {
             uint32_t va[4], one[4][R::kValueWords];
@@ -422,21 +453,29 @@ __device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Pla
 
 // ---------------------------------------------------------------- kernel
 // Blocks of 128 threads that fit an SM together, from the registers that the accumulators, the rows in flight and the
-// queries take; the launch holds the compiler to it.
-template <int kStorage, int DP, int RT>
-constexpr int resident_blocks() {
-  return DP > 64 ? (RT == 1 ? 4 : RT == 2 ? 3 : 2) : (RT == 1 ? 5 : RT == 2 ? 4 : RT == 4 ? 3 : 2);
+// queries take; the launch holds the compiler to it, and the grid is one wave of them.
+__host__ __device__ constexpr int resident_blocks(int storage, int row_tiles, int padded_dim) {
+  return padded_dim > 64 ? (row_tiles == 1 || (row_tiles == 2 && storage != WM_BF16) ? 3 : 2) : (row_tiles == 1 ? 4 : row_tiles <= 4 ? 3 : 2);
+}
+
+// Shared memory joins the warps at the end of a piece: side by side where their accumulators fit (one meeting), else one
+// warp after another.
+template <int DP, int RT>
+__host__ __device__ constexpr int joined_warps() {
+  return RT * DP <= 256 ? kWarps : 1;
 }
 
 template <int kStorage, int DP, int RT, bool kTree>
-__global__ void __launch_bounds__(kThreads, resident_blocks<kStorage, DP, RT>()) pool_attn_mma_kernel(const wm_pool_attn_args a, const Plan plan) {
-  constexpr int kRows = RT * 8, kPitch = DP + 4;
-  __shared__ __align__(16) float sm_acc[kRows][kPitch];
+__global__ void __launch_bounds__(kThreads, resident_blocks(kStorage, RT, DP)) pool_attn_mma_kernel(const wm_pool_attn_args a, const Plan plan) {
+  constexpr int kRows = RT * 8, kPitch = DP + 4, kSide = joined_warps<DP, RT>();
+  __shared__ __align__(16) float sm_acc[kSide][kRows][kPitch];
   __shared__ float sm_m[kWarps][kRows], sm_l[kWarps][kRows];
   __shared__ uint2 sm_q[Queries<DP, RT>::kShared ? RT * (DP / 16) * 32 : 1];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining kernel may take its place: it waits for this one's end
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   Share share = find_share(a, plan, blockIdx.x, gridDim.x);
-  for (long long at = share.begin; at < share.end;) {
+  if (threadIdx.x == 0) note_of(a, blockIdx.x)->last = -1;
+  for (int at = share.begin; at < share.end;) {
     const Piece c = next_piece(a, plan, at, share.end, share.b, share.b_begin);
     at += c.stop - c.tile;
 
@@ -445,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, resident_blocks<kStorage, DP, RT>())
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       int token, head;
-      row_place(a, c, plan, rt * 8 + g, token, head);
+      row_place(a, plan, c.kv_head, c.row_block, rt * 8 + g, token, head);
       const bool live = token < a.q_len;
       const char* row = static_cast<const char*>(a.q) + (live ? (c.b * a.q_strides[0] + head * a.q_strides[1] + token * a.q_strides[2]) * 2 : 0);
 #pragma unroll
@@ -477,83 +516,92 @@ __global__ void __launch_bounds__(kThreads, resident_blocks<kStorage, DP, RT>())
     if (kTree && c.stop > c.past_tiles)
       draft_keys<kStorage, DP, RT>(a, plan, c, max(c.tile - c.past_tiles, 0), c.stop - c.past_tiles, q, st);
 
-    // join the warps: the largest reference first, then the sums one warp after another
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        if (g == 0) sm_m[warp][rt * 8 + 2 * t + j] = st.m[rt][j];
-    __syncthreads();
+    // join the warps: references and sums first, then the accumulators
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int r = rt * 8 + 2 * t + j;
-        float top = sm_m[0][r];
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm_m[w][r]);
-        const float f = exp2_approx(st.m[rt][j] - top);
         float l = st.l[rt][j];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if (g == 0) sm_l[warp][r] = l * f;
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) {
-          st.o[s][rt][j] *= f;
-          st.o[s][rt][2 + j] *= f;
+        if (g == 0) {
+          sm_m[warp][rt * 8 + 2 * t + j] = st.m[rt][j];
+          sm_l[warp][rt * 8 + 2 * t + j] = l;
         }
       }
+    const int d0 = Rows<WM_BF16, DP>::value_piece(g, a.head_dim * 2) / 2;
+    if (kSide == 1) __syncthreads();
 #pragma unroll 1
-    for (int w = 0; w < kWarps; ++w) {
-      if (w == warp) {
+    for (int w = 0; w < (kSide == 1 ? kWarps : 1); ++w) {
+      if (kSide > 1 || w == warp) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-          for (int s = 0; s < DP / 16; ++s)
+          for (int j = 0; j < 2; ++j) {
+            const int r = rt * 8 + 2 * t + j;
+            float f = 1.f;
+            if (kSide == 1) {
+              float top = sm_m[0][r];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int d = Rows<WM_BF16, DP>::value_piece(g, a.head_dim * 2) / 2 + 2 * s;
-              if (d < g * (DP / 8)) continue;  // a lower lane's
-              float2* p = reinterpret_cast<float2*>(&sm_acc[rt * 8 + 2 * t + j][d]);
-              float2 y = make_float2(st.o[s][rt][j], st.o[s][rt][2 + j]);
-              if (w > 0) {
+              for (int o = 1; o < kWarps; ++o) top = fmaxf(top, sm_m[o][r]);
+              f = exp2_approx(st.m[rt][j] - top);
+            }
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s) {
+              if (d0 + 2 * s < g * (DP / 8)) continue;  // a lower lane's
+              float2* p = reinterpret_cast<float2*>(&sm_acc[kSide == 1 ? 0 : warp][r][d0 + 2 * s]);
+              float2 y = make_float2(st.o[s][rt][j] * f, st.o[s][rt][2 + j] * f);
+              if (kSide == 1 && w > 0) {
                 const float2 z = *p;
                 y.x += z.x;
                 y.y += z.y;
               }
               *p = y;
             }
+          }
       }
       __syncthreads();
     }
-    const int pairs = a.head_dim / 2;
-    for (int i = threadIdx.x; i < kRows * pairs; i += kThreads) {
-      const int r = i / pairs, d = 2 * (i - r * pairs);
-      int token, head;
-      row_place(a, c, plan, r, token, head);
-      if (token >= a.q_len) continue;
-      float l = 0.f, top = sm_m[0][r];
+
+    // one row per thread group
+    constexpr int kPerRow = kRows < kThreads ? kThreads / kRows : 1;
+    const int r = threadIdx.x / kPerRow;
+    int token, head;
+    row_place(a, plan, c.kv_head, c.row_block, r, token, head);
+    if (token < a.q_len) {
+      float top = sm_m[0][r], l = 0.f, f[kWarps];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm_m[w][r]);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        l += sm_l[w][r];
-        top = fmaxf(top, sm_m[w][r]);
+        f[w] = exp2_approx(sm_m[w][r] - top);
+        l = fmaf(sm_l[w][r], f[w], l);
       }
-      float2 y = *reinterpret_cast<const float2*>(&sm_acc[r][d]);
-      if (kTree && a.depths[(a.shared_tree ? 0ll : static_cast<long long>(c.b) * a.q_len) + token] < 0) {  // a padding node sees nothing
-        l = 0.f;
-        y = make_float2(0.f, 0.f);
-      }
-      if (whole(c)) {
-        const float inverse = l == 0.f ? 0.f : 1.f / l;
-        const long long place = c.b * a.out_strides[0] + head * a.out_strides[1] + token * a.out_strides[2] + d;
-        // 0 * infinity: a row without weights is zero whatever its sums are
-        *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + place) = l == 0.f ? 0u : pack_bf16(y.x * inverse, y.y * inverse);
-      } else {
-        float* row = partial_row(static_cast<float*>(a.workspace), a, plan, blockIdx.x, c.tile == 0, r);
-        if (d == 0) *reinterpret_cast<float2*>(row) = make_float2(top, l);
-        *reinterpret_cast<float2*>(row + 2 + d) = y;
+      bool empty = l == 0.f;
+      if (kTree && a.depths[(a.shared_tree ? 0ll : static_cast<long long>(c.b) * a.q_len) + token] < 0) empty = true;  // a padding node sees nothing
+      const float inverse = 1.f / l;
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + c.b * a.out_strides[0] + head * a.out_strides[1] + token * a.out_strides[2];
+      float* partial = partial_row(a, plan, gridDim.x, blockIdx.x, c.tile == 0, r);
+      if (!whole(c) && threadIdx.x % kPerRow == 0) *reinterpret_cast<float2*>(partial) = make_float2(top, empty ? 0.f : l);
+      for (int d = 2 * (threadIdx.x % kPerRow); d < a.head_dim; d += 2 * kPerRow) {
+        float2 y = *reinterpret_cast<const float2*>(&sm_acc[0][r][d]);
+        if (kSide > 1) {
+          y.x *= f[0], y.y *= f[0];
+#pragma unroll
+          for (int w = 1; w < kWarps; ++w) {
+            const float2 z = *reinterpret_cast<const float2*>(&sm_acc[kSide > 1 ? w : 0][r][d]);
+            y.x = fmaf(z.x, f[w], y.x);
+            y.y = fmaf(z.y, f[w], y.y);
+          }
+        }
+        if (empty) y = make_float2(0.f, 0.f);
+        if (whole(c))
+          *reinterpret_cast<uint32_t*>(out + d) = empty ? 0u : pack_bf16(y.x * inverse, y.y * inverse);
+        else
+          *reinterpret_cast<float2*>(partial + 2 + d) = y;
       }
     }
+    if (threadIdx.x == 0) leave_note(a, share, c, blockIdx.x, gridDim.x);
     __syncthreads();
   }
 }
@@ -600,10 +648,6 @@ inline int mma_rows_per_block(long long rows, int head_dim) {
   int n = 8;
   while (n < most && n < rows) n *= 2;
   return n;
-}
-
-inline int mma_resident_blocks(int rows_per_block, int head_dim) {
-  return head_dim > 64 ? (rows_per_block == 8 ? 4 : rows_per_block == 16 ? 3 : 2) : (rows_per_block == 8 ? 5 : rows_per_block == 16 ? 4 : rows_per_block == 32 ? 3 : 2);
 }
 
 }  // namespace pool

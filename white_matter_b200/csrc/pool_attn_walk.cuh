@@ -18,6 +18,7 @@ constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 
 struct Plan {
+  int group;           // query heads per KV head
   int row_blocks;      // of rows_per_block rows, per KV head
   int rows_per_block;
   int draft_tiles;
@@ -34,66 +35,50 @@ __device__ __forceinline__ int sequence_tiles(const wm_pool_attn_args& a, const 
   return tiles > 0 ? tiles : 1;  // a segment that sees nothing still writes its zeros
 }
 
-// One share: units [begin, end) of `total`, and where its first unit lies.
+// One share: units [begin, end) of `total` (less than 2^31, the host sees to it), and where its first unit lies.
 struct Share {
-  long long total, begin, end;
-  int b;               // sequence of unit `begin`
-  long long b_begin;   // first unit of that sequence
+  int total, begin, end;
+  int b;        // sequence of unit `begin`
+  int b_begin;  // first unit of that sequence
 };
 
-__device__ __forceinline__ long long share_begin(long long total, int share, int shares) { return total * share / shares; }
-
-// Inclusive prefix sum over the block, and the block's total; `sums` holds kWarps values.
-__device__ __forceinline__ long long block_scan(long long x, long long* sums, long long& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();
-  if (lane == 31) sums[warp] = x;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) x += sums[w];
-    total += sums[w];
-  }
-  return x;
+// The first unit of a share: equal shares, the first total % shares of them one unit longer.
+__device__ __forceinline__ int share_begin(int total, int share, int shares) {
+  const int each = total / shares;
+  return share * each + min(share, total - each * shares);
 }
 
-// The share of block `share`; all threads of the block call it.
+// The share of block `share`.  Every warp finds it for itself, 32 sequences at a time, so the block does not meet.
 __device__ __forceinline__ Share find_share(const wm_pool_attn_args& a, const Plan& p, int share, int shares) {
-  __shared__ long long sums[kWarps];
-  __shared__ long long found_begin;
-  __shared__ int found;
-  const long long per_tile = static_cast<long long>(a.kv_heads) * p.row_blocks;
+  const int lane = threadIdx.x & 31, per_tile = a.kv_heads * p.row_blocks;
   Share s;
-  s.total = 0;
-  for (int base = 0; base < a.batch; base += kThreads) {
-    const int b = base + threadIdx.x;
-    long long chunk;
-    block_scan(b < a.batch ? sequence_tiles(a, p, b) : 0, sums, chunk);
-    s.total += chunk * per_tile;
-  }
+  int sum = 0;
+  for (int b = lane; b < a.batch; b += 32) sum += sequence_tiles(a, p, b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  s.total = sum * per_tile;
   s.begin = share_begin(s.total, share, shares);
   s.end = share_begin(s.total, share + 1, shares);
-  long long before = 0;
-  for (int base = 0; base < a.batch; base += kThreads) {
-    const int b = base + threadIdx.x;
-    const long long mine = b < a.batch ? sequence_tiles(a, p, b) : 0;
-    long long chunk;
-    const long long upto = (before + block_scan(mine, sums, chunk)) * per_tile;
-    if (s.begin < upto && s.begin >= upto - mine * per_tile) {
-      found = b;
-      found_begin = upto - mine * per_tile;
+  s.b = s.b_begin = 0;
+  if (s.begin >= s.end) return s;
+  for (int base = 0, before = 0; base < a.batch; base += 32) {
+    int upto = base + lane < a.batch ? sequence_tiles(a, p, base + lane) : 0;
+    const int mine = upto;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
     }
-    before += chunk;
+    upto += before;
+    const uint32_t hit = __ballot_sync(0xffffffffu, upto * per_tile > s.begin);
+    if (hit != 0) {
+      const int at = __ffs(hit) - 1;
+      s.b = base + at;
+      s.b_begin = __shfl_sync(0xffffffffu, (upto - mine) * per_tile, at);
+      break;
+    }
+    before = __shfl_sync(0xffffffffu, upto, 31);
   }
-  __syncthreads();
-  s.b = found;
-  s.b_begin = found_begin;
   return s;
 }
 
@@ -107,41 +92,55 @@ struct Piece {
 
 __device__ __forceinline__ bool whole(const Piece& c) { return c.tile == 0 && c.stop == c.tiles; }
 
-// The piece that starts at unit `at` (at < s.end) and ends with its segment or with the share; moves (b, b_begin) on.
-__device__ __forceinline__ Piece next_piece(const wm_pool_attn_args& a, const Plan& p, long long at, long long end, int& b, long long& b_begin) {
+// The piece that starts at unit `at` (at < end) and ends with its segment or with the share; moves (b, b_begin) on.
+__device__ __forceinline__ Piece next_piece(const wm_pool_attn_args& a, const Plan& p, int at, int end, int& b, int& b_begin) {
   Piece c;
   const int segments = a.kv_heads * p.row_blocks;
   for (;;) {
     c.slots = visible_slots(a, b);
     c.past_tiles = (c.slots + kTileKeys - 1) / kTileKeys;
-    c.tiles = c.past_tiles + p.draft_tiles;
-    if (c.tiles < 1) c.tiles = 1;
-    const long long b_end = b_begin + static_cast<long long>(c.tiles) * segments;
+    c.tiles = max(c.past_tiles + p.draft_tiles, 1);
+    const int b_end = b_begin + c.tiles * segments;
     if (at < b_end) break;
     b_begin = b_end;
     ++b;
   }
-  const long long in = at - b_begin;
-  const int segment = static_cast<int>(in / c.tiles);
+  const int in = at - b_begin, segment = in / c.tiles;
   c.b = b;
-  c.tile = static_cast<int>(in - static_cast<long long>(segment) * c.tiles);
+  c.tile = in - segment * c.tiles;
   c.kv_head = segment / p.row_blocks;
   c.row_block = segment - c.kv_head * p.row_blocks;
-  const long long room = end - at;
-  c.stop = room < c.tiles - c.tile ? c.tile + static_cast<int>(room) : c.tiles;
+  c.stop = min(c.tiles, c.tile + end - at);
   return c;
 }
 
-// Partial records: two per share (0: the rest of a segment begun by an earlier share, 1: the start of one that a
-// later share ends), each rows_per_block x (reference, sum, head_dim accumulators).
-__device__ __forceinline__ float* partial_row(float* workspace, const wm_pool_attn_args& a, const Plan& p, int share, int which, int row) {
-  return workspace + ((static_cast<long long>(share) * 2 + which) * p.rows_per_block + row) * (a.head_dim + 2);
+// Workspace: a note per share, then the partial records, two per share (0: the rest of a segment begun by an earlier
+// share, 1: the start of one that a later share ends), each rows_per_block x (reference, sum, head_dim accumulators).
+// The note says which segment the share begins and leaves unfinished, and which share ends it (-1: there is none).
+struct Note {
+  int b, kv_head, row_block, last;
+};
+
+__device__ __forceinline__ Note* note_of(const wm_pool_attn_args& a, int share) { return static_cast<Note*>(a.workspace) + share; }
+
+__device__ __forceinline__ float* partial_row(const wm_pool_attn_args& a, const Plan& p, int shares, int share, int which, int row) {
+  return reinterpret_cast<float*>(note_of(a, shares)) + ((static_cast<long long>(share) * 2 + which) * p.rows_per_block + row) * (a.head_dim + 2);
 }
 
-__device__ __forceinline__ void row_place(const wm_pool_attn_args& a, const Piece& c, const Plan& p, int row, int& token, int& head) {
-  const int group = a.q_heads / a.kv_heads, r = c.row_block * p.rows_per_block + row;
-  token = r / group;
-  head = c.kv_head * group + (r - token * group);
+// One thread of the block notes what its last piece leaves.
+__device__ __forceinline__ void leave_note(const wm_pool_attn_args& a, const Share& s, const Piece& c, int share, int shares) {
+  Note n = {c.b, c.kv_head, c.row_block, -1};
+  if (c.tile == 0 && c.stop < c.tiles) {  // the share that holds the segment's last unit
+    const int unit = s.end + c.tiles - c.stop - 1, each = s.total / shares, longer = s.total - each * shares;
+    n.last = unit < longer * (each + 1) ? unit / (each + 1) : longer + (unit - longer * (each + 1)) / each;
+  }
+  *note_of(a, share) = n;
+}
+
+__device__ __forceinline__ void row_place(const wm_pool_attn_args& a, const Plan& p, int kv_head, int row_block, int row, int& token, int& head) {
+  const int r = row_block * p.rows_per_block + row;
+  token = r / p.group;
+  head = kv_head * p.group + (r - token * p.group);
 }
 
 }  // namespace pool
