@@ -98,7 +98,7 @@ def test_attention_refusals(change, status, text):
         (dict(head_dim=256), -2, b"up to 128"),
         (dict(values=(1 << 20) + 4), -2, b"aligned"),
         (dict(new_key_strides=_native._Strides(64, 64, 60)), -2, b"aligned"),
-        (dict(batch=65536, heads=65536), -2, b"planes"),
+        (dict(heads=65536, rows=65536, source_rows=65536), -2, b"rows per sequence"),
     ],
 )
 def test_commit_refusals(change, status, text):

@@ -98,7 +98,8 @@ __global__ void __launch_bounds__(kThreads) pool_attn_simt_kernel(const wm_pool_
   if (threadIdx.x == 0) note_of(a, blockIdx.x)->last = -1;
   for (int at = share.begin; at < share.end;) {
     const Piece c = next_piece(a, plan, at, share.end, share.b, share.b_begin);
-    at += c.stop - c.tile;
+    at = c.end;
+    if (c.tile >= c.stop) continue;
     SimtState<R> s;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -171,40 +172,56 @@ __global__ void __launch_bounds__(kThreads) pool_attn_simt_kernel(const wm_pool_
 }
 
 // ---------------------------------------------------------------- joining the pieces of a segment
-// Block i joins the segment that share i began and left unfinished, if its note names one.  Every thread keeps one row.
+// Block (i, j) joins rows 8 j .. of the segment that share i began and left unfinished, if its note names one.
+constexpr int kJoinRows = 8, kJoinThreads = 256;
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads) pool_attn_join_kernel(const wm_pool_attn_args a, const Plan plan) {
+__global__ void __launch_bounds__(kJoinThreads) pool_attn_join_kernel(const wm_pool_attn_args a, const Plan plan) {
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched ahead of the first kernel's end
   const int shares = gridDim.x, first = blockIdx.x;
   const Note note = *note_of(a, first);
   if (note.last < 0) return;
-  const int per_row = kThreads / min(plan.rows_per_block, 16), pairs = a.head_dim / 2;
-  for (int r = threadIdx.x / per_row; r < plan.rows_per_block; r += kThreads / per_row) {
-    int token, head;
-    row_place(a, plan, note.kv_head, note.row_block, r, token, head);
-    if (token >= a.q_len) continue;
-    // the reference and the sum of the whole row first, by every thread of the row
+  const int rows = min(plan.rows_per_block, kJoinRows), per_row = kJoinThreads / rows;
+  const int r = blockIdx.y * rows + threadIdx.x / per_row;
+  int token, head;
+  row_place(a, plan, note.kv_head, note.row_block, r, token, head);
+  if (token >= a.q_len) return;
+  const long long pitch = 2ll * plan.rows_per_block * (a.head_dim + 2);  // between the records of consecutive shares
+  const float* begun = partial_row(a, plan, shares, first, 1, r);
+  const float* rest = partial_row(a, plan, shares, first, 0, r);
+  T* out = static_cast<T*>(a.out) + note.b * a.out_strides[0] + head * a.out_strides[1] + token * a.out_strides[2];
+  for (int d = 2 * (threadIdx.x % per_row); d < a.head_dim; d += 2 * per_row) {
+    // the running mean of the records so far; kBatch records in flight
     float top = -INFINITY, l = 0.f;
-    for (int s = first; s <= note.last; ++s) top = fmaxf(top, *partial_row(a, plan, shares, s, s == first, r));
-    const float ref = top == -INFINITY ? 0.f : top;
-    for (int s = first; s <= note.last; ++s) {
-      const float2 x = *reinterpret_cast<const float2*>(partial_row(a, plan, shares, s, s == first, r));
-      l += x.y * exp2f(x.x - ref);
-    }
-    const float inverse = l == 0.f ? 0.f : 1.f / l;
-    T* out = static_cast<T*>(a.out) + note.b * a.out_strides[0] + head * a.out_strides[1] + token * a.out_strides[2];
-    for (int d = threadIdx.x % per_row; d < pairs; d += per_row) {
-      float2 sum = make_float2(0.f, 0.f);
-      for (int s = first; s <= note.last; ++s) {
-        const float* row = partial_row(a, plan, shares, s, s == first, r);
-        const float f = exp2f(row[0] - ref);
-        const float2 y = *reinterpret_cast<const float2*>(row + 2 + 2 * d);
-        sum.x = fmaf(y.x, f, sum.x);
-        sum.y = fmaf(y.y, f, sum.y);
+    float2 acc = make_float2(0.f, 0.f);
+    constexpr int kBatch = 4;
+    for (int n = 0; n <= note.last - first; n += kBatch) {
+      float2 ml[kBatch], y[kBatch];
+      float both = top;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const bool there = n + i <= note.last - first;
+        const float* row = n + i == 0 ? begun : rest + (n + i) * pitch;
+        ml[i] = there ? *reinterpret_cast<const float2*>(row) : make_float2(-INFINITY, 0.f);
+        y[i] = there ? *reinterpret_cast<const float2*>(row + 2 + d) : make_float2(0.f, 0.f);
       }
-      out[2 * d] = from_float<T>(l == 0.f ? 0.f : sum.x * inverse);
-      out[2 * d + 1] = from_float<T>(l == 0.f ? 0.f : sum.y * inverse);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) both = fmaxf(both, ml[i].x);
+      const float ref = both == -INFINITY ? 0.f : both, keep = exp2f(top - ref);
+      l *= keep;
+      acc.x *= keep;
+      acc.y *= keep;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const float f = exp2f(ml[i].x - ref);
+        l = fmaf(ml[i].y, f, l);
+        acc.x = fmaf(y[i].x, f, acc.x);
+        acc.y = fmaf(y[i].y, f, acc.y);
+      }
+      top = both;
     }
+    out[d] = from_float<T>(l == 0.f ? 0.f : acc.x / l);
+    out[d + 1] = from_float<T>(l == 0.f ? 0.f : acc.y / l);
   }
 }
 
@@ -223,15 +240,15 @@ bool make_plan(const wm_pool_attn_args& a, Plan& p) {
   const long long blocks = (rows + p.rows_per_block - 1) / p.rows_per_block;
   p.draft_tiles = a.ancestors != nullptr ? (a.q_len + kTileKeys - 1) / kTileKeys : 0;
   p.group = a.q_heads / a.kv_heads;
-  const double units = (static_cast<double>(a.k_len) / kTileKeys + 1 + p.draft_tiles) * a.batch * a.kv_heads * blocks;
+  const double units = (static_cast<double>(a.k_len) / kTileKeys + 2 + kSegmentCost + p.draft_tiles) * a.batch * a.kv_heads * blocks;
   if (units >= INT_MAX || rows > INT_MAX) return false;  // the kernels count in 32 bits
   p.row_blocks = static_cast<int>(blocks);
   return true;
 }
 
-// One wave: as many shares as blocks fit the GPU, and no more than there can be tiles.
+// One wave: as many shares as blocks fit the GPU, and no more than there can be units.
 int count_shares(const wm_pool_attn_args& a, const Plan& p) {
-  const double tiles = static_cast<double>((a.k_len + kTileKeys - 1) / kTileKeys + p.draft_tiles) * a.batch * a.kv_heads * p.row_blocks;
+  const double tiles = static_cast<double>((a.k_len + kTileKeys - 1) / kTileKeys + p.draft_tiles + kSegmentCost) * a.batch * a.kv_heads * p.row_blocks;
   const int wave = kSms * (a.dtype == WM_F32 ? 6 : resident_blocks(a.storage, p.rows_per_block / 8, a.head_dim));
   return tiles < wave ? (tiles < 1 ? 1 : static_cast<int>(tiles)) : wave;
 }
@@ -319,8 +336,8 @@ int pool_attn_launch(const wm_pool_attn_args& a, cudaStream_t stream) {
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(shares);
-  config.blockDim = dim3(kThreads);
+  config.gridDim = dim3(shares, (plan.rows_per_block + kJoinRows - 1) / kJoinRows);
+  config.blockDim = dim3(kJoinThreads);
   config.stream = stream;
   config.attrs = &early;
   config.numAttrs = 1;

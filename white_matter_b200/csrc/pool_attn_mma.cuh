@@ -458,11 +458,11 @@ __host__ __device__ constexpr int resident_blocks(int storage, int row_tiles, in
   return padded_dim > 64 ? (row_tiles == 1 || (row_tiles == 2 && storage != WM_BF16) ? 3 : 2) : (row_tiles == 1 ? 4 : row_tiles <= 4 ? 3 : 2);
 }
 
-// Shared memory joins the warps at the end of a piece: side by side where their accumulators fit (one meeting), else one
-// warp after another.
+// Shared memory joins the warps at the end of a piece: four accumulators side by side where they fit, else two, to which the
+// other two warps add theirs.
 template <int DP, int RT>
 __host__ __device__ constexpr int joined_warps() {
-  return RT * DP <= 256 ? kWarps : 1;
+  return RT * DP <= 256 ? kWarps : 2;
 }
 
 template <int kStorage, int DP, int RT, bool kTree>
@@ -477,7 +477,8 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(kStorage, RT, DP)) p
   if (threadIdx.x == 0) note_of(a, blockIdx.x)->last = -1;
   for (int at = share.begin; at < share.end;) {
     const Piece c = next_piece(a, plan, at, share.end, share.b, share.b_begin);
-    at += c.stop - c.tile;
+    at = c.end;
+    if (c.tile >= c.stop) continue;
 
     Queries<DP, RT> q;
     q.shared = sm_q;
@@ -530,34 +531,37 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(kStorage, RT, DP)) p
         }
       }
     const int d0 = Rows<WM_BF16, DP>::value_piece(g, a.head_dim * 2) / 2;
-    if (kSide == 1) __syncthreads();
-#pragma unroll 1
-    for (int w = 0; w < (kSide == 1 ? kWarps : 1); ++w) {
-      if (kSide > 1 || w == warp) {
+    if (kSide < kWarps) __syncthreads();  // the references of all warps
+#pragma unroll
+    for (int turn = 0; turn < kWarps / kSide; ++turn) {
+      if (warp / kSide == turn) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const int r = rt * 8 + 2 * t + j;
             float f = 1.f;
-            if (kSide == 1) {
+            if (kSide < kWarps) {
               float top = sm_m[0][r];
 #pragma unroll
               for (int o = 1; o < kWarps; ++o) top = fmaxf(top, sm_m[o][r]);
               f = exp2_approx(st.m[rt][j] - top);
             }
+            float2 y[DP / 16];
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s) {
-              if (d0 + 2 * s < g * (DP / 8)) continue;  // a lower lane's
-              float2* p = reinterpret_cast<float2*>(&sm_acc[kSide == 1 ? 0 : warp][r][d0 + 2 * s]);
-              float2 y = make_float2(st.o[s][rt][j] * f, st.o[s][rt][2 + j] * f);
-              if (kSide == 1 && w > 0) {
-                const float2 z = *p;
-                y.x += z.x;
-                y.y += z.y;
+            for (int s = 0; s < DP / 16; ++s) y[s] = make_float2(st.o[s][rt][j] * f, st.o[s][rt][2 + j] * f);
+            float* row = &sm_acc[warp % kSide][r][d0];
+            if (turn > 0) {
+#pragma unroll
+              for (int s = 0; s < DP / 16; ++s) {
+                const float2 z = *reinterpret_cast<const float2*>(row + 2 * s);
+                y[s].x += z.x;
+                y[s].y += z.y;
               }
-              *p = y;
             }
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s)
+              if (d0 + 2 * s >= g * (DP / 8)) *reinterpret_cast<float2*>(row + 2 * s) = y[s];  // else a lower lane's
           }
       }
       __syncthreads();
@@ -585,14 +589,12 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(kStorage, RT, DP)) p
       if (!whole(c) && threadIdx.x % kPerRow == 0) *reinterpret_cast<float2*>(partial) = make_float2(top, empty ? 0.f : l);
       for (int d = 2 * (threadIdx.x % kPerRow); d < a.head_dim; d += 2 * kPerRow) {
         float2 y = *reinterpret_cast<const float2*>(&sm_acc[0][r][d]);
-        if (kSide > 1) {
-          y.x *= f[0], y.y *= f[0];
+        if (kSide == kWarps) y.x *= f[0], y.y *= f[0];
 #pragma unroll
-          for (int w = 1; w < kWarps; ++w) {
-            const float2 z = *reinterpret_cast<const float2*>(&sm_acc[kSide > 1 ? w : 0][r][d]);
-            y.x = fmaf(z.x, f[w], y.x);
-            y.y = fmaf(z.y, f[w], y.y);
-          }
+        for (int w = 1; w < kSide; ++w) {
+          const float2 z = *reinterpret_cast<const float2*>(&sm_acc[w][r][d]);
+          y.x = fmaf(z.x, kSide == kWarps ? f[w] : 1.f, y.x);
+          y.y = fmaf(z.y, kSide == kWarps ? f[w] : 1.f, y.y);
         }
         if (empty) y = make_float2(0.f, 0.f);
         if (whole(c))

@@ -14,6 +14,10 @@ namespace wm {
 namespace pool {
 
 constexpr int kTileKeys = 128;
+#ifndef SEGCOST
+#define SEGCOST 2
+#endif
+constexpr int kSegmentCost = SEGCOST;
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 
@@ -32,7 +36,7 @@ __device__ __forceinline__ int visible_slots(const wm_pool_attn_args& a, int b) 
 
 __device__ __forceinline__ int sequence_tiles(const wm_pool_attn_args& a, const Plan& p, int b) {
   const int tiles = (visible_slots(a, b) + kTileKeys - 1) / kTileKeys + p.draft_tiles;
-  return tiles > 0 ? tiles : 1;  // a segment that sees nothing still writes its zeros
+  return max(tiles, 1);  // a segment that sees nothing still writes its zeros
 }
 
 // One share: units [begin, end) of `total` (less than 2^31, the host sees to it), and where its first unit lies.
@@ -53,7 +57,7 @@ __device__ __forceinline__ Share find_share(const wm_pool_attn_args& a, const Pl
   const int lane = threadIdx.x & 31, per_tile = a.kv_heads * p.row_blocks;
   Share s;
   int sum = 0;
-  for (int b = lane; b < a.batch; b += 32) sum += sequence_tiles(a, p, b);
+  for (int b = lane; b < a.batch; b += 32) sum += kSegmentCost + sequence_tiles(a, p, b);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   s.total = sum * per_tile;
@@ -62,7 +66,7 @@ __device__ __forceinline__ Share find_share(const wm_pool_attn_args& a, const Pl
   s.b = s.b_begin = 0;
   if (s.begin >= s.end) return s;
   for (int base = 0, before = 0; base < a.batch; base += 32) {
-    int upto = base + lane < a.batch ? sequence_tiles(a, p, base + lane) : 0;
+    int upto = base + lane < a.batch ? kSegmentCost + sequence_tiles(a, p, base + lane) : 0;
     const int mine = upto;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -87,7 +91,8 @@ struct Piece {
   int b, kv_head, row_block;
   int slots;  // visible slots of the sequence
   int past_tiles, tiles;
-  int tile, stop;
+  int tile, stop;  // empty where the share holds no more than the segment's own cost
+  int end;         // first unit behind the piece
 };
 
 __device__ __forceinline__ bool whole(const Piece& c) { return c.tile == 0 && c.stop == c.tiles; }
@@ -100,17 +105,18 @@ __device__ __forceinline__ Piece next_piece(const wm_pool_attn_args& a, const Pl
     c.slots = visible_slots(a, b);
     c.past_tiles = (c.slots + kTileKeys - 1) / kTileKeys;
     c.tiles = max(c.past_tiles + p.draft_tiles, 1);
-    const int b_end = b_begin + c.tiles * segments;
+    const int b_end = b_begin + (c.tiles + kSegmentCost) * segments;
     if (at < b_end) break;
     b_begin = b_end;
     ++b;
   }
-  const int in = at - b_begin, segment = in / c.tiles;
+  const int units = c.tiles + kSegmentCost, in = at - b_begin, segment = in / units, first = in - segment * units;
   c.b = b;
-  c.tile = in - segment * c.tiles;
   c.kv_head = segment / p.row_blocks;
   c.row_block = segment - c.kv_head * p.row_blocks;
-  c.stop = min(c.tiles, c.tile + end - at);
+  c.end = min(end, at + units - first);
+  c.tile = max(first - kSegmentCost, 0);
+  c.stop = max(first + c.end - at - kSegmentCost, 0);
   return c;
 }
 

@@ -65,70 +65,85 @@ __device__ __forceinline__ void row_scale(uint32_t top, int storage, float& inve
   }
 }
 
-// LPR lanes hold one row, 16 source bytes each.  grid: (row groups of a plane, planes = (b, head), K or V).
+// LPR lanes hold one row, 16 source bytes each; a thread has its part of kRows rows in flight.  The rows of a sequence are
+// numbered head by head, so that a block covers neighbouring slots.  grid: (rows of a sequence, sequences, K or V).
+constexpr int kRows = 4;
+
 template <typename T, int LPR, bool kCopy>
 __global__ void __launch_bounds__(kThreads) pool_commit_kernel(const wm_pool_commit_args a) {
-  constexpr int N = Piece<T>::N;
+  constexpr int N = Piece<T>::N, kGroups = kThreads / LPR;
   const bool values = blockIdx.z != 0;
   const int64_t* pool_strides = values ? a.value_strides : a.key_strides;
-  const int64_t* scale_strides = values ? a.value_scale_strides : a.key_scale_strides;
   const int64_t* src_strides = values ? a.new_value_strides : a.new_key_strides;
-  char* pool = static_cast<char*>(values ? a.values : a.keys);
-  float* scales = values ? a.value_scales : a.key_scales;
-  const T* src = static_cast<const T*>(values ? a.new_values : a.new_keys);
   const int lane = threadIdx.x % LPR;
-  const int row = blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR;
   const bool live = lane * N < a.head_dim;
-  for (int plane = blockIdx.y; plane < a.batch * a.heads; plane += gridDim.y) {
-    const int b = plane / a.heads, h = plane - b * a.heads;
-    const long long slot = load_index(a.lengths, a.lengths_is64, b) + a.lead + row;
-    long long from = row;
-    bool keep = row < a.rows && slot >= 0 && slot < a.slots;
-    if (keep && a.counts != nullptr) keep = row < a.counts[b];
-    if (keep && a.index != nullptr) {
-      from = a.index[static_cast<long long>(b) * a.rows + row];
-      keep = from >= 0 && from < a.source_rows;
-    }
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (keep && live) raw = *reinterpret_cast<const uint4*>(src + b * src_strides[0] + h * src_strides[1] + from * src_strides[2] + lane * N);
-    if (kCopy) {
-      if (keep && live)
-        *reinterpret_cast<uint4*>(pool + (b * pool_strides[0] + h * pool_strides[1] + slot * pool_strides[2] + lane * N) * static_cast<int>(sizeof(T))) = raw;
-      continue;
-    }
-    float x[N];
-    Piece<T>::unpack(raw, x);
-    uint32_t top = 0;
+  for (int b = blockIdx.y; b < a.batch; b += gridDim.y) {
+    char* pool = static_cast<char*>(values ? a.values : a.keys) + b * pool_strides[0] * (kCopy ? static_cast<int>(sizeof(T)) : 1);
+    const T* src = static_cast<const T*>(values ? a.new_values : a.new_keys) + b * src_strides[0] + lane * N;
+    const long long first = load_index(a.lengths, a.lengths_is64, b) + a.lead;
+    const int count = a.counts != nullptr ? a.counts[b] : a.rows;
+    uint4 raw[kRows];
+    long long slot[kRows];
+    int head[kRows];
+    bool keep[kRows];
 #pragma unroll
-    for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float inverse, scale;
-    row_scale(top, a.storage, inverse, scale);
-    if (!keep) continue;
-    if (inverse == 0.f) {  // codes of a row of zeros, and of a row that is not finite
-#pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = 0.f;
+    for (int i = 0; i < kRows; ++i) {
+      const int at = (blockIdx.x * kRows + i) * kGroups + threadIdx.x / LPR;
+      head[i] = at / a.rows;
+      const int row = at - head[i] * a.rows;
+      slot[i] = first + row;
+      keep[i] = head[i] < a.heads && row < count && slot[i] >= 0 && slot[i] < a.slots;
+      int from = row;
+      if (keep[i] && a.index != nullptr) {
+        from = a.index[static_cast<long long>(b) * a.rows + row];
+        keep[i] = from >= 0 && from < a.source_rows;
+      }
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if (keep[i] && live) raw[i] = *reinterpret_cast<const uint4*>(src + head[i] * src_strides[1] + from * src_strides[2]);
     }
-    if (live) {
-      uint32_t w[N / 4];
 #pragma unroll
-      for (int i = 0; i < N / 4; ++i) w[i] = a.storage == WM_INT8 ? int8_codes(x + 4 * i, inverse) : e4m3_codes(x + 4 * i, inverse);
-      char* dst = pool + b * pool_strides[0] + h * pool_strides[1] + slot * pool_strides[2] + lane * N;
-      if (N == 8)
-        *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[N / 4 - 1]);
-      else
-        *reinterpret_cast<uint32_t*>(dst) = w[0];
+    for (int i = 0; i < kRows; ++i) {
+      char* dst = pool + (head[i] * pool_strides[1] + slot[i] * pool_strides[2] + lane * N) * (kCopy ? static_cast<int>(sizeof(T)) : 1);
+      if (kCopy) {
+        if (keep[i] && live) *reinterpret_cast<uint4*>(dst) = raw[i];
+        continue;
+      }
+      float x[N];
+      Piece<T>::unpack(raw[i], x);
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < N; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      float inverse, scale;
+      row_scale(top, a.storage, inverse, scale);
+      if (!keep[i]) continue;
+      if (inverse == 0.f) {  // codes of a row of zeros, and of a row that is not finite
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = 0.f;
+      }
+      if (live) {
+        uint32_t w[N / 4];
+#pragma unroll
+        for (int e = 0; e < N / 4; ++e) w[e] = a.storage == WM_INT8 ? int8_codes(x + 4 * e, inverse) : e4m3_codes(x + 4 * e, inverse);
+        if (N == 8)
+          *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[N / 4 - 1]);
+        else
+          *reinterpret_cast<uint32_t*>(dst) = w[0];
+      }
+      if (lane == 0) {
+        float* scales = values ? a.value_scales : a.key_scales;
+        const int64_t* strides = values ? a.value_scale_strides : a.key_scale_strides;
+        scales[b * strides[0] + head[i] * strides[1] + slot[i] * strides[2]] = scale;
+      }
     }
-    if (lane == 0) scales[b * scale_strides[0] + h * scale_strides[1] + slot * scale_strides[2]] = scale;
   }
 }
 
 template <typename T, int LPR>
 int commit(const wm_pool_commit_args& a, cudaStream_t stream) {
-  const int per_block = kThreads / LPR;
-  const long long planes = static_cast<long long>(a.batch) * a.heads;
-  const dim3 grid(static_cast<unsigned>((static_cast<long long>(a.rows) + per_block - 1) / per_block), static_cast<unsigned>(planes < 65535 ? planes : 65535), 2);
+  const long long rows = static_cast<long long>(a.heads) * a.rows, per_block = kRows * kThreads / LPR;
+  const dim3 grid(static_cast<unsigned>((rows + per_block - 1) / per_block), static_cast<unsigned>(a.batch < 65535 ? a.batch : 65535), 2);
   if (a.storage == a.dtype)
     pool_commit_kernel<T, LPR, true><<<grid, kThreads, 0, stream>>>(a);
   else
@@ -146,38 +161,50 @@ int commit_type(const wm_pool_commit_args& a, cudaStream_t stream) {
 }
 
 // ---------------------------------------------------------------- read back
-// One thread turns 16 codes; a plane is one (b, head).
+// A plane is one (b, head).  A thread turns kUnits units of eight codes, all in flight together; neighbouring threads write
+// neighbouring 16 (or 32) bytes.
+constexpr int kUnits = 4;
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) pool_dequant_kernel(const wm_pool_dequant_args a) {
-  const int per_row = a.head_dim / 16;
-  const long long unit = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x;
-  if (unit >= static_cast<long long>(a.slots) * per_row) return;
-  const int slot = static_cast<int>(unit / per_row), piece = static_cast<int>(unit - static_cast<long long>(slot) * per_row);
+  const int per_row = a.head_dim / 8;
+  const long long units = static_cast<long long>(a.slots) * per_row;
   for (int plane = blockIdx.y; plane < a.batch * a.heads; plane += gridDim.y) {
     const int b = plane / a.heads, h = plane - b * a.heads;
-    const bool live = a.lengths == nullptr || slot < load_index(a.lengths, a.lengths_is64, b) + a.lead;
-    float x[16];
-    if (live) {
-      const char* codes = static_cast<const char*>(a.codes) + b * a.code_strides[0] + h * a.code_strides[1] + slot * a.code_strides[2];
-      const uint4 raw = *reinterpret_cast<const uint4*>(codes + 16 * piece);
-      const float scale = a.scales[b * a.scale_strides[0] + h * a.scale_strides[1] + slot * a.scale_strides[2]];
-      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    const long long end = a.lengths == nullptr ? a.slots : load_index(a.lengths, a.lengths_is64, b) + a.lead;
+    const char* codes = static_cast<const char*>(a.codes) + b * a.code_strides[0] + h * a.code_strides[1];
+    const float* scales = a.scales + b * a.scale_strides[0] + h * a.scale_strides[1];
+    T* out = static_cast<T*>(a.out) + b * a.out_strides[0] + h * a.out_strides[1];
+    uint2 raw[kUnits];
+    float scale[kUnits];
+    int slot[kUnits], piece[kUnits];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) codes_to_float(w[i], a.storage == WM_INT8, x + 4 * i);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] *= scale;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = 0.f;
+    for (int i = 0; i < kUnits; ++i) {
+      const long long unit = (static_cast<long long>(blockIdx.x) * kUnits + i) * kThreads + threadIdx.x;
+      slot[i] = unit < units ? static_cast<int>(unit / per_row) : a.slots;
+      piece[i] = static_cast<int>(unit - static_cast<long long>(slot[i]) * per_row);
+      raw[i] = make_uint2(0, 0);
+      scale[i] = 0.f;
+      if (slot[i] < a.slots && slot[i] < end) {
+        raw[i] = *reinterpret_cast<const uint2*>(codes + slot[i] * a.code_strides[2] + 8 * piece[i]);
+        scale[i] = scales[slot[i] * a.scale_strides[2]];
+      }
     }
-    T* dst = static_cast<T*>(a.out) + b * a.out_strides[0] + h * a.out_strides[1] + slot * a.out_strides[2] + 16 * piece;
-    constexpr int N = 16 / sizeof(T);
 #pragma unroll
-    for (int i = 0; i < 16 / N; ++i) {
-      __align__(16) T y[N];
+    for (int i = 0; i < kUnits; ++i) {
+      if (slot[i] >= a.slots) continue;
+      float x[8];
+      codes_to_float(raw[i].x, a.storage == WM_INT8, x);
+      codes_to_float(raw[i].y, a.storage == WM_INT8, x + 4);
+      constexpr int N = 16 / sizeof(T);
+      T* dst = out + slot[i] * a.out_strides[2] + 8 * piece[i];
 #pragma unroll
-      for (int j = 0; j < N; ++j) y[j] = from_float<T>(x[N * i + j]);
-      reinterpret_cast<uint4*>(dst)[i] = *reinterpret_cast<const uint4*>(y);
+      for (int q = 0; q < 8 / N; ++q) {
+        __align__(16) T y[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) y[j] = from_float<T>(x[N * q + j] * scale[i]);
+        reinterpret_cast<uint4*>(dst)[q] = *reinterpret_cast<const uint4*>(y);
+      }
     }
   }
 }
@@ -261,7 +288,7 @@ int pool_commit_launch(const wm_pool_commit_args& a, cudaStream_t stream) {
   if (a.index == nullptr && a.source_rows < a.rows) return fail(WM_EINVAL, "%s: more rows than the source has", who);
   if (a.lead != 0 && a.lead != 1) return fail(WM_EINVAL, "%s: lead must be 0 or 1", who);
   if (a.head_dim % 16 || a.head_dim > 128) return fail(WM_EUNSUPPORTED, "%s: head_dim must be a multiple of 16 up to 128", who);
-  if (static_cast<long long>(a.batch) * a.heads > INT_MAX) return fail(WM_EUNSUPPORTED, "%s: too many (sequence, head) planes", who);
+  if (static_cast<long long>(a.heads) * a.rows > INT_MAX - kRows * kThreads) return fail(WM_EUNSUPPORTED, "%s: too many rows per sequence", who);
   const int wide = a.dtype == WM_F32 ? 4 : 2, held = quantised ? 1 : wide;
   if (!aligned16(a.keys) || !aligned16(a.values) || !aligned16(a.new_keys) || !aligned16(a.new_values) || !aligned16(a.key_strides, held) ||
       !aligned16(a.value_strides, held) || !aligned16(a.new_key_strides, wide) || !aligned16(a.new_value_strides, wide))
@@ -282,8 +309,8 @@ int pool_dequant_launch(const wm_pool_dequant_args& a, cudaStream_t stream) {
   const int wide = a.dtype == WM_F32 ? 4 : 2;
   if (!aligned16(a.codes) || !aligned16(a.out) || !aligned16(a.code_strides, 1) || !aligned16(a.out_strides, wide))
     return fail(WM_EUNSUPPORTED, "%s: rows must be 16-byte aligned", who);
-  const long long units = static_cast<long long>(a.slots) * (a.head_dim / 16);
-  const dim3 grid(static_cast<unsigned>((units + kThreads - 1) / kThreads), static_cast<unsigned>(planes < 65535 ? planes : 65535));
+  const long long units = static_cast<long long>(a.slots) * (a.head_dim / 8), per_block = kUnits * kThreads;
+  const dim3 grid(static_cast<unsigned>((units + per_block - 1) / per_block), static_cast<unsigned>(planes < 65535 ? planes : 65535));
   if (a.dtype == WM_F32)
     pool_dequant_kernel<float><<<grid, kThreads, 0, stream>>>(a);
   else
