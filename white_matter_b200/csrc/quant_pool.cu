@@ -65,12 +65,13 @@ __device__ __forceinline__ void row_scale(uint32_t top, int storage, float& inve
   }
 }
 
-// LPR lanes hold one row, 16 source bytes each; a thread has its part of kRows rows in flight.  The rows of a sequence are
-// numbered head by head, so that a block covers neighbouring slots.  grid: (rows of a sequence, sequences, K or V).
+// LPR lanes hold one row, 16 source bytes each; a thread has its part of kRows rows in flight.  Sources that keep a token's
+// heads side by side (head_major false) are read that way, kRows tokens of neighbouring heads; the others slot by slot.
+// grid: (rows of a sequence, sequences, K or V).
 constexpr int kRows = 4;
 
 template <typename T, int LPR, bool kCopy>
-__global__ void __launch_bounds__(kThreads) pool_commit_kernel(const wm_pool_commit_args a) {
+__global__ void __launch_bounds__(kThreads) pool_commit_kernel(const wm_pool_commit_args a, bool head_major) {
   constexpr int N = Piece<T>::N, kGroups = kThreads / LPR;
   const bool values = blockIdx.z != 0;
   const int64_t* pool_strides = values ? a.value_strides : a.key_strides;
@@ -88,11 +89,18 @@ __global__ void __launch_bounds__(kThreads) pool_commit_kernel(const wm_pool_com
     bool keep[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-      const int at = (blockIdx.x * kRows + i) * kGroups + threadIdx.x / LPR;
-      head[i] = at / a.rows;
-      const int row = at - head[i] * a.rows;
+      int row;
+      if (head_major) {
+        const int at = (blockIdx.x * kRows + i) * kGroups + threadIdx.x / LPR;
+        head[i] = at / a.rows;
+        row = at - head[i] * a.rows;
+      } else {
+        const int at = blockIdx.x * kGroups + threadIdx.x / LPR, block = at / a.heads;
+        head[i] = at - block * a.heads;
+        row = block * kRows + i;
+      }
       slot[i] = first + row;
-      keep[i] = head[i] < a.heads && row < count && slot[i] >= 0 && slot[i] < a.slots;
+      keep[i] = head[i] < a.heads && row < a.rows && row < count && slot[i] >= 0 && slot[i] < a.slots;
       int from = row;
       if (keep[i] && a.index != nullptr) {
         from = a.index[static_cast<long long>(b) * a.rows + row];
@@ -142,12 +150,14 @@ __global__ void __launch_bounds__(kThreads) pool_commit_kernel(const wm_pool_com
 
 template <typename T, int LPR>
 int commit(const wm_pool_commit_args& a, cudaStream_t stream) {
-  const long long rows = static_cast<long long>(a.heads) * a.rows, per_block = kRows * kThreads / LPR;
+  const bool head_major = a.rows < kRows || a.new_key_strides[1] >= a.new_key_strides[2];
+  const long long rows = static_cast<long long>(a.heads) * (head_major ? a.rows : (a.rows + kRows - 1) / kRows * kRows);
+  const long long per_block = kRows * kThreads / LPR;
   const dim3 grid(static_cast<unsigned>((rows + per_block - 1) / per_block), static_cast<unsigned>(a.batch < 65535 ? a.batch : 65535), 2);
   if (a.storage == a.dtype)
-    pool_commit_kernel<T, LPR, true><<<grid, kThreads, 0, stream>>>(a);
+    pool_commit_kernel<T, LPR, true><<<grid, kThreads, 0, stream>>>(a, head_major);
   else
-    pool_commit_kernel<T, LPR, false><<<grid, kThreads, 0, stream>>>(a);
+    pool_commit_kernel<T, LPR, false><<<grid, kThreads, 0, stream>>>(a, head_major);
   count_launch();
   return cuda_check(cudaGetLastError(), "pool_commit_kernel");
 }
@@ -161,49 +171,51 @@ int commit_type(const wm_pool_commit_args& a, cudaStream_t stream) {
 }
 
 // ---------------------------------------------------------------- read back
-// A plane is one (b, head).  A thread turns kUnits units of eight codes, all in flight together; neighbouring threads write
-// neighbouring 16 (or 32) bytes.
-constexpr int kUnits = 4;
+// A plane is one (b, head).  A thread turns 16 codes of kUnits rows, all in flight together; the threads of a block that do
+// not fill a row are idle.
+constexpr int kUnits = 2;
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) pool_dequant_kernel(const wm_pool_dequant_args a) {
-  const int per_row = a.head_dim / 8;
-  const long long units = static_cast<long long>(a.slots) * per_row;
+  const int per_row = a.head_dim / 16, rows = kThreads / per_row, row = threadIdx.x / per_row, piece = threadIdx.x - row * per_row;
+  if (row >= rows) return;
   for (int plane = blockIdx.y; plane < a.batch * a.heads; plane += gridDim.y) {
     const int b = plane / a.heads, h = plane - b * a.heads;
     const long long end = a.lengths == nullptr ? a.slots : load_index(a.lengths, a.lengths_is64, b) + a.lead;
-    const char* codes = static_cast<const char*>(a.codes) + b * a.code_strides[0] + h * a.code_strides[1];
+    const char* codes = static_cast<const char*>(a.codes) + b * a.code_strides[0] + h * a.code_strides[1] + 16 * piece;
     const float* scales = a.scales + b * a.scale_strides[0] + h * a.scale_strides[1];
-    T* out = static_cast<T*>(a.out) + b * a.out_strides[0] + h * a.out_strides[1];
-    uint2 raw[kUnits];
+    T* out = static_cast<T*>(a.out) + b * a.out_strides[0] + h * a.out_strides[1] + 16 * piece;
+    uint4 raw[kUnits];
     float scale[kUnits];
-    int slot[kUnits], piece[kUnits];
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
-      const long long unit = (static_cast<long long>(blockIdx.x) * kUnits + i) * kThreads + threadIdx.x;
-      slot[i] = unit < units ? static_cast<int>(unit / per_row) : a.slots;
-      piece[i] = static_cast<int>(unit - static_cast<long long>(slot[i]) * per_row);
-      raw[i] = make_uint2(0, 0);
+      const int slot = (blockIdx.x * kUnits + i) * rows + row;
+      raw[i] = make_uint4(0, 0, 0, 0);
       scale[i] = 0.f;
-      if (slot[i] < a.slots && slot[i] < end) {
-        raw[i] = *reinterpret_cast<const uint2*>(codes + slot[i] * a.code_strides[2] + 8 * piece[i]);
-        scale[i] = scales[slot[i] * a.scale_strides[2]];
+      if (slot < a.slots && slot < end) {
+        raw[i] = *reinterpret_cast<const uint4*>(codes + slot * a.code_strides[2]);
+        scale[i] = scales[slot * a.scale_strides[2]];
       }
     }
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
-      if (slot[i] >= a.slots) continue;
-      float x[8];
-      codes_to_float(raw[i].x, a.storage == WM_INT8, x);
-      codes_to_float(raw[i].y, a.storage == WM_INT8, x + 4);
-      constexpr int N = 16 / sizeof(T);
-      T* dst = out + slot[i] * a.out_strides[2] + 8 * piece[i];
+      const int slot = (blockIdx.x * kUnits + i) * rows + row;
+      if (slot >= a.slots) continue;
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      constexpr int N = 32 / sizeof(T);  // one 32-byte store
 #pragma unroll
-      for (int q = 0; q < 8 / N; ++q) {
+      for (int q = 0; q < 16 / N; ++q) {
         __align__(16) T y[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j) y[j] = from_float<T>(x[N * q + j] * scale[i]);
-        reinterpret_cast<uint4*>(dst)[q] = *reinterpret_cast<const uint4*>(y);
+        for (int j = 0; j < N; j += 4) {
+          float x[4];
+          codes_to_float(w[(q * N + j) / 4], a.storage == WM_INT8, x);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[j + e] = from_float<T>(x[e] * scale[i]);
+        }
+        uint4* dst = reinterpret_cast<uint4*>(out + slot * a.out_strides[2] + q * N);
+        __stcs(dst, reinterpret_cast<const uint4*>(y)[0]);
+        __stcs(dst + 1, reinterpret_cast<const uint4*>(y)[1]);
       }
     }
   }
@@ -309,8 +321,8 @@ int pool_dequant_launch(const wm_pool_dequant_args& a, cudaStream_t stream) {
   const int wide = a.dtype == WM_F32 ? 4 : 2;
   if (!aligned16(a.codes) || !aligned16(a.out) || !aligned16(a.code_strides, 1) || !aligned16(a.out_strides, wide))
     return fail(WM_EUNSUPPORTED, "%s: rows must be 16-byte aligned", who);
-  const long long units = static_cast<long long>(a.slots) * (a.head_dim / 8), per_block = kUnits * kThreads;
-  const dim3 grid(static_cast<unsigned>((units + per_block - 1) / per_block), static_cast<unsigned>(planes < 65535 ? planes : 65535));
+  const int per_block = kUnits * (kThreads / (a.head_dim / 16));
+  const dim3 grid(static_cast<unsigned>((static_cast<long long>(a.slots) + per_block - 1) / per_block), static_cast<unsigned>(planes < 65535 ? planes : 65535));
   if (a.dtype == WM_F32)
     pool_dequant_kernel<float><<<grid, kThreads, 0, stream>>>(a);
   else
