@@ -444,13 +444,18 @@ def strides3(t: torch.Tensor) -> _Strides:
     return _Strides(t.stride(0), t.stride(1), t.stride(2))
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the handle without a Stream object around it: 0.1 us, not 2
+
+
 def current_stream(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
 def call(name: str, args, device: torch.device) -> None:
     """Invoke an entry point on the current stream of ``device``; raise on failure."""
-    lib = load_library()
+    lib = _library or load_library()
     if device.index is None or device.index == torch.cuda.current_device():
         status = getattr(lib, name)(ctypes.byref(args), current_stream(device))
     else:  # the library launches on the current device: make the tensors' device current for the call

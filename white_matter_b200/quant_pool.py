@@ -25,8 +25,8 @@ _QUANTISED = (torch.int8, torch.float8_e4m3fn)
 _ROWS = (torch.bfloat16, torch.float32)
 
 
-def _refuse_grad(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _refuse_grad(what: str, *tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and True in [t.requires_grad for t in tensors]:
         raise ValueError(f"{what} has no gradients: call it under torch.no_grad()")
 
 
@@ -38,12 +38,13 @@ def _int_vector(name: str, t: torch.Tensor, batch: int, device: torch.device) ->
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """The tensor itself where its rows have unit stride and start on 16 bytes, else a copy."""
-    wide = t.element_size()
-    if t.stride(3) == 1 and not t.data_ptr() % 16 and not any(t.stride(i) * wide % 16 for i in range(3)):
-        return t
-    return t.contiguous()
+def _aligned(t: torch.Tensor) -> tuple[torch.Tensor, int, tuple[int, int, int]]:
+    """(tensor, address, strides) of the tensor itself where its rows have unit stride and start on 16 bytes, else of a copy."""
+    address, (batch, head, token, inner) = t.data_ptr(), t.stride()
+    if inner != 1 or (address | (batch | head | token) * t.element_size()) & 15:
+        t = t.contiguous()
+        address, (batch, head, token, inner) = t.data_ptr(), t.stride()
+    return t, address, (batch, head, token)
 
 
 def _check_pool(keys: torch.Tensor, values: torch.Tensor, key_scales, value_scales) -> None:
@@ -53,7 +54,7 @@ def _check_pool(keys: torch.Tensor, values: torch.Tensor, key_scales, value_scal
         raise ValueError("pool keys and values must share dtype and device")
     if not keys.is_cuda:
         raise ValueError("sm100 pool operators require CUDA tensors")
-    if keys.stride(3) != 1 or values.stride(3) != 1:
+    if keys.stride()[3] != 1 or values.stride()[3] != 1:
         raise ValueError("pool rows must have unit stride in head_dim")
     if keys.dtype in _QUANTISED:
         for name, scales in (("key_scales", key_scales), ("value_scales", value_scales)):
@@ -94,15 +95,14 @@ def pool_commit(
             counts = counts.clamp(0, rows).to(torch.int32)
     if not batch or not heads or not slots or not dim or not rows or not new_keys.shape[2]:
         return rows
-    new_keys, new_values = _aligned(new_keys), _aligned(new_values)
     a = _native.PoolCommitArgs()
+    new_keys, a.new_keys, a.new_key_strides = _aligned(new_keys)
+    new_values, a.new_values, a.new_value_strides = _aligned(new_values)
     a.keys, a.values = keys.data_ptr(), values.data_ptr()
-    a.key_strides, a.value_strides = _native.strides3(keys), _native.strides3(values)
+    a.key_strides, a.value_strides = keys.stride()[:3], values.stride()[:3]
     if key_scales is not None:
         a.key_scales, a.value_scales = key_scales.data_ptr(), value_scales.data_ptr()
-        a.key_scale_strides, a.value_scale_strides = _native.strides3(key_scales), _native.strides3(value_scales)
-    a.new_keys, a.new_values = new_keys.data_ptr(), new_values.data_ptr()
-    a.new_key_strides, a.new_value_strides = _native.strides3(new_keys), _native.strides3(new_values)
+        a.key_scale_strides, a.value_scale_strides = key_scales.stride(), value_scales.stride()
     a.lengths, a.lengths_is64 = lengths.data_ptr(), lengths.dtype == torch.int64
     if index is not None:
         a.index = index.data_ptr()
@@ -172,7 +172,7 @@ def dequantize_kv_rows(
         return out
     a = _native.PoolDequantArgs()
     a.codes, a.scales, a.out = codes.data_ptr(), scales.data_ptr(), out.data_ptr()
-    a.code_strides, a.scale_strides, a.out_strides = _native.strides3(codes), _native.strides3(scales), _native.strides3(out)
+    a.code_strides, a.scale_strides, a.out_strides = codes.stride()[:3], scales.stride(), out.stride()[:3]
     if lengths is not None:
         a.lengths, a.lengths_is64 = lengths.data_ptr(), lengths.dtype == torch.int64
     a.storage, a.dtype = _native.storage_code(codes.dtype), _native.dtype_code(dtype)
@@ -217,14 +217,14 @@ def pool_attention(
         return out
     if not slots:
         return out.zero_()
-    query = _aligned(query)
     a = _native.PoolAttnArgs()
-    a.q, a.k, a.v, a.out = query.data_ptr(), keys.data_ptr(), values.data_ptr(), out.data_ptr()
-    a.q_strides, a.k_strides, a.v_strides = _native.strides3(query), _native.strides3(keys), _native.strides3(values)
-    a.out_strides = _native._Strides(length * heads * dim, dim, heads * dim)
+    query, a.q, a.q_strides = _aligned(query)
+    a.k, a.v, a.out = keys.data_ptr(), values.data_ptr(), out.data_ptr()
+    a.k_strides, a.v_strides = keys.stride()[:3], values.stride()[:3]
+    a.out_strides = length * heads * dim, dim, heads * dim
     if key_scales is not None:
         a.k_scales, a.v_scales = key_scales.data_ptr(), value_scales.data_ptr()
-        a.k_scale_strides, a.v_scale_strides = _native.strides3(key_scales), _native.strides3(value_scales)
+        a.k_scale_strides, a.v_scale_strides = key_scales.stride(), value_scales.stride()
     if kv_lengths is not None:
         a.lengths, a.lengths_is64 = kv_lengths.data_ptr(), kv_lengths.dtype == torch.int64
     if key_mask is not None:
@@ -232,10 +232,10 @@ def pool_attention(
         a.key_mask = key_mask.data_ptr()
     if draft is not None:
         draft_keys, draft_values, ancestors, depths = draft
-        draft_keys, draft_values = _aligned(draft_keys), _aligned(draft_values)
+        draft_keys, a.draft_k, a.draft_k_strides = _aligned(draft_keys)
+        draft_values, a.draft_v, a.draft_v_strides = _aligned(draft_values)
         ancestors, depths = ancestors.contiguous(), depths.contiguous()
-        a.draft_k, a.draft_v, a.ancestors, a.depths = (t.data_ptr() for t in (draft_keys, draft_values, ancestors, depths))
-        a.draft_k_strides, a.draft_v_strides = _native.strides3(draft_keys), _native.strides3(draft_values)
+        a.ancestors, a.depths = ancestors.data_ptr(), depths.data_ptr()
         a.shared_tree = depths.shape[0] == 1
     a.dtype, a.storage = _native.dtype_code(query.dtype), _native.storage_code(keys.dtype)
     a.batch, a.q_heads, a.q_len, a.head_dim = batch, heads, length, dim
