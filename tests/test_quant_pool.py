@@ -52,7 +52,7 @@ def fake_attn(**change):
     for name in ("q_strides", "k_strides", "v_strides", "out_strides"):
         setattr(a, name, _native._Strides(4096, 1024, 64))
     a.dtype, a.storage = _native.WM_BF16, _native.WM_INT8
-    a.batch, a.q_heads, a.kv_heads, a.q_len, a.k_len, a.head_dim, a.scale = 1, 2, 1, 1, 16, 64, 1.0
+    a.batch, a.q_heads, a.kv_heads, a.q_len, a.k_len, a.head_dim, a.scale = 1, 2, 1, 1, 8000, 64, 1.0
     for name, value in change.items():
         setattr(a, name, value)
     return a

@@ -234,6 +234,24 @@ int rows_per_block(const wm_pool_attn_args& a) {
   return a.dtype == WM_F32 ? (rows == 1 ? 1 : 4) : mma_rows_per_block(rows, a.head_dim);
 }
 
+// One wave: as many shares as blocks fit the GPU, and no more than there can be units.
+int count_shares(const wm_pool_attn_args& a, const Plan& p) {
+  const double tiles = static_cast<double>((a.k_len + kTileKeys - 1) / kTileKeys + p.draft_tiles + kSegmentCost) * a.batch * a.kv_heads * p.row_blocks;
+  const int wave = kSms * (a.dtype == WM_F32 ? 6 : resident_blocks(a.storage, p.rows_per_block / 8, a.head_dim));
+  return tiles < wave ? (tiles < 1 ? 1 : static_cast<int>(tiles)) : wave;
+}
+
+// A cluster per segment where all clusters fit one wave and no block gets more than four tiles of the longest sequence the
+// pool can hold: one launch instead of two, XXX us against XXX us on one sequence of 480 tokens with 16 heads.
+int cluster_size(const wm_pool_attn_args& a, const Plan& p) {
+  if (a.dtype == WM_F32 || p.rows_per_block > 16) return 0;
+  const int tiles = (a.k_len + kTileKeys - 1) / kTileKeys + p.draft_tiles;
+  int size = 1;
+  while (size < kMaxCluster && size < tiles) size *= 2;
+  const double blocks = static_cast<double>(a.batch) * a.kv_heads * p.row_blocks * size;
+  return tiles <= 4 * size && blocks <= kSms * resident_blocks(a.storage, p.rows_per_block / 8, a.head_dim) ? size : 0;
+}
+
 bool make_plan(const wm_pool_attn_args& a, Plan& p) {
   const long long rows = static_cast<long long>(a.q_heads / a.kv_heads) * a.q_len;
   p.rows_per_block = rows_per_block(a);
@@ -243,14 +261,9 @@ bool make_plan(const wm_pool_attn_args& a, Plan& p) {
   const double units = (static_cast<double>(a.k_len) / kTileKeys + 2 + kSegmentCost + p.draft_tiles) * a.batch * a.kv_heads * blocks;
   if (units >= INT_MAX || rows > INT_MAX) return false;  // the kernels count in 32 bits
   p.row_blocks = static_cast<int>(blocks);
+  p.cluster = cluster_size(a, p);
+  p.blocks = p.cluster > 0 ? a.batch * a.kv_heads * p.row_blocks * p.cluster : count_shares(a, p);
   return true;
-}
-
-// One wave: as many shares as blocks fit the GPU, and no more than there can be units.
-int count_shares(const wm_pool_attn_args& a, const Plan& p) {
-  const double tiles = static_cast<double>((a.k_len + kTileKeys - 1) / kTileKeys + p.draft_tiles + kSegmentCost) * a.batch * a.kv_heads * p.row_blocks;
-  const int wave = kSms * (a.dtype == WM_F32 ? 6 : resident_blocks(a.storage, p.rows_per_block / 8, a.head_dim));
-  return tiles < wave ? (tiles < 1 ? 1 : static_cast<int>(tiles)) : wave;
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -283,21 +296,19 @@ int validate(const wm_pool_attn_args& a, Plan& plan) {
 }
 
 template <int kStorage, int LPK>
-void launch_simt_rows(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream) {
+cudaError_t launch_simt_rows(const wm_pool_attn_args& a, const Plan& plan, cudaStream_t stream) {
   if (plan.rows_per_block == 1)
-    pool_attn_simt_kernel<kStorage, LPK, 1><<<shares, kThreads, 0, stream>>>(a, plan);
+    pool_attn_simt_kernel<kStorage, LPK, 1><<<plan.blocks, kThreads, 0, stream>>>(a, plan);
   else
-    pool_attn_simt_kernel<kStorage, LPK, 4><<<shares, kThreads, 0, stream>>>(a, plan);
+    pool_attn_simt_kernel<kStorage, LPK, 4><<<plan.blocks, kThreads, 0, stream>>>(a, plan);
+  return cudaGetLastError();
 }
 
 template <int kStorage>
-void launch_simt(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream) {
-  if (a.head_dim <= 32)
-    launch_simt_rows<kStorage, 8>(a, plan, shares, stream);
-  else if (a.head_dim <= 64)
-    launch_simt_rows<kStorage, 16>(a, plan, shares, stream);
-  else
-    launch_simt_rows<kStorage, 32>(a, plan, shares, stream);
+cudaError_t launch_simt(const wm_pool_attn_args& a, const Plan& plan, cudaStream_t stream) {
+  if (a.head_dim <= 32) return launch_simt_rows<kStorage, 8>(a, plan, stream);
+  if (a.head_dim <= 64) return launch_simt_rows<kStorage, 16>(a, plan, stream);
+  return launch_simt_rows<kStorage, 32>(a, plan, stream);
 }
 
 }  // namespace
@@ -305,7 +316,8 @@ void launch_simt(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaS
 size_t pool_attn_workspace(const wm_pool_attn_args& a) {
   Plan plan;
   if (a.batch < 1 || a.kv_heads < 1 || a.q_heads < a.kv_heads || a.q_len < 1 || a.k_len < 1 || !make_plan(a, plan)) return 0;
-  return static_cast<size_t>(count_shares(a, plan)) * (sizeof(Note) + 2 * plan.rows_per_block * (a.head_dim + 2) * sizeof(float));
+  if (plan.cluster > 0) return 0;
+  return static_cast<size_t>(plan.blocks) * (sizeof(Note) + 2 * plan.rows_per_block * (a.head_dim + 2) * sizeof(float));
 }
 
 int pool_attn_launch(const wm_pool_attn_args& a, cudaStream_t stream) {
@@ -313,30 +325,25 @@ int pool_attn_launch(const wm_pool_attn_args& a, cudaStream_t stream) {
   const int status = validate(a, plan);
   if (status != WM_OK) return status;
   const size_t need = pool_attn_workspace(a);
-  if (a.workspace == nullptr || a.workspace_bytes < need) return fail(WM_EWORKSPACE, "wm_pool_attn needs %zu workspace bytes, got %zu", need, a.workspace_bytes);
-  const int shares = count_shares(a, plan);
-  if (a.dtype == WM_F32) {
-    if (a.storage == WM_INT8)
-      launch_simt<WM_INT8>(a, plan, shares, stream);
-    else if (a.storage == WM_E4M3)
-      launch_simt<WM_E4M3>(a, plan, shares, stream);
-    else
-      launch_simt<WM_F32>(a, plan, shares, stream);
-  } else if (a.storage == WM_INT8) {
-    launch_mma_int8(a, plan, shares, stream);
-  } else if (a.storage == WM_E4M3) {
-    launch_mma_e4m3(a, plan, shares, stream);
-  } else {
-    launch_mma_bf16(a, plan, shares, stream);
-  }
+  if (need > 0 && (a.workspace == nullptr || a.workspace_bytes < need)) return fail(WM_EWORKSPACE, "wm_pool_attn needs %zu workspace bytes, got %zu", need, a.workspace_bytes);
+  const bool tree = a.ancestors != nullptr;
+  cudaError_t launched;
+  if (a.dtype == WM_F32)
+    launched = a.storage == WM_INT8 ? launch_simt<WM_INT8>(a, plan, stream) : a.storage == WM_E4M3 ? launch_simt<WM_E4M3>(a, plan, stream) : launch_simt<WM_F32>(a, plan, stream);
+  else if (a.storage == WM_INT8)
+    launched = tree ? launch_mma_storage<WM_INT8, true>(a, plan, stream) : launch_mma_storage<WM_INT8, false>(a, plan, stream);
+  else if (a.storage == WM_E4M3)
+    launched = tree ? launch_mma_storage<WM_E4M3, true>(a, plan, stream) : launch_mma_storage<WM_E4M3, false>(a, plan, stream);
+  else
+    launched = tree ? launch_mma_storage<WM_BF16, true>(a, plan, stream) : launch_mma_storage<WM_BF16, false>(a, plan, stream);
   count_launch();
-  WM_CUDA(cudaGetLastError());
-  if (shares == 1) return WM_OK;
+  WM_CUDA(launched);
+  if (plan.cluster > 0 || plan.blocks == 1) return WM_OK;
   cudaLaunchAttribute early = {};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(shares, (plan.rows_per_block + kJoinRows - 1) / kJoinRows);
+  config.gridDim = dim3(plan.blocks, (plan.rows_per_block + kJoinRows - 1) / kJoinRows);
   config.blockDim = dim3(kJoinThreads);
   config.stream = stream;
   config.attrs = &early;

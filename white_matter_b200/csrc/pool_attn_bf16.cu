@@ -3,10 +3,6 @@
 
 namespace wm {
 namespace pool {
-
-void launch_mma_bf16(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream) {
-  launch_mma_storage<WM_BF16>(a, plan, shares, stream);
-}
-
+WM_POOL_ATTN_UNIT(WM_BF16, false)
 }  // namespace pool
 }  // namespace wm

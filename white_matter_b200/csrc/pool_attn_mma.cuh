@@ -486,20 +486,70 @@ __host__ __device__ constexpr int joined_warps() {
   return RT * DP <= 256 ? kWarps : 2;
 }
 
-template <int kStorage, int DP, int RT, bool kTree, bool kDense>
+// How the blocks of a launch share the work.
+enum Mode {
+  kShares,       // equal shares of all tiles, any strides
+  kDenseShares,  // the same, for pools whose rows are DP elements and lie one behind the other
+  kCluster       // few short segments: one cluster per segment, which joins its blocks' sums through shared memory
+};
+constexpr int kMaxCluster = 8;
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_blocks() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float2 load_remote(const void* mine, uint32_t rank) {
+  float2 y;
+  asm volatile("{.reg .u32 at;\nmapa.shared::cluster.u32 at, %2, %3;\nld.shared::cluster.v2.f32 {%0, %1}, [at];}"
+               : "=f"(y.x), "=f"(y.y)
+               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(mine))), "r"(rank)
+               : "memory");
+  return y;
+}
+
+// The cluster's segment, cut into equal runs of tiles.
+__device__ __forceinline__ Piece cluster_piece(const wm_pool_attn_args& a, const Plan& p) {
+  const int n = cluster_blocks(), rank = cluster_rank(), at = blockIdx.x / n;
+  Piece c;
+  c.row_block = at % p.row_blocks;
+  c.kv_head = at / p.row_blocks % a.kv_heads;
+  c.b = at / p.row_blocks / a.kv_heads;
+  c.slots = visible_slots(a, c.b);
+  c.past_tiles = (c.slots + kTileKeys - 1) / kTileKeys;
+  c.tiles = max(c.past_tiles + p.draft_tiles, 1);
+  c.tile = c.tiles * rank / n;
+  c.stop = c.tiles * (rank + 1) / n;
+  c.end = 0;
+  return c;
+}
+
+template <int kStorage, int DP, int RT, bool kTree, Mode kMode>
 __global__ void __launch_bounds__(kThreads, resident_blocks(kStorage, RT, DP)) pool_attn_mma_kernel(const wm_pool_attn_args a, const Plan plan) {
   constexpr int kRows = RT * 8, kPitch = DP + 4, kSide = joined_warps<DP, RT>();
   __shared__ __align__(16) float sm_acc[kSide][kRows][kPitch];
   __shared__ float sm_m[kWarps][kRows], sm_l[kWarps][kRows];
   __shared__ uint2 sm_q[Queries<DP, RT>::kShared ? RT * (DP / 16) * 32 : 1];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining kernel may take its place: it waits for this one's end
+  __shared__ float2 sm_sum[kMode == kCluster ? kRows : 1];  // reference and sum of the block's rows
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  Share share = find_share(a, plan, blockIdx.x, gridDim.x);
-  if (threadIdx.x == 0) note_of(a, blockIdx.x)->last = -1;
+  Share share = {0, 0, 1, 0, 0};
+  if (kMode != kCluster) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining kernel may take its place: it waits for this one's end
+    share = find_share(a, plan, blockIdx.x, gridDim.x);
+    if (threadIdx.x == 0) note_of(a, blockIdx.x)->last = -1;
+  }
   for (int at = share.begin; at < share.end;) {
-    const Piece c = next_piece(a, plan, at, share.end, share.b, share.b_begin);
-    at = c.end;
-    if (c.tile >= c.stop) continue;
+    const Piece c = kMode == kCluster ? cluster_piece(a, plan) : next_piece(a, plan, at, share.end, share.b, share.b_begin);
+    at = kMode == kCluster ? 1 : c.end;
+    if (kMode != kCluster && c.tile >= c.stop) continue;
 
     Queries<DP, RT> q;
     q.shared = sm_q;
@@ -534,8 +584,8 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(kStorage, RT, DP)) p
     }
     if (Queries<DP, RT>::kShared) __syncthreads();
 
-    if (c.tile < c.past_tiles) past_keys<kStorage, DP, RT, kDense>(a, c, c.tile, min(c.stop, c.past_tiles), q, st);
-    if (kTree && c.stop > c.past_tiles)
+    if (c.tile < c.past_tiles) past_keys<kStorage, DP, RT, kMode == kDenseShares>(a, c, c.tile, min(c.stop, c.past_tiles), q, st);
+    if (kTree && c.stop > c.past_tiles && c.stop > c.tile)
       draft_keys<kStorage, DP, RT>(a, plan, c, max(c.tile - c.past_tiles, 0), c.stop - c.past_tiles, q, st);
 
     // join the warps: references and sums first, then the accumulators
@@ -606,8 +656,14 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(kStorage, RT, DP)) p
       if (kTree && a.depths[(a.shared_tree ? 0ll : static_cast<long long>(c.b) * a.q_len) + token] < 0) empty = true;  // a padding node sees nothing
       const float inverse = 1.f / l;
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + c.b * a.out_strides[0] + head * a.out_strides[1] + token * a.out_strides[2];
-      float* partial = partial_row(a, plan, gridDim.x, blockIdx.x, c.tile == 0, r);
-      if (!whole(c) && threadIdx.x % kPerRow == 0) *reinterpret_cast<float2*>(partial) = make_float2(top, empty ? 0.f : l);
+      float* partial = kMode == kCluster ? nullptr : partial_row(a, plan, gridDim.x, blockIdx.x, c.tile == 0, r);
+      if (threadIdx.x % kPerRow == 0) {
+        const float2 sum = make_float2(top, empty ? 0.f : l);
+        if (kMode == kCluster)
+          sm_sum[r] = sum;
+        else if (!whole(c))
+          *reinterpret_cast<float2*>(partial) = sum;
+      }
       for (int d = 2 * (threadIdx.x % kPerRow); d < a.head_dim; d += 2 * kPerRow) {
         float2 y = *reinterpret_cast<const float2*>(&sm_acc[0][r][d]);
         if (kSide == kWarps) y.x *= f[0], y.y *= f[0];
@@ -618,62 +674,105 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(kStorage, RT, DP)) p
           y.y = fmaf(z.y, kSide == kWarps ? f[w] : 1.f, y.y);
         }
         if (empty) y = make_float2(0.f, 0.f);
-        if (whole(c))
+        if (kMode == kCluster)
+          *reinterpret_cast<float2*>(&sm_acc[0][r][d]) = y;  // its own place: no other thread has read or will write it
+        else if (whole(c))
           *reinterpret_cast<uint32_t*>(out + d) = empty ? 0u : pack_bf16(y.x * inverse, y.y * inverse);
         else
           *reinterpret_cast<float2*>(partial + 2 + d) = y;
       }
     }
-    if (threadIdx.x == 0) leave_note(a, share, c, blockIdx.x, gridDim.x);
-    __syncthreads();
-  }
-}
-
-template <int kStorage, int DP, int RT>
-void launch_mma(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream) {
-  if constexpr (DP % 64 == 0) {  // heads of 64 and 128 in a pool whose rows lie one behind the other: measured 125 us against 153 us
-    const bool scaled = kStorage != WM_BF16;
-    if (a.head_dim == DP && a.k_strides[2] == DP && a.v_strides[2] == DP && (!scaled || (a.k_scale_strides[2] == 1 && a.v_scale_strides[2] == 1))) {
-      if (a.ancestors != nullptr)
-        pool_attn_mma_kernel<kStorage, DP, RT, true, true><<<shares, kThreads, 0, stream>>>(a, plan);
-      else
-        pool_attn_mma_kernel<kStorage, DP, RT, false, true><<<shares, kThreads, 0, stream>>>(a, plan);
-      return;
+    if constexpr (kMode != kCluster) {
+      if (threadIdx.x == 0) leave_note(a, share, c, blockIdx.x, gridDim.x);
+      __syncthreads();
+    } else {
+      // every block finishes its part of the outputs from all blocks' sums
+      cluster_sync();
+      const int n = cluster_blocks(), pairs = a.head_dim / 2;
+      for (int i = cluster_rank() * kThreads + threadIdx.x; i < kRows * pairs; i += n * kThreads) {
+        const int row = i / pairs, d = 2 * (i - row * pairs);
+        row_place(a, plan, c.kv_head, c.row_block, row, token, head);
+        if (token >= a.q_len) continue;
+        float2 sum[kMaxCluster], y[kMaxCluster];
+        float top = kNoReference, l = 0.f;
+#pragma unroll
+        for (int o = 0; o < kMaxCluster; ++o) {
+          sum[o] = make_float2(kNoReference, 0.f);
+          y[o] = make_float2(0.f, 0.f);
+          if (o < n) {
+            sum[o] = load_remote(&sm_sum[row], o);
+            y[o] = load_remote(&sm_acc[0][row][d], o);
+          }
+          top = fmaxf(top, sum[o].x);
+        }
+        float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int o = 0; o < kMaxCluster; ++o) {
+          const float f = exp2_approx(sum[o].x - top);
+          l = fmaf(sum[o].y, f, l);
+          acc.x = fmaf(y[o].x, f, acc.x);
+          acc.y = fmaf(y[o].y, f, acc.y);
+        }
+        const float inverse = 1.f / l;
+        const long long place = c.b * a.out_strides[0] + head * a.out_strides[1] + token * a.out_strides[2] + d;
+        *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + place) = l == 0.f ? 0u : pack_bf16(acc.x * inverse, acc.y * inverse);
+      }
+      cluster_sync();  // no block leaves while another reads its shared memory
     }
   }
-  if (a.ancestors != nullptr)
-    pool_attn_mma_kernel<kStorage, DP, RT, true, false><<<shares, kThreads, 0, stream>>>(a, plan);
-  else
-    pool_attn_mma_kernel<kStorage, DP, RT, false, false><<<shares, kThreads, 0, stream>>>(a, plan);
 }
 
-template <int kStorage, int DP>
-void launch_mma_rows(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream) {
-  switch (plan.rows_per_block) {
-    case 8: return launch_mma<kStorage, DP, 1>(a, plan, shares, stream);
-    case 16: return launch_mma<kStorage, DP, 2>(a, plan, shares, stream);
-    case 32: return launch_mma<kStorage, DP, 4>(a, plan, shares, stream);
-    default:
-      if constexpr (DP <= 64) launch_mma<kStorage, DP, 8>(a, plan, shares, stream);
+template <int kStorage, int DP, int RT, bool kTree>
+cudaError_t launch_mma(const wm_pool_attn_args& a, const Plan& plan, cudaStream_t stream) {
+  if constexpr (RT <= 2) {
+    if (plan.cluster > 0) {
+      cudaLaunchAttribute dim = {};
+      dim.id = cudaLaunchAttributeClusterDimension;
+      dim.val.clusterDim.x = plan.cluster;
+      dim.val.clusterDim.y = dim.val.clusterDim.z = 1;
+      cudaLaunchConfig_t config = {};
+      config.gridDim = dim3(plan.blocks);
+      config.blockDim = dim3(kThreads);
+      config.stream = stream;
+      config.attrs = &dim;
+      config.numAttrs = 1;
+      return cudaLaunchKernelEx(&config, pool_attn_mma_kernel<kStorage, DP, RT, kTree, kCluster>, a, plan);
+    }
   }
+  if constexpr (DP % 64 == 0) {  // heads of 64 and 128, the usual pool: 142 us against 153 us on 64 sequences of up to 8192 int8 rows
+    const bool scaled = kStorage != WM_BF16;
+    if (a.head_dim == DP && a.k_strides[2] == DP && a.v_strides[2] == DP && (!scaled || (a.k_scale_strides[2] == 1 && a.v_scale_strides[2] == 1))) {
+      pool_attn_mma_kernel<kStorage, DP, RT, kTree, kDenseShares><<<plan.blocks, kThreads, 0, stream>>>(a, plan);
+      return cudaGetLastError();
+    }
+  }
+  pool_attn_mma_kernel<kStorage, DP, RT, kTree, kShares><<<plan.blocks, kThreads, 0, stream>>>(a, plan);
+  return cudaGetLastError();
 }
 
-template <int kStorage>
-void launch_mma_storage(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream) {
-  if (a.head_dim <= 32)
-    launch_mma_rows<kStorage, 32>(a, plan, shares, stream);
-  else if (a.head_dim <= 64)
-    launch_mma_rows<kStorage, 64>(a, plan, shares, stream);
-  else if (a.head_dim <= 96)
-    launch_mma_rows<kStorage, 96>(a, plan, shares, stream);
-  else
-    launch_mma_rows<kStorage, 128>(a, plan, shares, stream);
+template <int kStorage, int DP, bool kTree>
+cudaError_t launch_mma_rows(const wm_pool_attn_args& a, const Plan& plan, cudaStream_t stream) {
+  switch (plan.rows_per_block) {
+    case 8: return launch_mma<kStorage, DP, 1, kTree>(a, plan, stream);
+    case 16: return launch_mma<kStorage, DP, 2, kTree>(a, plan, stream);
+    case 32: return launch_mma<kStorage, DP, 4, kTree>(a, plan, stream);
+  }
+  if constexpr (DP <= 64) return launch_mma<kStorage, DP, 8, kTree>(a, plan, stream);
+  return cudaErrorInvalidValue;  // not reached: 64 rows are planned for heads of up to 64 alone
 }
 
-// One translation unit per way of holding the pool.
-void launch_mma_bf16(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream);
-void launch_mma_int8(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream);
-void launch_mma_e4m3(const wm_pool_attn_args& a, const Plan& plan, int shares, cudaStream_t stream);
+// One translation unit per way of holding the pool, with and without drafted tokens.
+template <int kStorage, bool kTree>
+cudaError_t launch_mma_storage(const wm_pool_attn_args& a, const Plan& plan, cudaStream_t stream);
+
+#define WM_POOL_ATTN_UNIT(kStorage, kTree)                                                                                          \
+  template <>                                                                                                                       \
+  cudaError_t launch_mma_storage<kStorage, kTree>(const wm_pool_attn_args& a, const Plan& plan, cudaStream_t stream) {              \
+    if (a.head_dim <= 32) return launch_mma_rows<kStorage, 32, kTree>(a, plan, stream);                                             \
+    if (a.head_dim <= 64) return launch_mma_rows<kStorage, 64, kTree>(a, plan, stream);                                             \
+    if (a.head_dim <= 96) return launch_mma_rows<kStorage, 96, kTree>(a, plan, stream);                                             \
+    return launch_mma_rows<kStorage, 128, kTree>(a, plan, stream);                                                                  \
+  }
 
 // Rows of a block: as many tiles of 8 as the rows of a KV head fill, up to what the registers hold.
 inline int mma_rows_per_block(long long rows, int head_dim) {

@@ -26,6 +26,8 @@ struct Plan {
   int row_blocks;      // of rows_per_block rows, per KV head
   int rows_per_block;
   int draft_tiles;
+  int blocks;   // of the launch: shares, or blocks of all clusters
+  int cluster;  // blocks per cluster, 0 where the launch works in shares
 };
 
 // Slots that the queries of sequence b may see: the dummy and the committed tokens.

@@ -242,8 +242,9 @@ def pool_attention(
     a.kv_heads, a.k_len, a.lead = kv_heads, slots, int(use_dummy_token)
     a.scale = dim**-0.5 if softmax_scale is None else float(softmax_scale)
     nbytes = _native.load_library().wm_pool_attn_workspace_bytes(_native.ctypes.byref(a))
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
-    a.workspace, a.workspace_bytes = workspace.data_ptr(), nbytes
+    if nbytes:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), nbytes
     _native.call("wm_pool_attn", a, query.device)
     return out
 
