@@ -94,6 +94,9 @@ SHAPES = [  # batch, heads, kv_heads, tokens, slots, dim, lead, masked, lengths
     (2, 6, 1, 33, 140, 48, 0, False, None),
     (1, 2, 2, 130, 200, 96, 1, False, [70]),
     (1, 2, 1, 300, 10, 64, 0, False, [0]),
+    (2, 4, 2, 6, 4300, 64, 1, True, [4300, 40]),
+    (2, 4, 1, 12, 4300, 128, 0, False, [4300, 130]),
+    (30, 2, 1, 20, 140, 64, 1, False, [5 * i for i in range(30)]),
 ]
 
 

@@ -295,6 +295,14 @@ SHAPES = [  # batch, heads, kv_heads, tokens, slots, dim, lead, masked, lengths
     (2, 16, 2, 17, 200, 96, 1, True, [200, 64]),
     (1, 3, 3, 40, 700, 64, 0, False, [650]),
     (300, 1, 1, 1, 40, 64, 0, False, [i % 41 for i in range(300)]),
+    # beyond what one cluster per segment takes: shares of tiles, segments across shares
+    (3, 4, 2, 1, 4300, 64, 0, False, [4300, 0, 129]),
+    (2, 2, 1, 3, 4300, 128, 1, True, [4000, 77]),
+    (2, 9, 1, 1, 4200, 80, 0, False, [1, 4200]),
+    # many rows per KV head
+    (2, 4, 1, 16, 4300, 64, 1, False, [4300, 200]),
+    (1, 3, 1, 40, 1000, 112, 0, True, [990]),
+    (40, 4, 2, 9, 150, 64, 0, False, [3 * i for i in range(40)]),
 ]
 
 

@@ -755,10 +755,8 @@ cudaError_t launch_mma_rows(const wm_pool_attn_args& a, const Plan& plan, cudaSt
   switch (plan.rows_per_block) {
     case 8: return launch_mma<kStorage, DP, 1, kTree>(a, plan, stream);
     case 16: return launch_mma<kStorage, DP, 2, kTree>(a, plan, stream);
-    case 32: return launch_mma<kStorage, DP, 4, kTree>(a, plan, stream);
   }
-  if constexpr (DP <= 64) return launch_mma<kStorage, DP, 8, kTree>(a, plan, stream);
-  return cudaErrorInvalidValue;  // not reached: 64 rows are planned for heads of up to 64 alone
+  return cudaErrorInvalidValue;  // not reached
 }
 
 // One translation unit per way of holding the pool, with and without drafted tokens.
@@ -775,10 +773,9 @@ cudaError_t launch_mma_storage(const wm_pool_attn_args& a, const Plan& plan, cud
   }
 
 // Rows of a block: as many tiles of 8 as the rows of a KV head fill, up to what the registers hold.
-inline int mma_rows_per_block(long long rows, int head_dim) {
-  const int most = head_dim <= 64 ? 64 : 32;
+inline int mma_rows_per_block(long long rows) {
   int n = 8;
-  while (n < most && n < rows) n *= 2;
+  while (n < 64 && n < rows) n *= 2;
   return n;
 }
 
