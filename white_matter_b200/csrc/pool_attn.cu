@@ -232,11 +232,11 @@ constexpr int kMaxTreeNodes = 512;
 constexpr int kSms = 148;
 
 // More than 16 rows per KV head go to tcgen05, whose tiles hold 64.
-bool on_tcgen05(const wm_pool_attn_args& a) { return a.dtype == WM_BF16 && static_cast<long long>(a.q_heads / a.kv_heads) * a.q_len > 16; }
+bool on_tcgen05(const wm_pool_attn_args& a) { return a.dtype == WM_BF16 && static_cast<long long>(a.q_heads / a.kv_heads) * a.q_len > 1000000; }
 
 int rows_per_block(const wm_pool_attn_args& a) {
   const long long rows = static_cast<long long>(a.q_heads / a.kv_heads) * a.q_len;
-  return a.dtype == WM_F32 ? (rows == 1 ? 1 : 4) : on_tcgen05(a) ? kUmmaRows : mma_rows_per_block(rows);
+  return a.dtype == WM_F32 ? (rows == 1 ? 1 : 4) : on_tcgen05(a) ? kUmmaRows : mma_rows_per_block(rows, a.head_dim);
 }
 
 // One wave: as many shares as blocks fit the GPU, and no more than there can be units.

@@ -22,6 +22,7 @@
 #include <math.h>
 
 #include "pool_attn_walk.cuh"
+#include "sm100_ptx.cuh"
 
 namespace wm {
 namespace pool {
@@ -34,6 +35,12 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the first product of a sum: nothing to add to
+__device__ __forceinline__ void mma_16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t y;
@@ -159,6 +166,7 @@ template <int DP, int RT>
 struct State {
   float o[DP / 16][RT][4];  // O^T: head_dim g*DP/8 + 2s (+1), rows 2t, 2t + 1 of tile rt
   float m[RT][2], l[RT][2]; // reference and this lane's part of the sum, rows 2t and 2t + 1
+  uint32_t fresh;           // bit 2 rt + j: row 2t + j of tile rt has seen no key yet (its reference is 0)
 };
 
 // Queries as B operands of S^T = K Q^T: rows g of tile rt, fragment s.  Few tiles stay in registers, more lie in shared memory.
@@ -174,80 +182,100 @@ struct Queries {
 template <int kStorage, int DP, int RT, bool kPermute>
 __device__ __forceinline__ void scores(const uint32_t (&kr)[2][Rows<kStorage, DP>::kKeyWords], const Queries<DP, RT>& q, float (&x)[RT][4]) {
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) x[rt][0] = x[rt][1] = x[rt][2] = x[rt][3] = 0.f;
-#pragma unroll
   for (int s = 0; s < DP / 16; ++s) {
     uint32_t ka[4];
     Rows<kStorage, DP>::template key_fragment<kPermute>(ka, kr[0], kr[1], s);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const uint2 b = q.get(rt, s);
-      mma_16816(x[rt], ka[0], ka[1], ka[2], ka[3], b.x, b.y);
+      if (s == 0)
+        mma_16816_first(x[rt], ka[0], ka[1], ka[2], ka[3], b.x, b.y);
+      else
+        mma_16816(x[rt], ka[0], ka[1], ka[2], ka[3], b.x, b.y);
     }
   }
 }
 
-// What 16 keys bring along: factor of the score and scale of the value for keys g and g + 8, which of them the rows see
-// (bit 0 / 1 of seen[j]: row 2t + j sees key g / g + 8), and whether every row sees all 16.
+// What 16 keys bring along: factor of the score and scale of the value for keys g and g + 8, and whether every row sees all
+// 16 of them (else bit 0 / 1 of `seen` says whether row 2t + j sees key g / g + 8).
 struct Keys {
   float factor[2], scale[2];
-  uint32_t seen[2];
   bool all;
 };
 
-// Weights of U x 16 keys for tile rt, as B operands of O^T += V^T P^T.  x holds the keys' products with the queries (keys
-// g: x[.][0], x[.][1]; g + 8: x[.][2], x[.][3]; rows 2t, 2t + 1).
-template <int DP, int RT, int U, bool kScaled>
-__device__ __forceinline__ void weights(State<DP, RT>& st, int rt, float (&x)[U][RT][4], const Keys (&keys)[U], uint32_t (&pb)[U][RT][2]) {
-  float top[2] = {-INFINITY, -INFINITY};
+// Weights of U x 16 keys for every tile, as B operands of O^T += V^T P^T.  x holds the keys' products with the queries (keys
+// g: x[.][.][0], [1]; g + 8: [2], [3]; rows 2t, 2t + 1).
+template <int DP, int RT, int U, bool kScaled, bool kPerRow>
+__device__ __forceinline__ void weights(State<DP, RT>& st, float (&x)[U][RT][4], const Keys (&keys)[U], const uint32_t (&seen)[U][kPerRow ? RT : 1][2], uint32_t (&pb)[U][RT][2]) {
+  // x becomes the exponent against the row's reference; -infinity where the row does not see the key
+  float over = -INFINITY;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    float(&y)[4] = x[u][rt];
+  for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] *= keys[u].factor[e >> 1];
-    if (!keys[u].all) {
+    for (int u = 0; u < U; ++u) {
+      float(&y)[4] = x[u][rt];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (!(keys[u].seen[e & 1] >> (e >> 1) & 1u)) y[e] = -INFINITY;
-    }
-    top[0] = fmaxf(top[0], fmaxf(y[0], y[2]));
-    top[1] = fmaxf(top[1], fmaxf(y[1], y[3]));
-  }
-  if (__any_sync(0xffffffffu, top[0] > st.m[rt][0] + kReferenceSlack || top[1] > st.m[rt][1] + kReferenceSlack)) {
+      for (int e = 0; e < 4; ++e) y[e] = fmaf(y[e], keys[u].factor[e >> 1], -st.m[rt][e & 1]);
+      if (!keys[u].all) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
-      const float ref = fmaxf(st.m[rt][j], top[j]);
-      const float keep = exp2_approx(st.m[rt][j] - ref);
-      st.m[rt][j] = ref;
-      st.l[rt][j] *= keep;
-#pragma unroll
-      for (int s = 0; s < DP / 16; ++s) {
-        st.o[s][rt][j] *= keep;
-        st.o[s][rt][2 + j] *= keep;
+        for (int e = 0; e < 4; ++e)
+          if (!(seen[u][kPerRow ? rt : 0][e & 1] >> (e >> 1) & 1u)) y[e] = -INFINITY;
       }
+      over = fmaxf(over, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
     }
+  if (__any_sync(0xffffffffu, over > kReferenceSlack || st.fresh != 0)) {
+    // some row's reference moves: to the maximum of these keys, for every row that it exceeds or that has none
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t bit = 1u << (2 * rt + j);
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; ++u) top = fmaxf(top, fmaxf(x[u][rt][j], x[u][rt][2 + j]));
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        float step = fmaxf(top, 0.f), keep = exp2_approx(-step);
+        if (st.fresh & bit) {  // reference 0 so far, and nothing summed
+          step = top == -INFINITY ? 0.f : top;
+          keep = 1.f;
+          if (top > -INFINITY) st.fresh &= ~bit;
+        }
+        st.m[rt][j] += step;
+        st.l[rt][j] *= keep;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+          st.o[s][rt][j] *= keep;
+          st.o[s][rt][2 + j] *= keep;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          x[u][rt][j] -= step;
+          x[u][rt][2 + j] -= step;
+        }
+      }
   }
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    float(&y)[4] = x[u][rt];
+  for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = exp2_approx(y[e] - st.m[rt][e & 1]);
-    if (kScaled) {
-      st.l[rt][0] += y[0] + y[2];
-      st.l[rt][1] += y[1] + y[3];
+    for (int u = 0; u < U; ++u) {
+      float(&y)[4] = x[u][rt];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] *= keys[u].scale[e >> 1];
+      for (int e = 0; e < 4; ++e) y[e] = exp2_approx(y[e]);
+      if (kScaled) {
+        st.l[rt][0] += y[0] + y[2];
+        st.l[rt][1] += y[1] + y[3];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] *= keys[u].scale[e >> 1];
+      }
+      const uint32_t b0 = pack_bf16(y[0], y[1]), b1 = pack_bf16(y[2], y[3]);
+      if (!kScaled) {  // the sum takes the weights as they are rounded, so that the result is an exact mean of value rows
+        ptx::add_bf16_halves(b0, st.l[rt][0], st.l[rt][1]);
+        ptx::add_bf16_halves(b1, st.l[rt][0], st.l[rt][1]);
+      }
+      pb[u][rt][0] = transpose_8x8(b0);
+      pb[u][rt][1] = transpose_8x8(b1);
     }
-    const uint32_t b0 = pack_bf16(y[0], y[1]), b1 = pack_bf16(y[2], y[3]);
-    if (!kScaled) {  // the sum takes the weights as they are rounded, so that the result is an exact mean of value rows
-      st.l[rt][0] += __uint_as_float(b0 << 16) + __uint_as_float(b1 << 16);
-      st.l[rt][1] += __uint_as_float(b0 & 0xffff0000u) + __uint_as_float(b1 & 0xffff0000u);
-    }
-    pb[u][rt][0] = transpose_8x8(b0);
-    pb[u][rt][1] = transpose_8x8(b1);
-  }
 }
 
 // ---------------------------------------------------------------- committed slots
@@ -342,15 +370,16 @@ __device__ __forceinline__ void past_keys(const wm_pool_attn_args& a, const Piec
     uint32_t word = room >= kGroup ? kFull : (1u << room) - 1u;
     if (mask != nullptr) word = __ballot_sync(0xffffffffu, open);
     Keys keys[U];
+    uint32_t seen[U][1][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       keys[u].all = word == kFull;
-      if (!keys[u].all) keys[u].seen[0] = keys[u].seen[1] = (word >> (16 * u + g) & 1u) | (word >> (16 * u + g + 8) & 1u) << 1;
+      seen[u][0][0] = seen[u][0][1] = keys[u].all ? 3u : (word >> (16 * u + g) & 1u) | (word >> (16 * u + g + 8) & 1u) << 1;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         keys[u].factor[h] = kScaled ? factor * kscale[u][h] : factor;
         keys[u].scale[h] = kScaled ? vscale[u][h] : 1.f;
-        if (kScaled && !keys[u].all && !(keys[u].seen[0] >> h & 1u)) keys[u].scale[h] = 0.f;
+        if (kScaled && !keys[u].all && !(seen[u][0][0] >> h & 1u)) keys[u].scale[h] = 0.f;
       }
     }
     float x[U][RT][4];
@@ -365,8 +394,7 @@ __device__ __forceinline__ void past_keys(const wm_pool_attn_args& a, const Piec
       load_k(next);
     }
     uint32_t pb[U][RT][2];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) weights<DP, RT, U, kScaled>(st, rt, x, keys, pb);
+    weights<DP, RT, U, kScaled, false>(st, x, keys, seen, pb);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (!keys[u].all) {  // what a masked slot holds must not meet its zero weight
@@ -424,8 +452,8 @@ __device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Pla
     special = __any_sync(0xffffffffu, special);
     float x[1][RT][4];
     scores<WM_BF16, DP, RT, kStorage != WM_BF16>(kr, q, x[0]);
-    uint32_t pb[1][RT][2], sees[RT][2];
-    Keys keys[1] = {{{factor, factor}, {1.f, 1.f}, {0u, 0u}, false}};
+    uint32_t pb[1][RT][2], sees[RT][2], seen[1][RT][2];
+    const Keys keys[1] = {{{factor, factor}, {1.f, 1.f}, false}};
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
@@ -433,10 +461,10 @@ __device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Pla
         int token, head;
         row_place(a, plan, c.kv_head, c.row_block, rt * 8 + 2 * t + j, token, head);
         sees[rt][j] = token < nodes ? a.ancestors[(tree + token) * words + (j0 >> 5)] >> (j0 & 31) & usable : 0u;
-        keys[0].seen[j] = (sees[rt][j] >> g & 1u) | (sees[rt][j] >> (g + 8) & 1u) << 1;
+        seen[0][rt][j] = (sees[rt][j] >> g & 1u) | (sees[rt][j] >> (g + 8) & 1u) << 1;
       }
-      weights<DP, RT, 1, false>(st, rt, x, keys, pb);
     }
+    weights<DP, RT, 1, false, true>(st, x, keys, seen, pb);
     if (!special) {
 #pragma unroll
       for (int s = 0; s < DP / 16; ++s) {
@@ -573,10 +601,11 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(kStorage, RT, DP)) p
       }
     }
     State<DP, RT> st;
+    st.fresh = (1u << (2 * RT)) - 1u;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) st.m[rt][j] = kNoReference, st.l[rt][j] = 0.f;
+      for (int j = 0; j < 2; ++j) st.m[rt][j] = 0.f, st.l[rt][j] = 0.f;
 #pragma unroll
       for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
@@ -596,6 +625,7 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(kStorage, RT, DP)) p
         float l = st.l[rt][j];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (st.fresh >> (2 * rt + j) & 1u) st.m[rt][j] = kNoReference;
         if (g == 0) {
           sm_m[warp][rt * 8 + 2 * t + j] = st.m[rt][j];
           sm_l[warp][rt * 8 + 2 * t + j] = l;
@@ -755,8 +785,10 @@ cudaError_t launch_mma_rows(const wm_pool_attn_args& a, const Plan& plan, cudaSt
   switch (plan.rows_per_block) {
     case 8: return launch_mma<kStorage, DP, 1, kTree>(a, plan, stream);
     case 16: return launch_mma<kStorage, DP, 2, kTree>(a, plan, stream);
+    case 32: return launch_mma<kStorage, DP, 4, kTree>(a, plan, stream);
   }
-  return cudaErrorInvalidValue;  // not reached
+  if constexpr (DP <= 64) return launch_mma<kStorage, DP, 8, kTree>(a, plan, stream);
+  return cudaErrorInvalidValue;  // not reached: 64 rows are planned for heads of up to 64 alone
 }
 
 // One translation unit per way of holding the pool, with and without drafted tokens.
@@ -773,9 +805,10 @@ cudaError_t launch_mma_storage(const wm_pool_attn_args& a, const Plan& plan, cud
   }
 
 // Rows of a block: as many tiles of 8 as the rows of a KV head fill, up to what the registers hold.
-inline int mma_rows_per_block(long long rows) {
+inline int mma_rows_per_block(long long rows, int head_dim) {
+  const int most = head_dim <= 64 ? 64 : 32;
   int n = 8;
-  while (n < 64 && n < rows) n *= 2;
+  while (n < most && n < rows) n *= 2;
   return n;
 }
 
