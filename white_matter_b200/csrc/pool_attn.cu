@@ -5,7 +5,7 @@
 
 #include <atomic>
 
-#include "pool_attn_umma.cuh"
+#include "pool_attn_shared.cuh"
 
 namespace wm {
 namespace {
@@ -231,18 +231,20 @@ __global__ void __launch_bounds__(kJoinThreads) pool_attn_join_kernel(const wm_p
 constexpr int kMaxTreeNodes = 512;
 constexpr int kSms = 148;
 
-// More than 16 rows per KV head go to tcgen05, whose tiles hold 64.
-bool on_tcgen05(const wm_pool_attn_args& a) { return a.dtype == WM_BF16 && static_cast<long long>(a.q_heads / a.kv_heads) * a.q_len > 1000000; }
+long long rows_of(const wm_pool_attn_args& a) { return static_cast<long long>(a.q_heads / a.kv_heads) * a.q_len; }
+
+// More than 16 rows per KV head share the pool rows of a block through shared memory.
+bool in_shared(const wm_pool_attn_args& a) { return a.dtype == WM_BF16 && rows_of(a) > 16; }
 
 int rows_per_block(const wm_pool_attn_args& a) {
-  const long long rows = static_cast<long long>(a.q_heads / a.kv_heads) * a.q_len;
-  return a.dtype == WM_F32 ? (rows == 1 ? 1 : 4) : on_tcgen05(a) ? kUmmaRows : mma_rows_per_block(rows, a.head_dim);
+  const long long rows = rows_of(a);
+  return a.dtype == WM_F32 ? (rows == 1 ? 1 : 4) : in_shared(a) ? shared_rows_per_block(rows, a.storage, a.head_dim) : mma_rows_per_block(rows, a.head_dim);
 }
 
 // One wave: as many shares as blocks fit the GPU, and no more than there can be units.
 int count_shares(const wm_pool_attn_args& a, const Plan& p) {
   const double tiles = static_cast<double>((a.k_len + kTileKeys - 1) / kTileKeys + p.draft_tiles + kSegmentCost) * a.batch * a.kv_heads * p.row_blocks;
-  const int wave = kSms * (a.dtype == WM_F32 ? 6 : on_tcgen05(a) ? 1 : resident_blocks(a.storage, p.rows_per_block / 8, a.head_dim));
+  const int wave = kSms * (a.dtype == WM_F32 ? 6 : in_shared(a) ? 2 : resident_blocks(a.storage, p.rows_per_block / 8, a.head_dim));
   return tiles < wave ? (tiles < 1 ? 1 : static_cast<int>(tiles)) : wave;
 }
 
@@ -333,12 +335,9 @@ int pool_attn_launch(const wm_pool_attn_args& a, cudaStream_t stream) {
   if (need > 0 && (a.workspace == nullptr || a.workspace_bytes < need)) return fail(WM_EWORKSPACE, "wm_pool_attn needs %zu workspace bytes, got %zu", need, a.workspace_bytes);
   const bool tree = a.ancestors != nullptr;
   cudaError_t launched;
-  if (on_tcgen05(a)) {
-    int* word = nullptr;
-    const int found = tc_status_word(&word);
-    if (found != WM_OK) return found;
-    launched = a.storage == WM_INT8 ? launch_umma<WM_INT8>(a, plan, word, stream) : a.storage == WM_E4M3 ? launch_umma<WM_E4M3>(a, plan, word, stream) : launch_umma<WM_BF16>(a, plan, word, stream);
-  } else if (a.dtype == WM_F32)
+  if (in_shared(a))
+    launched = a.storage == WM_INT8 ? launch_shared<WM_INT8>(a, plan, stream) : a.storage == WM_E4M3 ? launch_shared<WM_E4M3>(a, plan, stream) : launch_shared<WM_BF16>(a, plan, stream);
+  else if (a.dtype == WM_F32)
     launched = a.storage == WM_INT8 ? launch_simt<WM_INT8>(a, plan, stream) : a.storage == WM_E4M3 ? launch_simt<WM_E4M3>(a, plan, stream) : launch_simt<WM_F32>(a, plan, stream);
   else if (a.storage == WM_INT8)
     launched = tree ? launch_mma_storage<WM_INT8, true>(a, plan, stream) : launch_mma_storage<WM_INT8, false>(a, plan, stream);
