@@ -238,12 +238,12 @@ bool in_shared(const wm_pool_attn_args& a) { return a.dtype == WM_BF16 && rows_o
 
 int rows_per_block(const wm_pool_attn_args& a) {
   const long long rows = rows_of(a);
-  return a.dtype == WM_F32 ? (rows == 1 ? 1 : 4) : in_shared(a) ? shared_rows_per_block(rows, a.storage, a.head_dim) : mma_rows_per_block(rows, a.head_dim);
+  return a.dtype == WM_F32 ? (rows == 1 ? 1 : 4) : in_shared(a) ? shared_rows_per_block(rows, a.storage, a.head_dim) : rows <= 8 ? 8 : 16;
 }
 
 // One wave: as many shares as blocks fit the GPU, and no more than there can be units.
 int count_shares(const wm_pool_attn_args& a, const Plan& p) {
-  const double tiles = static_cast<double>((a.k_len + kTileKeys - 1) / kTileKeys + p.draft_tiles + kSegmentCost) * a.batch * a.kv_heads * p.row_blocks;
+  const double tiles = static_cast<double>((a.k_len + kTileKeys - 1) / kTileKeys + p.draft_tiles + p.segment_cost) * a.batch * a.kv_heads * p.row_blocks;
   const int wave = kSms * (a.dtype == WM_F32 ? 6 : in_shared(a) ? 2 : resident_blocks(a.storage, p.rows_per_block / 8, a.head_dim));
   return tiles < wave ? (tiles < 1 ? 1 : static_cast<int>(tiles)) : wave;
 }
@@ -262,10 +262,13 @@ int cluster_size(const wm_pool_attn_args& a, const Plan& p) {
 bool make_plan(const wm_pool_attn_args& a, Plan& p) {
   const long long rows = static_cast<long long>(a.q_heads / a.kv_heads) * a.q_len;
   p.rows_per_block = rows_per_block(a);
+  // measured with 1, 2, 4, 6: 241, 227, 197, 209 us on 64 sequences with 32 drafted tokens (shared memory, heads of 64); 113, 118, 126 us on
+  // 8 sequences with 41 and 4 heads per group (heads of 128); 143, 143, 147, 150 us on 64 sequences with one token
+  p.segment_cost = in_shared(a) ? (a.head_dim <= 64 ? 4 : 1) : 2;
   const long long blocks = (rows + p.rows_per_block - 1) / p.rows_per_block;
   p.draft_tiles = a.ancestors != nullptr ? (a.q_len + kTileKeys - 1) / kTileKeys : 0;
   p.group = a.q_heads / a.kv_heads;
-  const double units = (static_cast<double>(a.k_len) / kTileKeys + 2 + kSegmentCost + p.draft_tiles) * a.batch * a.kv_heads * blocks;
+  const double units = (static_cast<double>(a.k_len) / kTileKeys + 2 + p.segment_cost + p.draft_tiles) * a.batch * a.kv_heads * blocks;
   if (units >= INT_MAX || rows > INT_MAX) return false;  // the kernels count in 32 bits
   p.row_blocks = static_cast<int>(blocks);
   p.cluster = cluster_size(a, p);

@@ -504,14 +504,7 @@ __device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Pla
 // Blocks of 128 threads that fit an SM together, from the registers that the accumulators, the rows in flight and the
 // queries take; the launch holds the compiler to it, and the grid is one wave of them.
 __host__ __device__ constexpr int resident_blocks(int storage, int row_tiles, int padded_dim) {
-  return padded_dim > 64 ? (row_tiles == 1 || (row_tiles == 2 && storage != WM_BF16) ? 3 : 2) : (row_tiles == 1 ? 4 : row_tiles <= 4 ? 3 : 2);
-}
-
-// Shared memory joins the warps at the end of a piece: four accumulators side by side where they fit, else two, to which the
-// other two warps add theirs.
-template <int DP, int RT>
-__host__ __device__ constexpr int joined_warps() {
-  return RT * DP <= 256 ? kWarps : 2;
+  return padded_dim > 64 ? (row_tiles == 1 || storage != WM_BF16 ? 3 : 2) : (row_tiles == 1 ? 4 : 3);
 }
 
 // How the blocks of a launch share the work.
@@ -562,8 +555,8 @@ __device__ __forceinline__ Piece cluster_piece(const wm_pool_attn_args& a, const
 
 template <int kStorage, int DP, int RT, bool kTree, Mode kMode>
 __global__ void __launch_bounds__(kThreads, resident_blocks(kStorage, RT, DP)) pool_attn_mma_kernel(const wm_pool_attn_args a, const Plan plan) {
-  constexpr int kRows = RT * 8, kPitch = DP + 4, kSide = joined_warps<DP, RT>();
-  __shared__ __align__(16) float sm_acc[kSide][kRows][kPitch];
+  constexpr int kRows = RT * 8, kPitch = DP + 4;
+  __shared__ __align__(16) float sm_acc[kWarps][kRows][kPitch];
   __shared__ float sm_m[kWarps][kRows], sm_l[kWarps][kRows];
   __shared__ uint2 sm_q[Queries<DP, RT>::kShared ? RT * (DP / 16) * 32 : 1];
   __shared__ float2 sm_sum[kMode == kCluster ? kRows : 1];  // reference and sum of the block's rows
@@ -617,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(kStorage, RT, DP)) p
     if (kTree && c.stop > c.past_tiles && c.stop > c.tile)
       draft_keys<kStorage, DP, RT>(a, plan, c, max(c.tile - c.past_tiles, 0), c.stop - c.past_tiles, q, st);
 
-    // join the warps: references and sums first, then the accumulators
+    // join the warps: references, sums and accumulators side by side
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -632,41 +625,15 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(kStorage, RT, DP)) p
         }
       }
     const int d0 = Rows<WM_BF16, DP>::value_piece(g, a.head_dim * 2) / 2;
-    if (kSide < kWarps) __syncthreads();  // the references of all warps
 #pragma unroll
-    for (int turn = 0; turn < kWarps / kSide; ++turn) {
-      if (warp / kSide == turn) {
+    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int r = rt * 8 + 2 * t + j;
-            float f = 1.f;
-            if (kSide < kWarps) {
-              float top = sm_m[0][r];
-#pragma unroll
-              for (int o = 1; o < kWarps; ++o) top = fmaxf(top, sm_m[o][r]);
-              f = exp2_approx(st.m[rt][j] - top);
-            }
-            float2 y[DP / 16];
-#pragma unroll
-            for (int s = 0; s < DP / 16; ++s) y[s] = make_float2(st.o[s][rt][j] * f, st.o[s][rt][2 + j] * f);
-            float* row = &sm_acc[warp % kSide][r][d0];
-            if (turn > 0) {
-#pragma unroll
-              for (int s = 0; s < DP / 16; ++s) {
-                const float2 z = *reinterpret_cast<const float2*>(row + 2 * s);
-                y[s].x += z.x;
-                y[s].y += z.y;
-              }
-            }
-#pragma unroll
-            for (int s = 0; s < DP / 16; ++s)
-              if (d0 + 2 * s >= g * (DP / 8)) *reinterpret_cast<float2*>(row + 2 * s) = y[s];  // else a lower lane's
-          }
-      }
-      __syncthreads();
-    }
+        for (int s = 0; s < DP / 16; ++s)
+          if (d0 + 2 * s >= g * (DP / 8))  // else a lower lane's
+            *reinterpret_cast<float2*>(&sm_acc[warp][rt * 8 + 2 * t + j][d0 + 2 * s]) = make_float2(st.o[s][rt][j], st.o[s][rt][2 + j]);
+    __syncthreads();
 
     // one row per thread group
     constexpr int kPerRow = kRows < kThreads ? kThreads / kRows : 1;
@@ -696,12 +663,12 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(kStorage, RT, DP)) p
       }
       for (int d = 2 * (threadIdx.x % kPerRow); d < a.head_dim; d += 2 * kPerRow) {
         float2 y = *reinterpret_cast<const float2*>(&sm_acc[0][r][d]);
-        if (kSide == kWarps) y.x *= f[0], y.y *= f[0];
+        y.x *= f[0], y.y *= f[0];
 #pragma unroll
-        for (int w = 1; w < kSide; ++w) {
+        for (int w = 1; w < kWarps; ++w) {
           const float2 z = *reinterpret_cast<const float2*>(&sm_acc[w][r][d]);
-          y.x = fmaf(z.x, kSide == kWarps ? f[w] : 1.f, y.x);
-          y.y = fmaf(z.y, kSide == kWarps ? f[w] : 1.f, y.y);
+          y.x = fmaf(z.x, f[w], y.x);
+          y.y = fmaf(z.y, f[w], y.y);
         }
         if (empty) y = make_float2(0.f, 0.f);
         if (kMode == kCluster)
@@ -754,20 +721,18 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(kStorage, RT, DP)) p
 
 template <int kStorage, int DP, int RT, bool kTree>
 cudaError_t launch_mma(const wm_pool_attn_args& a, const Plan& plan, cudaStream_t stream) {
-  if constexpr (RT <= 2) {
-    if (plan.cluster > 0) {
-      cudaLaunchAttribute dim = {};
-      dim.id = cudaLaunchAttributeClusterDimension;
-      dim.val.clusterDim.x = plan.cluster;
-      dim.val.clusterDim.y = dim.val.clusterDim.z = 1;
-      cudaLaunchConfig_t config = {};
-      config.gridDim = dim3(plan.blocks);
-      config.blockDim = dim3(kThreads);
-      config.stream = stream;
-      config.attrs = &dim;
-      config.numAttrs = 1;
-      return cudaLaunchKernelEx(&config, pool_attn_mma_kernel<kStorage, DP, RT, kTree, kCluster>, a, plan);
-    }
+  if (plan.cluster > 0) {
+    cudaLaunchAttribute dim = {};
+    dim.id = cudaLaunchAttributeClusterDimension;
+    dim.val.clusterDim.x = plan.cluster;
+    dim.val.clusterDim.y = dim.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(plan.blocks);
+    config.blockDim = dim3(kThreads);
+    config.stream = stream;
+    config.attrs = &dim;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, pool_attn_mma_kernel<kStorage, DP, RT, kTree, kCluster>, a, plan);
   }
   if constexpr (DP % 64 == 0) {  // heads of 64 and 128, the usual pool: 142 us against 153 us on 64 sequences of up to 8192 int8 rows
     const bool scaled = kStorage != WM_BF16;
@@ -785,10 +750,8 @@ cudaError_t launch_mma_rows(const wm_pool_attn_args& a, const Plan& plan, cudaSt
   switch (plan.rows_per_block) {
     case 8: return launch_mma<kStorage, DP, 1, kTree>(a, plan, stream);
     case 16: return launch_mma<kStorage, DP, 2, kTree>(a, plan, stream);
-    case 32: return launch_mma<kStorage, DP, 4, kTree>(a, plan, stream);
   }
-  if constexpr (DP <= 64) return launch_mma<kStorage, DP, 8, kTree>(a, plan, stream);
-  return cudaErrorInvalidValue;  // not reached: 64 rows are planned for heads of up to 64 alone
+  return cudaErrorInvalidValue;  // not reached: more than 16 rows go through shared memory (pool_attn_shared.cuh)
 }
 
 // One translation unit per way of holding the pool, with and without drafted tokens.
@@ -803,14 +766,6 @@ cudaError_t launch_mma_storage(const wm_pool_attn_args& a, const Plan& plan, cud
     if (a.head_dim <= 96) return launch_mma_rows<kStorage, 96, kTree>(a, plan, stream);                                             \
     return launch_mma_rows<kStorage, 128, kTree>(a, plan, stream);                                                                  \
   }
-
-// Rows of a block: as many tiles of 8 as the rows of a KV head fill, up to what the registers hold.
-inline int mma_rows_per_block(long long rows, int head_dim) {
-  const int most = head_dim <= 64 ? 64 : 32;
-  int n = 8;
-  while (n < most && n < rows) n *= 2;
-  return n;
-}
 
 }  // namespace pool
 }  // namespace wm

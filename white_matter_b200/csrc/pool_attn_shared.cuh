@@ -42,7 +42,7 @@ struct BlockShared {
     float acc[kSide][kRowGroups * 16][kPitch];           // at the end of a piece: sums of two sets of warps
   };
   uint4 raw[kStorage == WM_BF16 ? 1 : 2 * C::kPasses][kStorage == WM_BF16 ? 1 : kBlockThreads];  // a step's codes, a corner per thread
-  unsigned char q[DP > 64 ? kRowGroups * 16 * C::kRowBytes : 16];
+  alignas(256) unsigned char q[DP > 64 ? kRowGroups * 16 * C::kRowBytes : 16];
   float scale[C::kStages][2][C::kStepKeys];
   unsigned char seen[C::kStages][C::kStepKeys];      // key_mask of a step's rows
   float m[kBlockWarps / kRowGroups][kRowGroups * 16], l[kBlockWarps / kRowGroups][kRowGroups * 16];
@@ -51,6 +51,9 @@ struct BlockShared {
 
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16u : 0u) : "memory");
+}
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 template <int kPending>
 __device__ __forceinline__ void cp_async_wait() {
@@ -114,15 +117,23 @@ struct Stager {
   __device__ void ask(int i, int j0) {
     const int row0 = threadIdx.x / C::kChunks, part = threadIdx.x % C::kChunks;
     if (inside) {
-      const bool whole_step = mask == nullptr && j0 + C::kStepKeys <= c.slots;
       const uint32_t to = kStorage == WM_BF16 ? ptx::smem_u32(sm.tile[i % C::kStages][0]) + piece_at<DP>(row0, part)  // passes are multiples of 8 rows
                                               : ptx::smem_u32(&sm.raw[0][kStorage == WM_BF16 ? 0 : threadIdx.x]);
       constexpr int kStep = kStorage == WM_BF16 ? C::kPassRows * C::kRowBytes : kBlockThreads * 16, kValues = kStorage == WM_BF16 ? C::kTileBytes : C::kPasses * kStep;
+      if (mask == nullptr && j0 + C::kStepKeys <= c.slots) {
 #pragma unroll
-      for (int p = 0; p < C::kPasses; ++p) {
-        const bool yes = whole_step || live(j0 + row0 + p * C::kPassRows);
-        cp_async_16(to + p * kStep, yes ? k + p * k_pass : static_cast<const char*>(a.k), yes);
-        cp_async_16(to + p * kStep + kValues, yes ? v + p * v_pass : static_cast<const char*>(a.k), yes);
+        for (int p = 0; p < C::kPasses; ++p) cp_async_16(to + p * kStep, k + p * k_pass);
+#pragma unroll
+        for (int p = 0; p < C::kPasses; ++p) cp_async_16(to + p * kStep + kValues, v + p * v_pass);
+      } else {
+        bool yes[C::kPasses];
+#pragma unroll
+        for (int p = 0; p < C::kPasses; ++p) yes[p] = live(j0 + row0 + p * C::kPassRows);
+#pragma unroll
+        for (int p = 0; p < C::kPasses; ++p) {
+          cp_async_16(to + p * kStep, yes[p] ? k + p * k_pass : static_cast<const char*>(a.k), yes[p]);
+          cp_async_16(to + p * kStep + kValues, yes[p] ? v + p * v_pass : static_cast<const char*>(a.k), yes[p]);
+        }
       }
     }
     if (kStorage != WM_BF16 && static_cast<int>(threadIdx.x) < 2 * C::kStepKeys) {
@@ -196,49 +207,57 @@ struct RowQueries {
   uint32_t shared;                                             // ldmatrix address: rows of a tile, pieces 0 .. 3
 };
 
+// Where a lane's ldmatrix rows lie in 16 keys: their piece 0 or 1 (`high` half of 16 elements), permuted by the row.  The pieces
+// of elements 16 s on are that address with s in bits 5 and up flipped, since a key's row is aligned to its own size.
 template <int DP>
-__device__ __forceinline__ void shared_scores(const RowQueries<DP>& q, uint32_t k_tile, float (&x)[1][2][4]) {
-  const int lane = threadIdx.x & 31;
-  // rows 0-7 and 8-15 of the keys, pieces 2s and 2s + 1
-  const int row = (lane & 7) + (lane & 8), half = lane >> 4;
-  const uint32_t base = k_tile + row * (DP * 2);
+__device__ __forceinline__ uint32_t lane_rows(int row, int high) {
+  return row * (DP * 2) + ((high ^ (row & 7)) << 4);
+}
+
+// U groups of 16 keys against the warp's 16 rows; `k` is the lane's address in the first of them.
+template <int DP, int U>
+__device__ __forceinline__ void shared_scores(const RowQueries<DP>& q, uint32_t k, float (&x)[U][2][4]) {
 #pragma unroll
   for (int s = 0; s < DP / 16; s += 2) {
-    uint32_t ka[2][4];
-    ldmatrix_x4(ka[0], base + (((2 * s + half) ^ (row & 7)) << 4));
-    ldmatrix_x4(ka[1], base + (((2 * s + 2 + half) ^ (row & 7)) << 4));
+    uint32_t b[2][4];
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
-      uint32_t b[4];
       if (RowQueries<DP>::kInRegisters) {
         const uint2 lo = q.reg[rt][RowQueries<DP>::kInRegisters ? s : 0], hi = q.reg[rt][RowQueries<DP>::kInRegisters ? s + 1 : 0];
-        b[0] = lo.x, b[1] = lo.y, b[2] = hi.x, b[3] = hi.y;
+        b[rt][0] = lo.x, b[rt][1] = lo.y, b[rt][2] = hi.x, b[rt][3] = hi.y;
       } else {
         // lanes 0-7, 8-15, 16-23, 24-31 name the rows of pieces 2s .. 2s + 3
-        ldmatrix_x4(b, q.shared + rt * 8 * (DP * 2) + (lane & 7) * (DP * 2) + (((2 * s + (lane >> 3)) ^ (lane & 7)) << 4));
+        ldmatrix_x4(b[rt], (q.shared + rt * 8 * (DP * 2)) ^ (s << 5));
       }
-      if (s == 0)
-        mma_16816_first(x[0][rt], ka[0][0], ka[0][1], ka[0][2], ka[0][3], b[0], b[1]);
-      else
-        mma_16816(x[0][rt], ka[0][0], ka[0][1], ka[0][2], ka[0][3], b[0], b[1]);
-      mma_16816(x[0][rt], ka[1][0], ka[1][1], ka[1][2], ka[1][3], b[2], b[3]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      uint32_t ka[4], kb[4];
+      ldmatrix_x4(ka, (k + u * 16 * (DP * 2)) ^ (s << 5));
+      ldmatrix_x4(kb, (k + u * 16 * (DP * 2)) ^ ((s + 1) << 5));
+#pragma unroll
+      for (int rt = 0; rt < 2; ++rt) {
+        if (s == 0)
+          mma_16816_first(x[u][rt], ka[0], ka[1], ka[2], ka[3], b[rt][0], b[rt][1]);
+        else
+          mma_16816(x[u][rt], ka[0], ka[1], ka[2], ka[3], b[rt][0], b[rt][1]);
+        mma_16816(x[u][rt], kb[0], kb[1], kb[2], kb[3], b[rt][2], b[rt][3]);
+      }
     }
   }
 }
 
-template <int DP>
-__device__ __forceinline__ void shared_values(State<DP, 2>& st, uint32_t v_tile, const uint32_t (&pb)[1][2][2]) {
-  const int lane = threadIdx.x & 31;
-  // matrices: keys 0-7 of pieces 2s and 2s + 1, then keys 8-15
-  const int row = (lane & 7) + ((lane & 16) >> 1), half = lane >> 3 & 1;
-  const uint32_t base = v_tile + row * (DP * 2);
+template <int DP, int U>
+__device__ __forceinline__ void shared_values(State<DP, 2>& st, uint32_t v, const uint32_t (&pb)[U][2][2]) {
 #pragma unroll
-  for (int s = 0; s < DP / 16; ++s) {
-    uint32_t va[4];
-    ldmatrix_x4_trans(va, base + (((2 * s + half) ^ (row & 7)) << 4));
+  for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt) mma_16816(st.o[s][rt], va[0], va[1], va[2], va[3], pb[0][rt][0], pb[0][rt][1]);
-  }
+    for (int s = 0; s < DP / 16; ++s) {
+      uint32_t va[4];
+      ldmatrix_x4_trans(va, (v + u * 16 * (DP * 2)) ^ (s << 5));
+#pragma unroll
+      for (int rt = 0; rt < 2; ++rt) mma_16816(st.o[s][rt], va[0], va[1], va[2], va[3], pb[u][rt][0], pb[u][rt][1]);
+    }
 }
 
 template <int kStorage, int DP, int kRowGroups, bool kTree>
@@ -246,17 +265,24 @@ __global__ void __launch_bounds__(kBlockThreads, 2) pool_attn_shared_kernel(cons
   using C = SharedCfg<kStorage, DP>;
   constexpr bool kScaled = kStorage != WM_BF16;
   constexpr int kRows = kRowGroups * 16, kSets = kBlockWarps / kRowGroups, kSetKeys = C::kStepKeys / kSets;
-  extern __shared__ __align__(128) unsigned char smem_raw[];
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
   BlockShared<kStorage, DP, kRowGroups>& sm = *reinterpret_cast<BlockShared<kStorage, DP, kRowGroups>*>(smem_raw);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining kernel may take its place: it waits for this one's end
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, row_group = warp % kRowGroups, set = warp / kRowGroups;
   const float factor = a.scale * kLog2e;
+  constexpr int U = DP == 64 ? 2 : 1;  // groups of 16 keys taken together: what the registers hold
+  constexpr uint32_t kFull = U == 2 ? 0xffffffffu : 0xffffu;
+  // ldmatrix of K: lanes 0-15 name the 16 keys' low halves of 16 elements, 16-31 the high ones; of V, transposed: lanes 0-7 and 8-15 keys
+  // 0-7 (low, high), 16-23 and 24-31 keys 8-15
+  const uint32_t k_lane = lane_rows<DP>(lane & 15, lane >> 4), v_lane = lane_rows<DP>((lane & 7) + ((lane & 16) >> 1), lane >> 3 & 1);
   if (tid == 0) {
     note_of(a, blockIdx.x)->last = -1;
     sm.poison[0] = sm.poison[1] = 0;
   }
   // columns behind head_dim are never written: zeros
-  for (int i = tid; i < static_cast<int>(sizeof(sm.tile) / 16); i += kBlockThreads) reinterpret_cast<uint4*>(sm.tile)[i] = make_uint4(0, 0, 0, 0);
+  if (a.head_dim < DP) {
+    for (int i = tid; i < static_cast<int>(sizeof(sm.tile) / 16); i += kBlockThreads) reinterpret_cast<uint4*>(sm.tile)[i] = make_uint4(0, 0, 0, 0);
+  }
   __syncthreads();
   Share share = find_share(a, plan, blockIdx.x, gridDim.x);
   int turn = 0;
@@ -314,7 +340,7 @@ __global__ void __launch_bounds__(kBlockThreads, 2) pool_attn_shared_kernel(cons
     }
     if (!RowQueries<DP>::kInRegisters) {
       constexpr int kPieces = DP / 8;
-      q.shared = ptx::smem_u32(sm.q) + row_group * 16 * C::kRowBytes;
+      q.shared = ptx::smem_u32(sm.q) + row_group * 16 * C::kRowBytes + lane_rows<DP>(lane & 7, lane >> 3);
       for (int i = tid; i < kRows * kPieces; i += kBlockThreads) {
         const int row = i / kPieces, part = i % kPieces;
         int token, head;
@@ -350,33 +376,40 @@ __global__ void __launch_bounds__(kBlockThreads, 2) pool_attn_shared_kernel(cons
       __syncthreads();  // step i is there for every warp, and step i - 1 has been read by every warp
       if (i + kAhead < past_steps) stager.ask(i + kAhead, j0 + kAhead * C::kStepKeys);
       ptx::cp_async_commit();
-      const uint32_t k_tile = ptx::smem_u32(sm.tile[i % C::kStages][0]), v_tile = k_tile + C::kTileBytes;
+      const int stage = i % C::kStages;
+      const uint32_t k_rows = ptx::smem_u32(sm.tile[stage][0]) + k_lane, v_rows = ptx::smem_u32(sm.tile[stage][1]) + v_lane;
+      const int there = min(kSetKeys, (draft ? a.q_len : c.slots) - j0 - set * kSetKeys);
+      if (!draft) {
 #pragma unroll 1
-      for (int key = set * kSetKeys; key < (set + 1) * kSetKeys; key += 16) {
-        const int left = (draft ? a.q_len : c.slots) - j0 - key;
-        if (left <= 0) break;
-        Keys keys[1] = {{{factor, factor}, {1.f, 1.f}, left >= 16 && !draft}};
-        uint32_t word = left >= 16 ? 0xffffu : (1u << left) - 1u;
-        if (!draft) {
-          if (a.key_mask != nullptr) {
-            word = __ballot_sync(0xffffffffu, lane < 16 && sm.seen[i % C::kStages][key + (lane & 15)] != 0);
-            keys[0].all = word == 0xffffu;
-          }
-          if (kScaled) {
+        for (int key = 0; key < there; key += 16 * U) {
+          const int first = set * kSetKeys + key, left = there - key;
+          uint32_t word = left >= 16 * U ? kFull : (1u << left) - 1u;
+          if (a.key_mask != nullptr) word = __ballot_sync(0xffffffffu, lane < 16 * U && sm.seen[stage][first + (lane & (16 * U - 1))] != 0);
+          Keys keys[U];
+          uint32_t seen[U][1][2];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            keys[u].all = word == kFull;
+            seen[u][0][0] = seen[u][0][1] = keys[u].all ? 3u : (word >> (16 * u + g) & 1u) | (word >> (16 * u + g + 8) & 1u) << 1;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const bool yes = word >> (g + 8 * h) & 1u;
-              keys[0].factor[h] = yes ? factor * sm.scale[i % C::kStages][0][key + g + 8 * h] : 0.f;
-              keys[0].scale[h] = yes ? sm.scale[i % C::kStages][1][key + g + 8 * h] : 0.f;
+              keys[u].factor[h] = kScaled ? factor * sm.scale[stage][0][first + 16 * u + g + 8 * h] : factor;
+              keys[u].scale[h] = kScaled ? sm.scale[stage][1][first + 16 * u + g + 8 * h] : 1.f;
+              if (kScaled && !keys[u].all && !(seen[u][0][0] >> h & 1u)) keys[u].scale[h] = 0.f;
             }
           }
+          float x[U][2][4];
+          uint32_t pb[U][2][2];
+          shared_scores<DP, U>(q, k_rows + first * C::kRowBytes, x);
+          weights<DP, 2, U, kScaled, false>(st, x, keys, seen, pb);
+          shared_values<DP, U>(st, v_rows + first * C::kRowBytes, pb);
         }
-        float x[1][2][4];
-        shared_scores<DP>(q, k_tile + key * C::kRowBytes, x);
-        uint32_t pb[1][2][2];
-        if (draft) {
-          const int words = (a.q_len + 31) / 32;
+      } else if (kTree) {
+#pragma unroll 1
+        for (int key = 0; key < there; key += 16) {
+          const int first = set * kSetKeys + key, words = (a.q_len + 31) / 32;
           const long long tree = a.shared_tree ? 0 : static_cast<long long>(c.b) * a.q_len;
+          const Keys keys[1] = {{{factor, factor}, {1.f, 1.f}, false}};
           uint32_t seen[1][2][2];
 #pragma unroll
           for (int rt = 0; rt < 2; ++rt)
@@ -384,16 +417,15 @@ __global__ void __launch_bounds__(kBlockThreads, 2) pool_attn_shared_kernel(cons
             for (int j = 0; j < 2; ++j) {
               int token, head;
               row_place(a, plan, c.kv_head, c.row_block, row_group * 16 + rt * 8 + 2 * t + j, token, head);
-              const uint32_t sees = token < a.q_len ? a.ancestors[(tree + token) * words + ((j0 + key) >> 5)] >> ((j0 + key) & 31) : 0u;
+              const uint32_t sees = token < a.q_len ? a.ancestors[(tree + token) * words + ((j0 + first) >> 5)] >> ((j0 + first) & 31) : 0u;
               seen[0][rt][j] = (sees >> g & 1u) | (sees >> (g + 8) & 1u) << 1;
             }
+          float x[1][2][4];
+          uint32_t pb[1][2][2];
+          shared_scores<DP, 1>(q, k_rows + first * C::kRowBytes, x);
           weights<DP, 2, 1, kScaled, true>(st, x, keys, seen, pb);
-        } else {
-          uint32_t seen[1][1][2];
-          seen[0][0][0] = seen[0][0][1] = (word >> g & 1u) | (word >> (g + 8) & 1u) << 1;
-          weights<DP, 2, 1, kScaled, false>(st, x, keys, seen, pb);
+          shared_values<DP, 1>(st, v_rows + first * C::kRowBytes, pb);
         }
-        shared_values<DP>(st, v_tile + key * C::kRowBytes, pb);
       }
     }
 

@@ -14,10 +14,6 @@ namespace wm {
 namespace pool {
 
 constexpr int kTileKeys = 128;
-#ifndef SEGCOST
-#define SEGCOST 2
-#endif
-constexpr int kSegmentCost = SEGCOST;
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 
@@ -28,6 +24,7 @@ struct Plan {
   int draft_tiles;
   int blocks;   // of the launch: shares, or blocks of all clusters
   int cluster;  // blocks per cluster, 0 where the launch works in shares
+  int segment_cost;  // what a segment costs beside its tiles (set-up, joining its warps), in tiles
 };
 
 // Slots that the queries of sequence b may see: the dummy and the committed tokens.
@@ -59,7 +56,7 @@ __device__ __forceinline__ Share find_share(const wm_pool_attn_args& a, const Pl
   const int lane = threadIdx.x & 31, per_tile = a.kv_heads * p.row_blocks;
   Share s;
   int sum = 0;
-  for (int b = lane; b < a.batch; b += 32) sum += kSegmentCost + sequence_tiles(a, p, b);
+  for (int b = lane; b < a.batch; b += 32) sum += p.segment_cost + sequence_tiles(a, p, b);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   s.total = sum * per_tile;
@@ -68,7 +65,7 @@ __device__ __forceinline__ Share find_share(const wm_pool_attn_args& a, const Pl
   s.b = s.b_begin = 0;
   if (s.begin >= s.end) return s;
   for (int base = 0, before = 0; base < a.batch; base += 32) {
-    int upto = base + lane < a.batch ? kSegmentCost + sequence_tiles(a, p, base + lane) : 0;
+    int upto = base + lane < a.batch ? p.segment_cost + sequence_tiles(a, p, base + lane) : 0;
     const int mine = upto;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -107,18 +104,18 @@ __device__ __forceinline__ Piece next_piece(const wm_pool_attn_args& a, const Pl
     c.slots = visible_slots(a, b);
     c.past_tiles = (c.slots + kTileKeys - 1) / kTileKeys;
     c.tiles = max(c.past_tiles + p.draft_tiles, 1);
-    const int b_end = b_begin + (c.tiles + kSegmentCost) * segments;
+    const int b_end = b_begin + (c.tiles + p.segment_cost) * segments;
     if (at < b_end) break;
     b_begin = b_end;
     ++b;
   }
-  const int units = c.tiles + kSegmentCost, in = at - b_begin, segment = in / units, first = in - segment * units;
+  const int units = c.tiles + p.segment_cost, in = at - b_begin, segment = in / units, first = in - segment * units;
   c.b = b;
   c.kv_head = segment / p.row_blocks;
   c.row_block = segment - c.kv_head * p.row_blocks;
   c.end = min(end, at + units - first);
-  c.tile = max(first - kSegmentCost, 0);
-  c.stop = max(first + c.end - at - kSegmentCost, 0);
+  c.tile = max(first - p.segment_cost, 0);
+  c.stop = max(first + c.end - at - p.segment_cost, 0);
   return c;
 }
 
