@@ -7,6 +7,7 @@ missing, every operator of the package raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -408,11 +409,11 @@ def load_library() -> ctypes.CDLL:
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.POINTER(AttnArgs)]
             fn.restype = ctypes.c_size_t
-        for name, struct in SERVING_ENTRY_POINTS:
+        for name, _ in SERVING_ENTRY_POINTS:
             fn = getattr(lib, name)
-            fn.argtypes = [ctypes.POINTER(struct), ctypes.c_void_p]
+            fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]  # a structure by reference, or its packed record
             fn.restype = ctypes.c_int
-        lib.wm_pool_attn_workspace_bytes.argtypes = [ctypes.POINTER(PoolAttnArgs)]
+        lib.wm_pool_attn_workspace_bytes.argtypes = [ctypes.c_void_p]
         lib.wm_pool_attn_workspace_bytes.restype = ctypes.c_size_t
         lib.wm_mix_workspace_bytes.argtypes = [ctypes.POINTER(MixArgs)]
         lib.wm_mix_workspace_bytes.restype = ctypes.c_size_t
@@ -444,13 +445,46 @@ def strides3(t: torch.Tensor) -> _Strides:
     return _Strides(t.stride(0), t.stride(1), t.stride(2))
 
 
+def _packer(layout):
+    """The record of a structure from all its members in order, arrays element by element, pointers as integers: one call
+    instead of an attribute per member (these operators are called once per layer and token: 0.1 us per member counts)."""
+    codes = {ctypes.c_void_p: "P", ctypes.c_size_t: "N", ctypes.c_int32: "i", ctypes.c_float: "f", _Strides: "3q"}
+    record = struct.Struct("@" + "".join(codes[kind] for _, kind in layout._fields_))
+    if -(-record.size // 8) * 8 != ctypes.sizeof(layout):  # (a structure's own tail padding)
+        raise AssertionError(layout.__name__)
+    tail = bytes(ctypes.sizeof(layout) - record.size)
+    pack = record.pack
+    return (lambda *members: pack(*members) + tail) if tail else pack
+
+
+pack_pool_commit = _packer(PoolCommitArgs)
+pack_pool_dequant = _packer(PoolDequantArgs)
+pack_draft_tree = _packer(DraftTreeArgs)
+pack_pool_attn = _packer(PoolAttnArgs)
+
+
+def call_record(name: str, record: bytes, index: int) -> None:
+    """``call`` for a packed record and the index of the tensors' device."""
+    lib = _library or load_library()
+    if index == torch.cuda.current_device():
+        status = getattr(lib, name)(record, current_stream_of(index))
+    else:
+        with torch.cuda.device(index):
+            status = getattr(lib, name)(record, current_stream_of(index))
+    if status != 0:
+        message = lib.wm_last_error().decode(errors="replace")
+        raise RuntimeError(f"{name} failed ({status}): {message}")
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the handle without a Stream object around it: 0.1 us, not 2
 
 
+def current_stream_of(index: int) -> int:
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 def current_stream(device: torch.device) -> int:
-    if _raw_stream is not None and device.index is not None:
-        return _raw_stream(device.index)
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch.cuda.current_stream(device).cuda_stream if device.index is None else current_stream_of(device.index)
 
 
 def call(name: str, args, device: torch.device) -> None:

@@ -54,13 +54,11 @@ def prepare_draft_tree(parents: torch.Tensor, *, include_self: bool = False) -> 
     if parents.dtype != torch.int32:  # numbers outside the tree stay outside it
         parents = parents.clamp(-2, MAX_NODES).to(torch.int32)
     parents = parents.contiguous()
-    ancestors = torch.empty((batch, tokens, -(-tokens // 32)), dtype=torch.int32, device=parents.device)
-    depths = torch.empty((batch, tokens), dtype=torch.int32, device=parents.device)
+    ancestors = parents.new_empty((batch, tokens, -(-tokens // 32)))
+    depths = torch.empty_like(parents)
     if batch and tokens:
-        a = _native.DraftTreeArgs()
-        a.parents, a.ancestors, a.depths = parents.data_ptr(), ancestors.data_ptr(), depths.data_ptr()
-        a.batch, a.tokens, a.include_self = batch, tokens, int(include_self)
-        _native.call("wm_draft_tree", a, parents.device)
+        record = _native.pack_draft_tree(parents.data_ptr(), ancestors.data_ptr(), depths.data_ptr(), batch, tokens, include_self)
+        _native.call_record("wm_draft_tree", record, parents.get_device())
     return DraftTree(ancestors, depths)
 
 

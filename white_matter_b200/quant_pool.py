@@ -16,6 +16,8 @@ bf16 (models/cache.py:43-60); these operators have no counterpart there.  All of
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _native
@@ -30,10 +32,10 @@ def _refuse_grad(what: str, *tensors: torch.Tensor) -> None:
         raise ValueError(f"{what} has no gradients: call it under torch.no_grad()")
 
 
-def _int_vector(name: str, t: torch.Tensor, batch: int, device: torch.device) -> torch.Tensor:
-    if t.shape != (batch,) or t.dtype not in (torch.int32, torch.int64):
+def _int_vector(name: str, t: torch.Tensor, batch: int, index: int) -> torch.Tensor:
+    if t.shape != (batch,) or (t.dtype != torch.int32 and t.dtype != torch.int64):
         raise ValueError(f"{name} must be integer (B,)")
-    if t.device != device:
+    if t.get_device() != index:
         raise ValueError(f"{name} must be on the pool's device")
     return t if t.is_contiguous() else t.contiguous()
 
@@ -47,21 +49,34 @@ def _aligned(t: torch.Tensor) -> tuple[torch.Tensor, int, tuple[int, int, int]]:
     return t, address, (batch, head, token)
 
 
-def _check_pool(keys: torch.Tensor, values: torch.Tensor, key_scales, value_scales) -> None:
-    if keys.ndim != 4 or keys.shape != values.shape:
+_NO_STRIDES = (0, 0, 0)
+
+
+def _check_pool(keys: torch.Tensor, values: torch.Tensor, key_scales, value_scales) -> tuple:
+    """Checks of a pool's tensors; returns (shape, device index, is held in 8 bits, code of the element type, strides of keys,
+    values and both scales, the scales' addresses)."""
+    shape, dtype = keys.shape, keys.dtype
+    if len(shape) != 4 or (values is not keys and values.shape != shape):
         raise ValueError("pool keys and values must be matching (B,HKV,N,D) tensors")
-    if keys.dtype != values.dtype or keys.device != values.device:
+    index = keys.get_device()
+    if values is not keys and (values.dtype != dtype or values.get_device() != index):
         raise ValueError("pool keys and values must share dtype and device")
-    if not keys.is_cuda:
+    if index < 0:
         raise ValueError("sm100 pool operators require CUDA tensors")
-    if keys.stride()[3] != 1 or values.stride()[3] != 1:
+    k0, k1, k2, k3 = keys.stride()
+    v0, v1, v2, v3 = values.stride()
+    if k3 != 1 or v3 != 1:
         raise ValueError("pool rows must have unit stride in head_dim")
-    if keys.dtype in _QUANTISED:
+    if dtype in _QUANTISED:
+        rows = shape[:3]
         for name, scales in (("key_scales", key_scales), ("value_scales", value_scales)):
-            if scales is None or scales.shape != keys.shape[:3] or scales.dtype != torch.float32 or scales.device != keys.device:
+            if scales is None or scales.shape != rows or scales.dtype != torch.float32 or scales.get_device() != index:
                 raise ValueError(f"{name} must be float32 (B,HKV,N) on the pool's device")
-    elif key_scales is not None or value_scales is not None:
+        storage = _native.WM_INT8 if dtype == torch.int8 else _native.WM_E4M3
+        return shape, index, True, storage, (k0, k1, k2), (v0, v1, v2), key_scales.stride(), value_scales.stride(), key_scales.data_ptr(), value_scales.data_ptr()
+    if key_scales is not None or value_scales is not None:
         raise ValueError("only pools in int8 or float8_e4m3fn have scales")
+    return shape, index, False, _native.dtype_code(dtype), (k0, k1, k2), (v0, v1, v2), _NO_STRIDES, _NO_STRIDES, 0, 0
 
 
 def pool_commit(
@@ -69,49 +84,44 @@ def pool_commit(
     new_values: torch.Tensor, lead: int, index: torch.Tensor | None, counts: torch.Tensor | None,
 ) -> int:
     """Checks and the launch behind every commit that quantises or picks rows; returns how many rows a sequence can get."""
-    _check_pool(keys, values, key_scales, value_scales)
-    batch, heads, slots, dim = keys.shape
-    if new_keys.ndim != 4 or new_keys.shape != new_values.shape or new_keys.shape[:2] != (batch, heads) or new_keys.shape[3] != dim:
+    (batch, heads, slots, dim), device, quantised, storage, k_strides, v_strides, ks_strides, vs_strides, ks, vs = _check_pool(
+        keys, values, key_scales, value_scales
+    )
+    shape, dtype = new_keys.shape, new_keys.dtype
+    if len(shape) != 4 or new_values.shape != shape or shape[0] != batch or shape[1] != heads or shape[3] != dim:
         raise ValueError("new rows must be (B, heads, n, D) for both K and V")
-    if new_keys.dtype not in _ROWS or new_values.dtype != new_keys.dtype:
+    if dtype not in _ROWS or new_values.dtype != dtype:
         raise ValueError("new rows must be bfloat16 or float32")
-    if keys.dtype not in _QUANTISED and keys.dtype != new_keys.dtype:
+    if not quantised and keys.dtype != dtype:
         raise ValueError("new rows must have the pool's dtype")
-    if any(t.device != keys.device for t in (new_keys, new_values)):
+    if new_keys.get_device() != device or new_values.get_device() != device:
         raise ValueError("new rows must be on the pool's device")
     _refuse_grad("a pool commit", new_keys, new_values)
-    lengths = _int_vector("lengths", lengths, batch, keys.device)
-    rows = new_keys.shape[2]
+    lengths = _int_vector("lengths", lengths, batch, device)
+    rows = source_rows = shape[2]
     if index is not None:
-        if index.ndim != 2 or index.shape[0] != batch or index.dtype not in (torch.int32, torch.int64) or index.device != keys.device:
+        if index.ndim != 2 or index.shape[0] != batch or index.dtype not in (torch.int32, torch.int64) or index.get_device() != device:
             raise ValueError("index must be integer (B, n) on the pool's device")
         rows = index.shape[1]
         if index.dtype != torch.int32:  # numbers beyond the source stay beyond it
-            index = index.clamp(-1, new_keys.shape[2]).to(torch.int32)
+            index = index.clamp(-1, source_rows).to(torch.int32)
         index = index.contiguous()
     if counts is not None:
-        counts = _int_vector("counts", counts, batch, keys.device)
+        counts = _int_vector("counts", counts, batch, device)
         if counts.dtype != torch.int32:
             counts = counts.clamp(0, rows).to(torch.int32)
-    if not batch or not heads or not slots or not dim or not rows or not new_keys.shape[2]:
+    if not (batch and heads and slots and dim and rows and source_rows):
         return rows
-    a = _native.PoolCommitArgs()
-    new_keys, a.new_keys, a.new_key_strides = _aligned(new_keys)
-    new_values, a.new_values, a.new_value_strides = _aligned(new_values)
-    a.keys, a.values = keys.data_ptr(), values.data_ptr()
-    a.key_strides, a.value_strides = keys.stride()[:3], values.stride()[:3]
-    if key_scales is not None:
-        a.key_scales, a.value_scales = key_scales.data_ptr(), value_scales.data_ptr()
-        a.key_scale_strides, a.value_scale_strides = key_scales.stride(), value_scales.stride()
-    a.lengths, a.lengths_is64 = lengths.data_ptr(), lengths.dtype == torch.int64
-    if index is not None:
-        a.index = index.data_ptr()
-    if counts is not None:
-        a.counts = counts.data_ptr()
-    a.storage, a.dtype = _native.storage_code(keys.dtype), _native.dtype_code(new_keys.dtype)
-    a.batch, a.heads, a.slots, a.head_dim = batch, heads, slots, dim
-    a.rows, a.source_rows, a.lead = rows, new_keys.shape[2], lead
-    _native.call("wm_pool_commit", a, keys.device)
+    new_keys, nk, nk_strides = _aligned(new_keys)
+    new_values, nv, nv_strides = _aligned(new_values)
+    record = _native.pack_pool_commit(
+        keys.data_ptr(), values.data_ptr(), ks, vs, nk, nv, lengths.data_ptr(), 0 if index is None else index.data_ptr(),
+        0 if counts is None else counts.data_ptr(),
+        *k_strides, *v_strides, *ks_strides, *vs_strides, *nk_strides, *nv_strides,
+        storage, _native.WM_F32 if dtype == torch.float32 else _native.WM_BF16, batch, heads, slots, rows, source_rows, dim, lead,
+        lengths.dtype == torch.int64,
+    )
+    _native.call_record("wm_pool_commit", record, device)
     return rows
 
 
@@ -163,22 +173,19 @@ def dequantize_kv_rows(
         raise ValueError("codes must be (B,H,N,D) in int8 or float8_e4m3fn")
     if dtype not in _ROWS:
         raise ValueError("rows are read back in bfloat16 or float32")
-    _check_pool(codes, codes, scales, scales)
-    batch, heads, slots, dim = codes.shape
+    (batch, heads, slots, dim), device, _, storage, strides, _, scale_strides, _, scale, _ = _check_pool(codes, codes, scales, scales)
     if lengths is not None:
-        lengths = _int_vector("lengths", lengths, batch, codes.device)
-    out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
-    if not out.numel():
+        lengths = _int_vector("lengths", lengths, batch, device)
+    out = torch.empty_like(codes, dtype=dtype, memory_format=torch.contiguous_format)
+    if not (batch and heads and slots and dim):
         return out
-    a = _native.PoolDequantArgs()
-    a.codes, a.scales, a.out = codes.data_ptr(), scales.data_ptr(), out.data_ptr()
-    a.code_strides, a.scale_strides, a.out_strides = codes.stride()[:3], scales.stride(), out.stride()[:3]
-    if lengths is not None:
-        a.lengths, a.lengths_is64 = lengths.data_ptr(), lengths.dtype == torch.int64
-    a.storage, a.dtype = _native.storage_code(codes.dtype), _native.dtype_code(dtype)
-    a.batch, a.heads, a.slots, a.head_dim = batch, heads, slots, dim
-    a.lead = int(use_dummy_token)
-    _native.call("wm_pool_dequant", a, codes.device)
+    record = _native.pack_pool_dequant(
+        codes.data_ptr(), scale, 0 if lengths is None else lengths.data_ptr(), out.data_ptr(),
+        *strides, *scale_strides, heads * slots * dim, slots * dim, dim,
+        storage, _native.WM_F32 if dtype == torch.float32 else _native.WM_BF16, batch, heads, slots, dim, int(use_dummy_token),
+        lengths is not None and lengths.dtype == torch.int64,
+    )
+    _native.call_record("wm_pool_dequant", record, device)
     return out
 
 
@@ -192,61 +199,73 @@ def pool_attention(
         raise ValueError("use_dummy_token must be boolean")
     if query.ndim != 4:
         raise ValueError("query must be (B,H,T,D)")
-    _check_pool(keys, values, key_scales, value_scales)
+    (pool_batch, kv_heads, slots, pool_dim), device, quantised, storage, k_strides, v_strides, ks_strides, vs_strides, ks, vs = _check_pool(
+        keys, values, key_scales, value_scales
+    )
     batch, heads, length, dim = query.shape
-    kv_heads, slots = keys.shape[1], keys.shape[2]
-    if keys.shape[0] != batch or keys.shape[3] != dim or not kv_heads or heads % kv_heads:
+    dtype = query.dtype
+    if pool_batch != batch or pool_dim != dim or not kv_heads or heads % kv_heads:
         raise ValueError("Q/K/V require matching batch/head_dim and divisible heads")
-    if query.device != keys.device:
+    if query.get_device() != device:
         raise ValueError("Q/K/V must share a device")
-    if query.dtype not in _ROWS:
+    if dtype not in _ROWS:
         raise ValueError("query must be bfloat16 or float32")
-    if keys.dtype not in _QUANTISED and keys.dtype != query.dtype:
+    if not quantised and keys.dtype != dtype:
         raise ValueError("the pool must be held in 8 bits or in the query's dtype")
-    if slots < int(use_dummy_token) or (not slots and draft is not None):
+    if slots < use_dummy_token or (not slots and draft is not None):
         raise ValueError("the pool must have a slot")
     if kv_lengths is not None:
-        kv_lengths = _int_vector("kv_lengths", kv_lengths, batch, query.device)
-    if key_mask is not None and (key_mask.shape != (batch, slots) or key_mask.dtype != torch.bool or key_mask.device != query.device):
-        raise ValueError("key_mask must be boolean (B,N) on the pool's device")
-    _refuse_grad("pool attention", query, *(draft[:2] if draft is not None else ()))
-    if dim > 128 or dim * query.element_size() % 16 or dim * keys.element_size() % 16:
+        kv_lengths = _int_vector("kv_lengths", kv_lengths, batch, device)
+    if key_mask is not None:
+        if key_mask.shape != (batch, slots) or key_mask.dtype != torch.bool or key_mask.get_device() != device:
+            raise ValueError("key_mask must be boolean (B,N) on the pool's device")
+        key_mask = key_mask.contiguous()
+    wide = 4 if dtype == torch.float32 else 2
+    if dim > 128 or dim * wide % 16 or (quantised and dim % 16):
         raise RuntimeError("sm100 pool attention needs rows of a multiple of 16 bytes and head_dim <= 128")
-    out = torch.empty((batch, length, heads, dim), dtype=query.dtype, device=query.device)
-    if not out.numel():
+    if draft is None:
+        _refuse_grad("pool attention", query)
+    else:
+        _refuse_grad("pool attention", query, draft[0], draft[1])
+    out = query.new_empty((batch, length, heads, dim))
+    if not (batch and length and heads and dim):
         return out
     if not slots:
         return out.zero_()
-    a = _native.PoolAttnArgs()
-    query, a.q, a.q_strides = _aligned(query)
-    a.k, a.v, a.out = keys.data_ptr(), values.data_ptr(), out.data_ptr()
-    a.k_strides, a.v_strides = keys.stride()[:3], values.stride()[:3]
-    a.out_strides = length * heads * dim, dim, heads * dim
-    if key_scales is not None:
-        a.k_scales, a.v_scales = key_scales.data_ptr(), value_scales.data_ptr()
-        a.k_scale_strides, a.v_scale_strides = key_scales.stride(), value_scales.stride()
-    if kv_lengths is not None:
-        a.lengths, a.lengths_is64 = kv_lengths.data_ptr(), kv_lengths.dtype == torch.int64
-    if key_mask is not None:
-        key_mask = key_mask.contiguous()
-        a.key_mask = key_mask.data_ptr()
+    query, q, q_strides = _aligned(query)
+    dk = dv = ancestors = depths = shared = 0
+    dk_strides = dv_strides = _NO_STRIDES
     if draft is not None:
-        draft_keys, draft_values, ancestors, depths = draft
-        draft_keys, a.draft_k, a.draft_k_strides = _aligned(draft_keys)
-        draft_values, a.draft_v, a.draft_v_strides = _aligned(draft_values)
-        ancestors, depths = ancestors.contiguous(), depths.contiguous()
-        a.ancestors, a.depths = ancestors.data_ptr(), depths.data_ptr()
-        a.shared_tree = depths.shape[0] == 1
-    a.dtype, a.storage = _native.dtype_code(query.dtype), _native.storage_code(keys.dtype)
-    a.batch, a.q_heads, a.q_len, a.head_dim = batch, heads, length, dim
-    a.kv_heads, a.k_len, a.lead = kv_heads, slots, int(use_dummy_token)
-    a.scale = dim**-0.5 if softmax_scale is None else float(softmax_scale)
-    nbytes = _native.load_library().wm_pool_attn_workspace_bytes(_native.ctypes.byref(a))
+        draft_keys, draft_values, ancestor_bits, depth_rows = draft
+        draft_keys, dk, dk_strides = _aligned(draft_keys)
+        draft_values, dv, dv_strides = _aligned(draft_values)
+        ancestor_bits, depth_rows = ancestor_bits.contiguous(), depth_rows.contiguous()
+        ancestors, depths, shared = ancestor_bits.data_ptr(), depth_rows.data_ptr(), depth_rows.shape[0] == 1
+    lengths, lengths64 = (0, 0) if kv_lengths is None else (kv_lengths.data_ptr(), kv_lengths.dtype == torch.int64)
+    mask = 0 if key_mask is None else key_mask.data_ptr()
+    code, lead = _native.WM_F32 if wide == 4 else _native.WM_BF16, int(use_dummy_token)
+    nbytes = _workspace_bytes(code, storage, batch, heads, kv_heads, length, slots, dim, draft is not None)
+    workspace = 0
     if nbytes:
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), nbytes
-    _native.call("wm_pool_attn", a, query.device)
+        held = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
+        workspace = held.data_ptr()
+    record = _native.pack_pool_attn(
+        q, keys.data_ptr(), values.data_ptr(), ks, vs, dk, dv, ancestors, depths, lengths, mask, out.data_ptr(), workspace, nbytes,
+        *q_strides, *k_strides, *v_strides, *ks_strides, *vs_strides, *dk_strides, *dv_strides, length * heads * dim, dim, heads * dim,
+        code, storage, batch, heads, kv_heads, length, slots, dim, lead, lengths64, shared,
+        dim**-0.5 if softmax_scale is None else float(softmax_scale),
+    )
+    _native.call_record("wm_pool_attn", record, device)
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(dtype: int, storage: int, batch: int, heads: int, kv_heads: int, length: int, slots: int, dim: int, tree: bool) -> int:
+    """What the library asks for by the sizes of a call."""
+    a = _native.PoolAttnArgs()
+    a.dtype, a.storage, a.batch, a.q_heads, a.kv_heads, a.q_len, a.k_len, a.head_dim = dtype, storage, batch, heads, kv_heads, length, slots, dim
+    a.ancestors = 1 if tree else None  # only whether there is a tree matters
+    return _native.load_library().wm_pool_attn_workspace_bytes(_native.ctypes.byref(a))
 
 
 def quantized_pool_attention(
