@@ -97,6 +97,8 @@ SHAPES = [  # batch, heads, kv_heads, tokens, slots, dim, lead, masked, lengths
     (2, 4, 2, 6, 4300, 64, 1, True, [4300, 40]),
     (2, 4, 1, 12, 4300, 128, 0, False, [4300, 130]),
     (30, 2, 1, 20, 140, 64, 1, False, [5 * i for i in range(30)]),
+    (2, 16, 2, 20, 300, 64, 0, True, [300, 150]),  # 160 rows per KV head: two blocks of 128
+    (1, 12, 1, 10, 260, 128, 1, False, [200]),
 ]
 
 
@@ -131,10 +133,45 @@ def test_attention_matches_the_oracle(shape, storage, dtype, include_self):
 
 @pytest.mark.gpu
 @on_gpu
+@pytest.mark.parametrize("tokens", [3, 30])
+@pytest.mark.parametrize("dim, dtype", [(8, torch.bfloat16), (24, torch.bfloat16), (40, torch.bfloat16), (72, torch.bfloat16), (120, torch.bfloat16), (4, torch.float32), (20, torch.float32), (100, torch.float32)])
+def test_head_sizes_that_fill_no_tile(dim, dtype, tokens):
+    query, pools, rows, mask, parents, draft = problem(5, "plain", dtype, 2, 4, 2, tokens, 150, dim, 1, True, [149, 40])
+    visible, depths = oracle.tree_tables(parents, True)
+    got = draft_tree_attention(
+        query.cuda(), pools[0][0].cuda(), pools[1][0].cuda(), *(d.cuda() for d in draft), prepare_draft_tree(parents.cuda(), include_self=True),
+        kv_lengths=torch.tensor([149, 40]).cuda(), use_dummy_token=True, key_mask=mask.cuda(),
+    )
+    check_attention(got, query, rows, [149, 40], 1, mask, (*draft, visible, depths))
+
+
+@pytest.mark.gpu
+@on_gpu
+@pytest.mark.parametrize("tokens", [2, 24])
+def test_layouts_other_than_contiguous(tokens):
+    """Pools as (B,N,HKV,D) views with gaps between the rows, queries and drafts off their 16 bytes or with strided elements, a mask
+    out of a wider one: the same result as from contiguous copies."""
+    torch.manual_seed(6)
+    wide = torch.randn(2, 90, 3, 96, device="cuda").bfloat16()
+    key, value = wide[:, :, :2, :64].transpose(1, 2), wide[:, :, 1:, 16:80].transpose(1, 2)
+    query = torch.randn(2, 4, tokens, 130, device="cuda").bfloat16()[..., 1:129:2]
+    draft = [torch.randn(2 * 2 * tokens * 64 + 3, device="cuda").bfloat16()[3:].view(2, 2, tokens, 64) for _ in "kv"]
+    mask = (torch.rand(2, 180, device="cuda") < 0.8)[:, ::2]
+    tree = prepare_draft_tree(torch.arange(-1, tokens - 1, device="cuda"))
+    lengths = torch.tensor([[70, 0], [90, 0]], device="cuda")[:, 0]
+    common = dict(kv_lengths=lengths, key_mask=mask)
+    got = draft_tree_attention(query, key, value, *draft, tree, **common)
+    plain = [t.clone(memory_format=torch.contiguous_format) for t in (query, key, value, *draft)]
+    assert torch.equal(got, draft_tree_attention(*plain, tree, kv_lengths=lengths.clone(), key_mask=mask.clone(memory_format=torch.contiguous_format)))
+    check_attention(got, plain[0].cpu(), [plain[1].cpu(), plain[2].cpu()], lengths.cpu(), 0, mask.cpu(), (plain[3].cpu(), plain[4].cpu(), *oracle.tree_tables(torch.arange(-1, tokens - 1)[None], False)))
+
+
+@pytest.mark.gpu
+@on_gpu
+@pytest.mark.parametrize("tokens", [4, 20])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_a_poisoned_drafted_token_reaches_its_descendants_alone(dtype):
+def test_a_poisoned_drafted_token_reaches_its_descendants_alone(dtype, tokens):
     gen = torch.Generator().manual_seed(2)
-    tokens = 40
     parents = random_parents(gen, 2, tokens)
     visible, _ = oracle.tree_tables(parents, False)
     victim = int(visible[0].sum(0).argmax())  # the node most others descend from

@@ -303,6 +303,7 @@ SHAPES = [  # batch, heads, kv_heads, tokens, slots, dim, lead, masked, lengths
     (2, 4, 1, 16, 4300, 64, 1, False, [4300, 200]),
     (1, 3, 1, 40, 1000, 112, 0, True, [990]),
     (40, 4, 2, 9, 150, 64, 0, False, [3 * i for i in range(40)]),
+    (2, 16, 1, 8, 700, 64, 0, True, [700, 300]),
 ]
 
 
@@ -337,6 +338,38 @@ def test_scores_far_from_zero_and_far_apart(storage):
         (k, ks), (v, vs) = oracle.quantise_rows(x, storage), oracle.quantise_rows(torch.randn(2, 2, 400, 64, generator=gen), storage)
         got = quantized_pool_attention(query.cuda(), k.to(STORAGE[storage]).cuda(), v.to(STORAGE[storage]).cuda(), ks.cuda(), vs.cuda(), softmax_scale=1.0)
         check_attention(got, query, [k * ks[..., None].double(), v * vs[..., None].double()], None, 0, None, None, 1.0)
+
+
+@pytest.mark.gpu
+@on_gpu
+@pytest.mark.parametrize("tokens", [1, 3, 9])
+@pytest.mark.parametrize("storage", sorted(STORAGE))
+def test_codes_over_the_whole_range_of_their_type(storage, tokens):
+    """Elements spread over many powers of two inside a row: subnormal codes, zeros and full ones side by side."""
+    gen = torch.Generator().manual_seed(13)
+    x = [torch.randn(2, 2, 150, 64, generator=gen) * torch.exp2(-12 * torch.rand(2, 2, 150, 64, generator=gen)) for _ in "kv"]
+    (k, ks), (v, vs) = (oracle.quantise_rows(t, storage) for t in x)
+    query = torch.randn(2, 4, tokens, 64, generator=gen).bfloat16()
+    got = quantized_pool_attention(query.cuda(), k.to(STORAGE[storage]).cuda(), v.to(STORAGE[storage]).cuda(), ks.cuda(), vs.cuda(), softmax_scale=1.0)
+    check_attention(got, query, [k * ks[..., None].double(), v * vs[..., None].double()], None, 0, None, None, 1.0)
+
+
+@pytest.mark.gpu
+@on_gpu
+@pytest.mark.parametrize("tokens", [1, 9])
+def test_value_scales_far_apart(tokens):
+    """A row that attends to a token whose value is a millionth of the others' still gets it exactly enough."""
+    gen = torch.Generator().manual_seed(14)
+    k = torch.zeros(1, 1, 200, 64)
+    k[0, 0, :, 0] = -40.0
+    k[0, 0, 77, 0] = 40.0
+    v = torch.randn(1, 1, 200, 64, generator=gen)
+    v[0, 0, 77] *= 1e-6
+    (kc, ks), (vc, vs) = (oracle.quantise_rows(t, "int8") for t in (k, v))
+    query = torch.zeros(1, 2, tokens, 64).bfloat16()
+    query[..., 0] = 8.0
+    got = quantized_pool_attention(query.cuda(), kc.to(torch.int8).cuda(), vc.to(torch.int8).cuda(), ks.cuda(), vs.cuda())
+    check_attention(got, query, [kc * ks[..., None].double(), vc * vs[..., None].double()], None, 0, None)
 
 
 @pytest.mark.gpu

@@ -44,7 +44,7 @@ def _aligned(t: torch.Tensor) -> tuple[torch.Tensor, int, tuple[int, int, int]]:
     """(tensor, address, strides) of the tensor itself where its rows have unit stride and start on 16 bytes, else of a copy."""
     address, (batch, head, token, inner) = t.data_ptr(), t.stride()
     if inner != 1 or (address | (batch | head | token) * t.element_size()) & 15:
-        t = t.contiguous()
+        t = t.clone(memory_format=torch.contiguous_format)  # (a contiguous tensor may start off 16 bytes)
         address, (batch, head, token, inner) = t.data_ptr(), t.stride()
     return t, address, (batch, head, token)
 
