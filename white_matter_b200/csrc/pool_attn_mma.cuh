@@ -209,6 +209,9 @@ struct Keys {
   bool all;
 };
 
+// The value scale of a key.  A row of zeros has scale 0, a row that is not seen may have any: 1 does as well, and has an inverse.
+__device__ __forceinline__ float usable_scale(float scale, bool seen) { return seen && scale != 0.f ? scale : 1.f; }
+
 // Weights of U x 16 keys for every tile, as B operands of O^T += V^T P^T.  x holds the keys' products with the queries (keys
 // g: x[.][.][0], [1]; g + 8: [2], [3]; rows 2t, 2t + 1).
 template <int DP, int RT, int U, bool kScaled, bool kPerRow>
@@ -262,26 +265,33 @@ __device__ __forceinline__ void weights(State<DP, RT>& st, float (&x)[U][RT][4],
       }
   }
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt)
+  for (int u = 0; u < U; ++u) {
+    const float inverse[2] = {kScaled ? 1.f / keys[u].scale[0] : 1.f, kScaled ? 1.f / keys[u].scale[1] : 1.f};
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int rt = 0; rt < RT; ++rt) {
       float(&y)[4] = x[u][rt];
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = exp2_approx(y[e]);
       if (kScaled) {
-        st.l[rt][0] += y[0] + y[2];
-        st.l[rt][1] += y[1] + y[3];
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] *= keys[u].scale[e >> 1];
       }
       const uint32_t b0 = pack_bf16(y[0], y[1]), b1 = pack_bf16(y[2], y[3]);
-      if (!kScaled) {  // the sum takes the weights as they are rounded, so that the result is an exact mean of value rows
+      // the sum takes the weights as they are rounded, so that the result is an exact mean of value rows (with the sum of the
+      // unrounded ones a read of 8-bit rows was 1.45 times as far from the exact result as its own rounding to bf16)
+      if (kScaled) {
+        st.l[rt][0] = fmaf(__uint_as_float(b0 << 16), inverse[0], st.l[rt][0]);
+        st.l[rt][1] = fmaf(__uint_as_float(b0 & 0xffff0000u), inverse[0], st.l[rt][1]);
+        st.l[rt][0] = fmaf(__uint_as_float(b1 << 16), inverse[1], st.l[rt][0]);
+        st.l[rt][1] = fmaf(__uint_as_float(b1 & 0xffff0000u), inverse[1], st.l[rt][1]);
+      } else {
         ptx::add_bf16_halves(b0, st.l[rt][0], st.l[rt][1]);
         ptx::add_bf16_halves(b1, st.l[rt][0], st.l[rt][1]);
       }
       pb[u][rt][0] = transpose_8x8(b0);
       pb[u][rt][1] = transpose_8x8(b1);
     }
+  }
 }
 
 // ---------------------------------------------------------------- committed slots
@@ -384,8 +394,7 @@ __device__ __forceinline__ void past_keys(const wm_pool_attn_args& a, const Piec
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         keys[u].factor[h] = kScaled ? factor * kscale[u][h] : factor;
-        keys[u].scale[h] = kScaled ? vscale[u][h] : 1.f;
-        if (kScaled && !keys[u].all && !(seen[u][0][0] >> h & 1u)) keys[u].scale[h] = 0.f;
+        keys[u].scale[h] = kScaled ? usable_scale(vscale[u][h], keys[u].all || (seen[u][0][0] >> h & 1u)) : 1.f;
       }
     }
     float x[U][RT][4];

@@ -394,8 +394,7 @@ __global__ void __launch_bounds__(kBlockThreads, 2) pool_attn_shared_kernel(cons
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               keys[u].factor[h] = kScaled ? factor * sm.scale[stage][0][first + 16 * u + g + 8 * h] : factor;
-              keys[u].scale[h] = kScaled ? sm.scale[stage][1][first + 16 * u + g + 8 * h] : 1.f;
-              if (kScaled && !keys[u].all && !(seen[u][0][0] >> h & 1u)) keys[u].scale[h] = 0.f;
+              keys[u].scale[h] = kScaled ? usable_scale(sm.scale[stage][1][first + 16 * u + g + 8 * h], keys[u].all || (seen[u][0][0] >> h & 1u)) : 1.f;
             }
           }
           float x[U][2][4];
