@@ -374,6 +374,21 @@ def test_value_scales_far_apart(tokens):
 
 @pytest.mark.gpu
 @on_gpu
+@pytest.mark.parametrize("tokens", [1, 3, 9, 40])
+@pytest.mark.parametrize("storage", sorted(STORAGE))
+def test_value_scales_of_zero_and_next_to_it(storage, tokens):
+    """An element stands for code * scale whatever the code is: nothing where the scale is zero or subnormal."""
+    gen = torch.Generator().manual_seed(15)
+    k, v = torch.randn(2, 1, 2, 150, 64, generator=gen).unbind(0)
+    (kc, ks), (vc, vs) = (oracle.quantise_rows(t, storage) for t in (k, v))
+    vs[0, 0, ::3], vs[0, 1, 1::3] = 0.0, 2.0**-130
+    query = torch.randn(1, 2, tokens, 64, generator=gen).bfloat16()
+    got = quantized_pool_attention(query.cuda(), kc.to(STORAGE[storage]).cuda(), vc.to(STORAGE[storage]).cuda(), ks.cuda(), vs.cuda())
+    check_attention(got, query, [kc * ks[..., None].double(), vc * vs[..., None].double()], None, 0, None)
+
+
+@pytest.mark.gpu
+@on_gpu
 def test_a_poisoned_row_shows_in_the_queries_that_see_it():
     pool = QuantKVPoolCache(2, 1, 2, 40, 64)
     x = torch.randn(2, 2, 20, 64).bfloat16()

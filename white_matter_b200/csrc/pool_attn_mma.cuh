@@ -52,6 +52,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// within 2^-23 of the quotient: a weight is read back from its 8 bits with it
+__device__ __forceinline__ float reciprocal_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t y;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
@@ -209,8 +215,9 @@ struct Keys {
   bool all;
 };
 
-// The value scale of a key.  A row of zeros has scale 0, a row that is not seen may have any: 1 does as well, and has an inverse.
-__device__ __forceinline__ float usable_scale(float scale, bool seen) { return seen && scale != 0.f ? scale : 1.f; }
+// The value scale of a key, as a number that has an inverse: a row of zeros has scale 0, which becomes 2^-110 (a commit writes no
+// other scale below 2^-108), a row that is not seen may have any, which becomes 1.
+__device__ __forceinline__ float usable_scale(float scale, bool seen) { return !seen ? 1.f : fabsf(scale) < 0x1p-110f ? 0x1p-110f : scale; }
 
 // Weights of U x 16 keys for every tile, as B operands of O^T += V^T P^T.  x holds the keys' products with the queries (keys
 // g: x[.][.][0], [1]; g + 8: [2], [3]; rows 2t, 2t + 1).
@@ -266,7 +273,7 @@ __device__ __forceinline__ void weights(State<DP, RT>& st, float (&x)[U][RT][4],
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const float inverse[2] = {kScaled ? 1.f / keys[u].scale[0] : 1.f, kScaled ? 1.f / keys[u].scale[1] : 1.f};
+    const float inverse[2] = {kScaled ? reciprocal_approx(keys[u].scale[0]) : 1.f, kScaled ? reciprocal_approx(keys[u].scale[1]) : 1.f};
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float(&y)[4] = x[u][rt];

@@ -5,10 +5,9 @@
 // A block of eight warps holds 16 rows per warp: kRowGroups warps side by side cover the rows, 8 / kRowGroups such sets share
 // the keys of a step.  16 rows keep a warp's accumulators small, so two blocks fit an SM; the registers of one warp for 32
 // rows (its rows' accumulators beside the pool rows in flight) left 12 warps per SM, which hid too little latency
-// (IPC 1.35 on 64 sequences with 32 drafted tokens, 250 us; this kernel: XXX us).
+// (IPC 1.35 on 64 sequences with 32 drafted tokens, 250 us; this kernel: 198 us, 5 490 GB/s).
 //
-// A step is 128 keys (heads of up to 64) or 64 keys, as bf16 rows of DP elements whose 16-byte pieces are permuted by the row
-// (piece ^ row % 8), which keeps ldmatrix free of bank conflicts.  bf16 rows arrive by asynchronous copies, two steps ahead; 8-bit
+// A step is 128 keys (heads of up to 64) or 64 keys, as bf16 rows of DP elements.  bf16 rows arrive by asynchronous copies, two steps ahead; 8-bit
 // rows by the same copies, one step ahead, into a corner of the thread that turns their codes into bf16.  Rows that are not visible are
 // stored as zeros.
 #pragma once
@@ -20,12 +19,25 @@ namespace pool {
 
 constexpr int kBlockWarps = 8, kBlockThreads = kBlockWarps * 32;
 
+// Rows in shared memory, so that the eight rows of a matrix keep off each other's banks: wide ones 16 bytes apart, narrow ones
+// without a gap, their 16-byte pieces permuted by the row (piece ^ row % 8).  A gap costs no instruction where the permutation
+// costs one per matrix (8 sequences with 41 drafted tokens, 4 heads of 128 per KV head, int8: 106 us against 110 us); a gap in rows of
+// 64 cost more than it gave (64 sequences with 32 drafted tokens, bf16: some 5 % slower).
+template <int DP>
+struct RowLayout {
+  static constexpr bool kPermuted = DP == 64;
+  static constexpr int kPitch = DP * 2 + (kPermuted ? 0 : 16);
+  __device__ static uint32_t piece(int row, int piece) { return row * kPitch + ((kPermuted ? piece ^ (row & 7) : piece) << 4); }
+  // the piece 2 s behind the one that `at` names, which is piece 0 or 1 of a row in a buffer aligned to its rows
+  __device__ static uint32_t behind(uint32_t at, int s) { return kPermuted ? at ^ (s << 5) : at + (s << 5); }
+};
+
 template <int kStorage, int DP>
 struct SharedCfg {
   static constexpr int kBytes = kStorage == WM_BF16 ? 2 : 1;
   static constexpr int kStepKeys = DP == 64 ? 128 : 64;
   static constexpr int kStages = kStorage == WM_BF16 && DP == 64 ? 3 : 2;
-  static constexpr int kRowBytes = DP * 2;
+  static constexpr int kRowBytes = RowLayout<DP>::kPitch;
   static constexpr int kTileBytes = kStepKeys * kRowBytes;
   static constexpr int kChunks = DP * kBytes / 16;                               // 16-byte pieces of a pool row
   static constexpr int kPasses = kStepKeys * kChunks / kBlockThreads;            // pieces of K (or V) per thread and step
@@ -36,14 +48,14 @@ template <int kStorage, int DP, int kRowGroups>
 struct BlockShared {
   using C = SharedCfg<kStorage, DP>;
   static constexpr int kSide = kBlockWarps / kRowGroups > 2 ? 2 : kBlockWarps / kRowGroups;
-  static constexpr int kPitch = kStorage != WM_BF16 && DP == 128 ? DP : DP + 4;  // the padding keeps rows off each other's banks where it fits
+  static constexpr int kPitch = DP + 4;
   union {
     unsigned char tile[C::kStages][2][C::kTileBytes];    // K, V of a step
     float acc[kSide][kRowGroups * 16][kPitch];           // at the end of a piece: sums of two sets of warps
   };
   uint4 raw[kStorage == WM_BF16 ? 1 : 2 * C::kPasses][kStorage == WM_BF16 ? 1 : kBlockThreads];  // a step's codes, a corner per thread
-  alignas(256) unsigned char q[DP > 64 ? kRowGroups * 16 * C::kRowBytes : 16];
-  float scale[C::kStages][2][C::kStepKeys];
+  unsigned char q[DP > 64 ? kRowGroups * 16 * C::kRowBytes : 16];
+  float scale[kStorage == WM_BF16 ? 1 : C::kStages][2][C::kStepKeys];
   unsigned char seen[C::kStages][C::kStepKeys];      // key_mask of a step's rows
   float m[kBlockWarps / kRowGroups][kRowGroups * 16], l[kBlockWarps / kRowGroups][kRowGroups * 16];
   int poison[2];  // the drafted values of this piece, and of the next, hold an infinity or NaN
@@ -82,10 +94,6 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t x, bool& special) {
   if ((x & 0x7f800000u) == 0x7f800000u) x &= 0x0000ffffu, special = true;
   return x;
 }
-template <int DP>
-__device__ __forceinline__ uint32_t piece_at(int row, int piece) {
-  return row * (DP * 2) + ((piece ^ (row & 7)) << 4);
-}
 
 // ---------------------------------------------------------------- pool rows to shared memory
 template <int kStorage, int DP, int kRowGroups>
@@ -117,7 +125,7 @@ struct Stager {
   __device__ void ask(int i, int j0) {
     const int row0 = threadIdx.x / C::kChunks, part = threadIdx.x % C::kChunks;
     if (inside) {
-      const uint32_t to = kStorage == WM_BF16 ? ptx::smem_u32(sm.tile[i % C::kStages][0]) + piece_at<DP>(row0, part)  // passes are multiples of 8 rows
+      const uint32_t to = kStorage == WM_BF16 ? ptx::smem_u32(sm.tile[i % C::kStages][0]) + RowLayout<DP>::piece(row0, part)
                                               : ptx::smem_u32(&sm.raw[0][kStorage == WM_BF16 ? 0 : threadIdx.x]);
       constexpr int kStep = kStorage == WM_BF16 ? C::kPassRows * C::kRowBytes : kBlockThreads * 16, kValues = kStorage == WM_BF16 ? C::kTileBytes : C::kPasses * kStep;
       if (mask == nullptr && j0 + C::kStepKeys <= c.slots) {
@@ -155,7 +163,7 @@ struct Stager {
     if (!inside) return;
     const int row0 = threadIdx.x / C::kChunks, part = threadIdx.x % C::kChunks;
     const uint32_t to = ptx::smem_u32(sm.tile[i % C::kStages][0]);
-    const uint32_t first = to + piece_at<DP>(row0, 2 * part), second = to + piece_at<DP>(row0, 2 * part + 1);
+    const uint32_t first = to + RowLayout<DP>::piece(row0, 2 * part), second = to + RowLayout<DP>::piece(row0, 2 * part + 1);
 #pragma unroll
     for (int n = 0; n < 2 * C::kPasses; ++n) {
       const uint4 x = sm.raw[kStorage == WM_BF16 ? 0 : n][kStorage == WM_BF16 ? 0 : threadIdx.x];
@@ -192,7 +200,7 @@ struct Stager {
         uint4 y = x[n];
         if (value) y = make_uint4(finite_halves(y.x, special), finite_halves(y.y, special), finite_halves(y.z, special), finite_halves(y.w, special));
         if (kStorage != WM_BF16) y = permuted(y);
-        st_shared_16(ptx::smem_u32(sm.tile[i % C::kStages][0]) + value * C::kTileBytes + piece_at<DP>(row, part), y);
+        st_shared_16(ptx::smem_u32(sm.tile[i % C::kStages][0]) + value * C::kTileBytes + RowLayout<DP>::piece(row, part), y);
       }
     }
     if (special) sm.poison[turn] = 1;
@@ -207,16 +215,10 @@ struct RowQueries {
   uint32_t shared;                                             // ldmatrix address: rows of a tile, pieces 0 .. 3
 };
 
-// Where a lane's ldmatrix rows lie in 16 keys: their piece 0 or 1 (`high` half of 16 elements), permuted by the row.  The pieces
-// of elements 16 s on are that address with s in bits 5 and up flipped, since a key's row is aligned to its own size.
-template <int DP>
-__device__ __forceinline__ uint32_t lane_rows(int row, int high) {
-  return row * (DP * 2) + ((high ^ (row & 7)) << 4);
-}
-
 // U groups of 16 keys against the warp's 16 rows; `k` is the lane's address in the first of them.
 template <int DP, int U>
 __device__ __forceinline__ void shared_scores(const RowQueries<DP>& q, uint32_t k, float (&x)[U][2][4]) {
+  constexpr int kPitch = RowLayout<DP>::kPitch;
 #pragma unroll
   for (int s = 0; s < DP / 16; s += 2) {
     uint32_t b[2][4];
@@ -227,14 +229,14 @@ __device__ __forceinline__ void shared_scores(const RowQueries<DP>& q, uint32_t 
         b[rt][0] = lo.x, b[rt][1] = lo.y, b[rt][2] = hi.x, b[rt][3] = hi.y;
       } else {
         // lanes 0-7, 8-15, 16-23, 24-31 name the rows of pieces 2s .. 2s + 3
-        ldmatrix_x4(b[rt], (q.shared + rt * 8 * (DP * 2)) ^ (s << 5));
+        ldmatrix_x4(b[rt], RowLayout<DP>::behind(q.shared + rt * 8 * kPitch, s));
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       uint32_t ka[4], kb[4];
-      ldmatrix_x4(ka, (k + u * 16 * (DP * 2)) ^ (s << 5));
-      ldmatrix_x4(kb, (k + u * 16 * (DP * 2)) ^ ((s + 1) << 5));
+      ldmatrix_x4(ka, RowLayout<DP>::behind(k + u * 16 * kPitch, s));
+      ldmatrix_x4(kb, RowLayout<DP>::behind(k + u * 16 * kPitch, s + 1));
 #pragma unroll
       for (int rt = 0; rt < 2; ++rt) {
         if (s == 0)
@@ -249,12 +251,13 @@ __device__ __forceinline__ void shared_scores(const RowQueries<DP>& q, uint32_t 
 
 template <int DP, int U>
 __device__ __forceinline__ void shared_values(State<DP, 2>& st, uint32_t v, const uint32_t (&pb)[U][2][2]) {
+  constexpr int kPitch = RowLayout<DP>::kPitch;
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
       uint32_t va[4];
-      ldmatrix_x4_trans(va, (v + u * 16 * (DP * 2)) ^ (s << 5));
+      ldmatrix_x4_trans(va, RowLayout<DP>::behind(v + u * 16 * kPitch, s));
 #pragma unroll
       for (int rt = 0; rt < 2; ++rt) mma_16816(st.o[s][rt], va[0], va[1], va[2], va[3], pb[u][rt][0], pb[u][rt][1]);
     }
@@ -274,7 +277,7 @@ __global__ void __launch_bounds__(kBlockThreads, 2) pool_attn_shared_kernel(cons
   constexpr uint32_t kFull = U == 2 ? 0xffffffffu : 0xffffu;
   // ldmatrix of K: lanes 0-15 name the 16 keys' low halves of 16 elements, 16-31 the high ones; of V, transposed: lanes 0-7 and 8-15 keys
   // 0-7 (low, high), 16-23 and 24-31 keys 8-15
-  const uint32_t k_lane = lane_rows<DP>(lane & 15, lane >> 4), v_lane = lane_rows<DP>((lane & 7) + ((lane & 16) >> 1), lane >> 3 & 1);
+  const uint32_t k_lane = RowLayout<DP>::piece(lane & 15, lane >> 4), v_lane = RowLayout<DP>::piece((lane & 7) + ((lane & 16) >> 1), lane >> 3 & 1);
   if (tid == 0) {
     note_of(a, blockIdx.x)->last = -1;
     sm.poison[0] = sm.poison[1] = 0;
@@ -340,7 +343,7 @@ __global__ void __launch_bounds__(kBlockThreads, 2) pool_attn_shared_kernel(cons
     }
     if (!RowQueries<DP>::kInRegisters) {
       constexpr int kPieces = DP / 8;
-      q.shared = ptx::smem_u32(sm.q) + row_group * 16 * C::kRowBytes + lane_rows<DP>(lane & 7, lane >> 3);
+      q.shared = ptx::smem_u32(sm.q) + row_group * 16 * C::kRowBytes + RowLayout<DP>::piece(lane & 7, lane >> 3);
       for (int i = tid; i < kRows * kPieces; i += kBlockThreads) {
         const int row = i / kPieces, part = i % kPieces;
         int token, head;
@@ -349,7 +352,7 @@ __global__ void __launch_bounds__(kBlockThreads, 2) pool_attn_shared_kernel(cons
         if (token < a.q_len && part * 8 < a.head_dim)
           x = *reinterpret_cast<const uint4*>(static_cast<const char*>(a.q) + (c.b * a.q_strides[0] + head * a.q_strides[1] + token * a.q_strides[2] + part * 8) * 2);
         if (kScaled) x = permuted(x);
-        st_shared_16(ptx::smem_u32(sm.q) + piece_at<DP>(row, part), x);
+        st_shared_16(ptx::smem_u32(sm.q) + RowLayout<DP>::piece(row, part), x);
       }
     }
     State<DP, 2> st;
