@@ -3,175 +3,12 @@
 #include <limits.h>
 #include <math.h>
 
-#include <atomic>
-
-#include "pool_attn_shared.cuh"
+#include "pool_attn_simt.cuh"
 
 namespace wm {
 namespace {
 
 using namespace pool;
-
-// ---------------------------------------------------------------- fp32 queries
-// Products in fp32 on the FMA pipe: four elements per lane, LPK lanes per key, R rows per block.
-template <int kStorage>
-struct Held;  // how four elements of a row come in
-template <>
-struct Held<WM_F32> {
-  static constexpr int kBytes = 4;
-  __device__ static void load(const char* p, float (&x)[4]) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
-    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-  }
-};
-template <>
-struct Held<WM_INT8> {
-  static constexpr int kBytes = 1;
-  __device__ static void load(const char* p, float (&x)[4]) { codes_to_float(*reinterpret_cast<const uint32_t*>(p), true, x); }
-};
-template <>
-struct Held<WM_E4M3> {
-  static constexpr int kBytes = 1;
-  __device__ static void load(const char* p, float (&x)[4]) { codes_to_float(*reinterpret_cast<const uint32_t*>(p), false, x); }
-};
-
-template <int R>
-struct SimtState {
-  float q[R][4], m[R], l[R], acc[R][4];
-  int token[R];  // -1: no such row, or a padding node
-};
-
-// One warp takes its 32 keys of a tile: KPW keys at a time.
-template <int R, int LPK, int kStorage, bool kDraft>
-__device__ __forceinline__ void simt_keys(const wm_pool_attn_args& a, const Piece& c, int first, int limit, SimtState<R>& s) {
-  constexpr int KPW = 32 / LPK;
-  const int lane = threadIdx.x & 31, part = lane % LPK, which = lane / LPK;
-  const bool live = part * 4 < a.head_dim;
-  const int64_t* ks = kDraft ? a.draft_k_strides : a.k_strides;
-  const int64_t* vs = kDraft ? a.draft_v_strides : a.v_strides;
-  const char* k = static_cast<const char*>(kDraft ? a.draft_k : a.k) + (c.b * ks[0] + c.kv_head * ks[1] + part * 4) * Held<kStorage>::kBytes;
-  const char* v = static_cast<const char*>(kDraft ? a.draft_v : a.v) + (c.b * vs[0] + c.kv_head * vs[1] + part * 4) * Held<kStorage>::kBytes;
-  const int words = (a.q_len + 31) / 32;
-  const uint32_t* bits = kDraft ? a.ancestors + (a.shared_tree ? 0ll : static_cast<long long>(c.b) * a.q_len * words) : nullptr;
-  const int* depths = kDraft ? a.depths + (a.shared_tree ? 0ll : static_cast<long long>(c.b) * a.q_len) : nullptr;
-  for (int j0 = first; j0 < first + 32 && j0 < limit; j0 += KPW) {
-    const int j = j0 + which;
-    bool seen = j < limit;
-    if (seen && kDraft) seen = depths[j] >= 0;
-    if (seen && !kDraft && a.key_mask != nullptr) seen = a.key_mask[static_cast<long long>(c.b) * a.k_len + j] != 0;
-    float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f}, kscale = a.scale * kLog2e, vscale = 1.f;
-    if (seen) {
-      if (live) {
-        Held<kStorage>::load(k + j * ks[2] * Held<kStorage>::kBytes, x);
-        Held<kStorage>::load(v + j * vs[2] * Held<kStorage>::kBytes, y);
-      }
-      if (kStorage == WM_INT8 || kStorage == WM_E4M3) {
-        kscale *= a.k_scales[c.b * a.k_scale_strides[0] + c.kv_head * a.k_scale_strides[1] + j * a.k_scale_strides[2]];
-        vscale = a.v_scales[c.b * a.v_scale_strides[0] + c.kv_head * a.v_scale_strides[1] + j * a.v_scale_strides[2]];
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float d = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) d = fmaf(s.q[r][e], x[e], d);
-#pragma unroll
-      for (int o = LPK / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-      bool use = seen && s.token[r] >= 0;
-      if (kDraft && use) use = (bits[static_cast<long long>(s.token[r]) * words + (j >> 5)] >> (j & 31)) & 1u;
-      if (!use) continue;
-      d *= kscale;
-      const float top = fmaxf(s.m[r], d);
-      const float ref = top == -INFINITY ? 0.f : top;
-      const float keep = exp2f(s.m[r] - ref), p = exp2f(d - ref);
-      s.m[r] = top;
-      s.l[r] = fmaf(s.l[r], keep, p);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s.acc[r][e] = fmaf(p * vscale, y[e], s.acc[r][e] * keep);
-    }
-  }
-}
-
-template <int kStorage, int LPK, int R>
-__global__ void __launch_bounds__(kThreads) pool_attn_simt_kernel(const wm_pool_attn_args a, const Plan plan) {
-  __shared__ float sm_m[kWarps][R], sm_l[kWarps][R], sm_acc[kWarps][R][LPK * 4];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = lane % LPK;
-  Share share = find_share(a, plan, blockIdx.x, gridDim.x);
-  if (threadIdx.x == 0) note_of(a, blockIdx.x)->last = -1;
-  for (int at = share.begin; at < share.end;) {
-    const Piece c = next_piece(a, plan, at, share.end, share.b, share.b_begin);
-    at = c.end;
-    if (c.tile >= c.stop) continue;
-    SimtState<R> s;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      int token, head;
-      row_place(a, plan, c.kv_head, c.row_block, r, token, head);
-      s.token[r] = token < a.q_len ? token : -1;
-      s.m[r] = -INFINITY;
-      s.l[r] = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s.q[r][e] = s.acc[r][e] = 0.f;
-      if (s.token[r] >= 0) {
-        if (part * 4 < a.head_dim)
-          Held<WM_F32>::load(static_cast<const char*>(a.q) + (c.b * a.q_strides[0] + head * a.q_strides[1] + token * a.q_strides[2] + part * 4) * 4, s.q[r]);
-        if (a.depths != nullptr && a.depths[(a.shared_tree ? 0ll : static_cast<long long>(c.b) * a.q_len) + token] < 0) s.token[r] = -1;
-      }
-    }
-    for (int tile = c.tile; tile < c.stop; ++tile) {
-      if (tile < c.past_tiles)
-        simt_keys<R, LPK, kStorage, false>(a, c, tile * kTileKeys + warp * 32, c.slots, s);
-      else if (a.ancestors != nullptr)
-        simt_keys<R, LPK, WM_F32, true>(a, c, (tile - c.past_tiles) * kTileKeys + warp * 32, a.q_len, s);
-    }
-    // join the lane groups of the warp, then the warps
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-#pragma unroll
-      for (int o = LPK; o < 32; o <<= 1) {
-        const float m = __shfl_xor_sync(0xffffffffu, s.m[r], o), l = __shfl_xor_sync(0xffffffffu, s.l[r], o);
-        const float top = fmaxf(s.m[r], m), ref = top == -INFINITY ? 0.f : top;
-        const float f = exp2f(s.m[r] - ref), g = exp2f(m - ref);
-        s.l[r] = s.l[r] * f + l * g;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s.acc[r][e] = s.acc[r][e] * f + __shfl_xor_sync(0xffffffffu, s.acc[r][e], o) * g;
-        s.m[r] = top;
-      }
-      if (lane < LPK) {
-        if (lane == 0) sm_m[warp][r] = s.m[r], sm_l[warp][r] = s.l[r];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sm_acc[warp][r][part * 4 + e] = s.acc[r][e];
-      }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < R * a.head_dim; i += kThreads) {
-      const int r = i / a.head_dim, d = i - r * a.head_dim;
-      int token, head;
-      row_place(a, plan, c.kv_head, c.row_block, r, token, head);
-      if (token >= a.q_len) continue;
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w][r]);
-      const float ref = top == -INFINITY ? 0.f : top;
-      float l = 0.f, acc = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = exp2f(sm_m[w][r] - ref);
-        l += sm_l[w][r] * f;
-        acc += sm_acc[w][r][d] * f;
-      }
-      if (whole(c)) {
-        static_cast<float*>(a.out)[c.b * a.out_strides[0] + head * a.out_strides[1] + token * a.out_strides[2] + d] = l == 0.f ? 0.f : acc / l;
-      } else {
-        float* row = partial_row(a, plan, gridDim.x, blockIdx.x, c.tile == 0, r);
-        if (d == 0) row[0] = top, row[1] = l;
-        row[2 + d] = acc;
-      }
-    }
-    if (threadIdx.x == 0) leave_note(a, share, c, blockIdx.x, gridDim.x);
-    __syncthreads();
-  }
-}
 
 // ---------------------------------------------------------------- joining the pieces of a segment
 // Block (i, j) joins rows 8 j .. of the segment that share i began and left unfinished, if its note names one.
@@ -238,13 +75,13 @@ bool in_shared(const wm_pool_attn_args& a) { return a.dtype == WM_BF16 && rows_o
 
 int rows_per_block(const wm_pool_attn_args& a) {
   const long long rows = rows_of(a);
-  return a.dtype == WM_F32 ? (rows == 1 ? 1 : 4) : in_shared(a) ? shared_rows_per_block(rows, a.storage, a.head_dim) : rows <= 8 ? 8 : 16;
+  return a.dtype == WM_F32 ? (rows == 1 ? 1 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16) : in_shared(a) ? shared_rows_per_block(rows, a.storage, a.head_dim) : rows <= 8 ? 8 : 16;
 }
 
 // One wave: as many shares as blocks fit the GPU, and no more than there can be units.
 int count_shares(const wm_pool_attn_args& a, const Plan& p) {
   const double tiles = static_cast<double>((a.k_len + kTileKeys - 1) / kTileKeys + p.draft_tiles + p.segment_cost) * a.batch * a.kv_heads * p.row_blocks;
-  const int wave = kSms * (a.dtype == WM_F32 ? 6 : in_shared(a) ? 2 : resident_blocks(a.storage, p.rows_per_block / 8, a.head_dim));
+  const int wave = kSms * (a.dtype == WM_F32 ? simt_resident_blocks(p.rows_per_block) : in_shared(a) ? 2 : resident_blocks(a.storage, p.rows_per_block / 8, a.head_dim));
   return tiles < wave ? (tiles < 1 ? 1 : static_cast<int>(tiles)) : wave;
 }
 
@@ -303,22 +140,6 @@ int validate(const wm_pool_attn_args& a, Plan& plan) {
     if (strides[2] < 0 || strides[2] >= 1 << 24) return fail(WM_EUNSUPPORTED, "%s: pool rows must be less than 2^24 elements apart", who);
   if (!make_plan(a, plan)) return fail(WM_EUNSUPPORTED, "%s: too many query rows", who);
   return WM_OK;
-}
-
-template <int kStorage, int LPK>
-cudaError_t launch_simt_rows(const wm_pool_attn_args& a, const Plan& plan, cudaStream_t stream) {
-  if (plan.rows_per_block == 1)
-    pool_attn_simt_kernel<kStorage, LPK, 1><<<plan.blocks, kThreads, 0, stream>>>(a, plan);
-  else
-    pool_attn_simt_kernel<kStorage, LPK, 4><<<plan.blocks, kThreads, 0, stream>>>(a, plan);
-  return cudaGetLastError();
-}
-
-template <int kStorage>
-cudaError_t launch_simt(const wm_pool_attn_args& a, const Plan& plan, cudaStream_t stream) {
-  if (a.head_dim <= 32) return launch_simt_rows<kStorage, 8>(a, plan, stream);
-  if (a.head_dim <= 64) return launch_simt_rows<kStorage, 16>(a, plan, stream);
-  return launch_simt_rows<kStorage, 32>(a, plan, stream);
 }
 
 }  // namespace

@@ -1,6 +1,4 @@
 // Pool attention over e4m3 pools, many rows per KV head (see pool_attn_shared.cuh).
-#include <atomic>
-
 #include "pool_attn_shared.cuh"
 
 namespace wm {

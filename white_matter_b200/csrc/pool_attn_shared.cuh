@@ -12,6 +12,8 @@
 // stored as zeros.
 #pragma once
 
+#include <atomic>
+
 #include "pool_attn_mma.cuh"
 
 namespace wm {
@@ -531,21 +533,30 @@ __global__ void __launch_bounds__(kBlockThreads, 2) pool_attn_shared_kernel(cons
   }
 }
 
+// More than 48 KB of shared memory are opted into once per device and kernel.
+struct DeviceFlags {
+  static constexpr int kDevices = 64;
+  std::atomic<bool> set[kDevices];
+};
+template <typename Kernel>
+cudaError_t opt_in(Kernel* kernel, int bytes, DeviceFlags& done) {
+  int device = 0;
+  cudaError_t error = cudaGetDevice(&device);
+  if (error != cudaSuccess) return error;
+  const bool known = device >= 0 && device < DeviceFlags::kDevices;
+  if (known && done.set[device].load(std::memory_order_acquire)) return cudaSuccess;
+  error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (error == cudaSuccess && known) done.set[device].store(true, std::memory_order_release);
+  return error;
+}
+
 template <int kStorage, int DP, int kRowGroups, bool kTree>
 cudaError_t launch_shared_rows(const wm_pool_attn_args& a, const Plan& plan, cudaStream_t stream) {
   constexpr int kBytes = static_cast<int>(sizeof(BlockShared<kStorage, DP, kRowGroups>));
   static_assert(kBytes <= 232448 / 2 - 1024, "two blocks per SM");
-  // more than 48 KB is opted into once per device
-  constexpr int kMaxDevices = 64;
-  static std::atomic<bool> done[kMaxDevices];
-  int device = 0;
-  cudaError_t error = cudaGetDevice(&device);
+  static DeviceFlags done;
+  const cudaError_t error = opt_in(pool_attn_shared_kernel<kStorage, DP, kRowGroups, kTree>, kBytes, done);
   if (error != cudaSuccess) return error;
-  if (device < 0 || device >= kMaxDevices || !done[device].load(std::memory_order_acquire)) {
-    error = cudaFuncSetAttribute(pool_attn_shared_kernel<kStorage, DP, kRowGroups, kTree>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-    if (error != cudaSuccess) return error;
-    if (device >= 0 && device < kMaxDevices) done[device].store(true, std::memory_order_release);
-  }
   pool_attn_shared_kernel<kStorage, DP, kRowGroups, kTree><<<plan.blocks, kBlockThreads, kBytes, stream>>>(a, plan);
   return cudaGetLastError();
 }
