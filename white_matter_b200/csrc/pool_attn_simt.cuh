@@ -1,12 +1,15 @@
 // Pool attention for fp32 queries: products and sums in fp32 on the FMA pipe, over fp32 and 8-bit pools.
 //
 // A block of eight warps takes R rows of a KV head over a step of kStepKeys keys, whose rows arrive in shared memory by
-// asynchronous copies one step ahead.  Scores: a thread per key and set of rows, the whole head_dim, so that no lane has
-// to add with another; keys lie 16 bytes more than their size apart, which keeps them off each other's banks.  A warp per
-// row turns the scores into weights against the row's running maximum.  Values: a thread per four elements and every n-th key,
-// all R rows in its registers; those sums meet once per piece.
+// asynchronous copies one step ahead.  Scores: a thread per key, part of head_dim and up to eight rows; keys lie 16 bytes more than
+// their size apart, which keeps them off each other's banks.  A warp per row turns the scores into weights against the row's
+// running maximum.  Values: a thread per four elements and every n-th key, all R rows in its registers; those sums meet once
+// per piece of a segment.
 //
-// Few rows are bound by HBM, many by shared memory (a key's 16 bytes serve 4 R / row-sets products).  XXX
+// Few rows are bound by HBM, many by the reads of shared memory beside the products (16 bytes of a key serve eight rows at
+// most, 16 bytes of a query one key).  8 sequences of up to 8192 fp32 rows of 64, 16 heads: one token 52 us (5 130 GB/s), 8 drafted
+// tokens 85 us, 16 153 us (14 TFLOP/s).  Rows per thread, on 8 sequences of up to 4100 fp32 rows of 128 with 16 tokens and 4
+// heads per KV head: 4, 8, 16 take 332, 282, 424 us.
 #pragma once
 
 #include "pool_attn_shared.cuh"
@@ -115,60 +118,80 @@ __device__ __forceinline__ void simt_step(SimtShared<kStorage, DP, R>& sm, const
   using C = SimtCfg<kStorage, DP>;
   constexpr int kHeld = kDraft ? WM_F32 : kStorage, kBytes = kHeld == WM_F32 ? 4 : 1;
   constexpr int kKeys = kDraft ? C::kDraftKeys : C::kStepKeys, kPitch = kDraft ? C::kDraftPitch : C::kPitch;
-  constexpr int kSets = kBlockThreads / kKeys, kMine = R > kSets ? R / kSets : 1;  // sets of rows side by side, rows of a set
+  // The threads of a key: kSets with kEach rows each, and in a set kParts with every kParts-th 16 bytes of the key's row.  They
+  // lie so that eight lanes read eight different banks.
+  constexpr int kPerKey = kBlockThreads / kKeys, kEach = R < 8 ? R : 8, kSets = kPerKey < R / kEach ? kPerKey : R / kEach;
+  constexpr int kRows = R / kSets, kParts = kPerKey / kSets, kSide = kParts < 8 ? 32 / kParts : 1, kMine = kRows > kParts ? kRows / kParts : 1;
   constexpr int LPK = DP / 4, kSlices = kBlockThreads / LPK;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   {
-    const int key = tid % kKeys, set = tid / kKeys;
-    if (set < R) {
-      const unsigned char* row = sm.tile[stage][0] + key * kPitch;
-      float d[kMine][4] = {};
-#pragma unroll 2
-      for (int e = 0; e < a.head_dim; e += 16 / kBytes) {
-        const uint4 held = *reinterpret_cast<const uint4*>(row + e * kBytes);
-        const uint32_t word[4] = {held.x, held.y, held.z, held.w};
+    const int part = lane / kSide % kParts, key = warp % (kBlockWarps / kSets) * (32 / kParts) + (kParts < 8 ? lane % kSide : lane / kParts);
+    const unsigned char* row = sm.tile[stage][0] + key * kPitch;
+    int first = warp / (kBlockWarps / kSets) * kRows;
+    float d[kRows] = {};
+#pragma unroll kBytes == 4 ? 2 : 1
+    for (int e = part * (16 / kBytes); e < a.head_dim; e += kParts * (16 / kBytes)) {
+      const uint4 held = *reinterpret_cast<const uint4*>(row + e * kBytes);
+      const uint32_t word[4] = {held.x, held.y, held.z, held.w};
 #pragma unroll
-        for (int u = 0; u < 4 / kBytes; ++u) {
-          float x[4];
-          if (kHeld == WM_F32) {
+      for (int u = 0; u < 4 / kBytes; ++u) {
+        float x[4];
+        if (kHeld == WM_F32) {
 #pragma unroll
-            for (int n = 0; n < 4; ++n) x[n] = __uint_as_float(word[n]);
-          } else {
-            codes_to_float(word[u], kHeld == WM_INT8, x);
-          }
+          for (int n = 0; n < 4; ++n) x[n] = __uint_as_float(word[n]);
+        } else {
+          codes_to_float(word[u], kHeld == WM_INT8, x);
+        }
 #pragma unroll
-          for (int i = 0; i < kMine; ++i) {
-            const float4 y = *reinterpret_cast<const float4*>(&sm.q[set + i * kSets][e + 4 * u]);
-            d[i][0] = fmaf(x[0], y.x, d[i][0]);
-            d[i][1] = fmaf(x[1], y.y, d[i][1]);
-            d[i][2] = fmaf(x[2], y.z, d[i][2]);
-            d[i][3] = fmaf(x[3], y.w, d[i][3]);
-          }
+        for (int r = 0; r < kRows; ++r) {
+          const float4 y = *reinterpret_cast<const float4*>(&sm.q[first + r][e + 4 * u]);
+          d[r] = fmaf(x[0], y.x, d[r]);
+          d[r] = fmaf(x[1], y.y, d[r]);
+          d[r] = fmaf(x[2], y.z, d[r]);
+          d[r] = fmaf(x[3], y.w, d[r]);
         }
       }
-      float factor = a.scale * kLog2e;
-      if (kHeld != WM_F32) factor *= sm.scale[kHeld != WM_F32 ? stage : 0][0][key];
-      const bool seen = kDraft ? key < there : sm.seen[stage][key] != 0;
+    }
+    // the parts' sums, each lane keeping its share of the rows: rows `first` .. first + kMine - 1
+    __syncwarp();
 #pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        const int r = set + i * kSets;
-        bool use = seen;
-        if (kDraft && seen) {
-          const int token = sm.token[r], words = (a.q_len + 31) / 32, j = j0 + key;
-          use = token >= 0 && (a.ancestors[((a.shared_tree ? 0ll : static_cast<long long>(c.b) * a.q_len) + token) * words + (j >> 5)] >> (j & 31) & 1u);
+    for (int o = 1, n = kRows; o < kParts; o *= 2) {
+      const int to = o * kSide;
+      if (n > 1) {
+        n /= 2;
+        const bool high = lane & to;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+          const float other = high ? d[i] : d[n + i];
+          d[i] = (high ? d[n + i] : d[i]) + __shfl_xor_sync(0xffffffffu, other, to);
         }
-        sm.s[r][key] = use ? ((d[i][0] + d[i][1]) + (d[i][2] + d[i][3])) * factor : -INFINITY;
+        first += high ? n : 0;
+      } else {
+        d[0] += __shfl_xor_sync(0xffffffffu, d[0], to);
       }
+    }
+    float factor = a.scale * kLog2e;
+    if (kHeld != WM_F32) factor *= sm.scale[kHeld != WM_F32 ? stage : 0][0][key];
+    const bool seen = kDraft ? key < there : sm.seen[stage][key] != 0;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int r = first + i;
+      bool use = seen;
+      if (kDraft && seen) {
+        const int token = sm.token[r], words = (a.q_len + 31) / 32, j = j0 + key;
+        use = token >= 0 && (a.ancestors[((a.shared_tree ? 0ll : static_cast<long long>(c.b) * a.q_len) + token) * words + (j >> 5)] >> (j & 31) & 1u);
+      }
+      sm.s[r][key] = use ? d[i] * factor : -INFINITY;
     }
   }
   __syncthreads();
 #pragma unroll 1
   for (int r = warp; r < R; r += kBlockWarps) {
-    constexpr int kEach = kKeys > 32 ? kKeys / 32 : 1;
+    constexpr int kKeysEach = kKeys > 32 ? kKeys / 32 : 1;
     const float before = sm.m[r];
-    float x[kEach], top = before;
+    float x[kKeysEach], top = before;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
+    for (int i = 0; i < kKeysEach; ++i) {
       x[i] = lane < kKeys ? sm.s[r][lane + 32 * i] : -INFINITY;
       top = fmaxf(top, x[i]);
     }
@@ -177,7 +200,7 @@ __device__ __forceinline__ void simt_step(SimtShared<kStorage, DP, R>& sm, const
     const float ref = top == -INFINITY ? 0.f : top, keep = exp2f(before - ref);
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
+    for (int i = 0; i < kKeysEach; ++i) {
       const int key = lane + 32 * i;
       const float p = exp2f(x[i] - ref);
       sum += p;
