@@ -31,7 +31,8 @@ extern "C" {
  * is row i of the source or, with index, row index[b*rows + i] of its source_rows rows.  Slots outside the pool and
  * indices outside the source are skipped: such a slot keeps what it held.  Pool tensors are (batch, heads, slots,
  * head_dim), scales (batch, heads, slots), sources (batch, heads, source_rows, head_dim), with element strides for
- * (batch, head, token).  head_dim is a multiple of 16 up to 256; pool rows and source rows are 16-byte aligned. */
+ * (batch, head, token).  head_dim is a multiple of 16 up to 128; pool rows and source rows are 16-byte aligned.
+ * The pool must not overlap the source. */
 typedef struct wm_pool_commit_args {
   void* keys;
   void* values;
@@ -88,7 +89,11 @@ typedef struct wm_draft_tree_args {
  * s < lengths[b] + lead (lengths NULL: all) that key_mask keeps.  With ancestors, the queries are the nodes of a tree of
  * drafted tokens: node i also sees the rows j of draft_k / draft_v that its ancestor bits name, and a padding node
  * (depths[i] < 0) sees nothing.  Rows that see nothing are written as zeros.  Rows of the pool that are not seen are
- * not read, or not used; rows of padding nodes in draft_k / draft_v neither. */
+ * not read, or not used; rows of padding nodes in draft_k / draft_v neither.
+ * head_dim at most 128, rows of every tensor multiples of 16 bytes and 16-byte aligned, at most 512 drafted tokens; rows of
+ * the pool and of its scales lie less than 2^24 elements apart; batch * kv_heads * row blocks * tiles of 128 keys below 2^31.
+ * Other calls are refused with WM_EUNSUPPORTED.  The workspace (wm_pool_attn_workspace_bytes, the same for every content of the
+ * tensors) must not be shared by calls that may run at once. */
 typedef struct wm_pool_attn_args {
   const void* q; /* (batch, q_heads, q_len, head_dim) */
   const void* k; /* (batch, kv_heads, k_len, head_dim) in `storage` */

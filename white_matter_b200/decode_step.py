@@ -123,7 +123,6 @@ class KVPoolCache:
             key_mask=key_mask, softmax_scale=softmax_scale, static_cache=True,
         )
 
-
     def read_tree(
         self,
         query: torch.Tensor,
