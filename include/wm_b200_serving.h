@@ -92,7 +92,7 @@ typedef struct wm_draft_tree_args {
  * not read, or not used; rows of padding nodes in draft_k / draft_v neither.
  * head_dim at most 128, rows of every tensor multiples of 16 bytes and 16-byte aligned, at most 512 drafted tokens; rows of
  * the pool and of its scales lie less than 2^24 elements apart; batch * kv_heads * row blocks * tiles of 128 keys below 2^31.
- * Other calls are refused with WM_EUNSUPPORTED.  The workspace (wm_pool_attn_workspace_bytes, the same for every content of the
+ * Other calls are refused with WM_EUNSUPPORTED.  The workspace (wm_pool_attn_workspace_bytes, 16-byte aligned, the same for every content of the
  * tensors) must not be shared by calls that may run at once. */
 typedef struct wm_pool_attn_args {
   const void* q; /* (batch, q_heads, q_len, head_dim) */

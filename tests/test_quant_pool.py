@@ -85,6 +85,32 @@ def test_attention_refusals(change, status, text):
 
 
 @pytest.mark.parametrize(
+    "change, text",
+    [
+        (dict(out=(1 << 20) + 4), b"output rows"),
+        (dict(out_strides=_native._Strides(4096, 1024, 33)), b"output rows"),
+        (dict(workspace=(1 << 20) + 8), b"workspace must be"),
+        (dict(k_len=2**31 - 1), b"too many slots"),
+        (dict(k_strides=_native._Strides(4096, 1024, 1 << 24)), b"2^24"),
+    ],
+)
+def test_attention_refuses_what_it_could_not_address(change, text):
+    lib = _native.load_library()
+    assert lib.wm_pool_attn(ctypes.byref(fake_attn(**change)), None) == -2
+    assert text in lib.wm_last_error()
+
+
+def test_read_back_refuses_more_slots_than_it_counts():
+    a = _native.PoolDequantArgs()
+    for name in ("codes", "scales", "out"):
+        setattr(a, name, 1 << 20)
+    a.code_strides = a.out_strides = _native._Strides(1 << 35, 1 << 35, 16)
+    a.storage, a.dtype, a.batch, a.heads, a.slots, a.head_dim = _native.WM_INT8, _native.WM_BF16, 1, 1, 2**31 - 1, 16
+    lib = _native.load_library()
+    assert lib.wm_pool_dequant(ctypes.byref(a), None) == -2 and b"too many slots" in lib.wm_last_error()
+
+
+@pytest.mark.parametrize(
     "change, status, text",
     [
         (dict(lengths=None), -1, b"lengths"),
@@ -498,3 +524,34 @@ def test_two_streams_at_once_do_not_disturb_each_other():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(r, alone[i]) for r in results[i])
+
+
+@pytest.mark.gpu
+@on_gpu
+def test_nothing_that_requires_grad_is_taken():
+    pool = QuantKVPoolCache(1, 1, 2, 16, 64)
+    rows = torch.randn(1, 2, 3, 64, device="cuda").bfloat16()
+    pool.append(rows, rows)
+    query, scales = torch.randn(1, 2, 1, 64, device="cuda").bfloat16(), pool.key_scales.clone().requires_grad_()
+    with pytest.raises(ValueError, match="no gradients"):
+        quantized_pool_attention(query, pool.keys, pool.values, scales, pool.value_scales)
+    with pytest.raises(ValueError, match="no gradients"):
+        quantized_pool_append(pool.keys, pool.values, scales, pool.value_scales, pool.lengths, rows, rows)
+    with pytest.raises(ValueError, match="no gradients"):
+        dequantize_kv_rows(pool.keys, scales)
+    with torch.no_grad():
+        quantized_pool_attention(query, pool.keys, pool.values, scales, pool.value_scales)
+
+
+@pytest.mark.gpu
+@on_gpu
+def test_a_captured_step_notices_replaced_scales():
+    pool = QuantKVPoolCache(1, 1, 2, 16, 64)
+    rows = torch.randn(1, 2, 3, 64, device="cuda").bfloat16()
+    pool.append(rows, rows)
+    query = torch.randn(1, 2, 1, 64, device="cuda").bfloat16()
+    step = DecodeStepGraph(lambda: pool.read(query, 0), pool)
+    step()
+    pool.key_scales = pool.key_scales.clone()
+    with pytest.raises(ValueError, match="capture the step again"):
+        step()

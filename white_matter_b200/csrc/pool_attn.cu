@@ -65,7 +65,6 @@ __global__ void __launch_bounds__(kJoinThreads) pool_attn_join_kernel(const wm_p
 }
 
 // ---------------------------------------------------------------- host
-constexpr int kMaxTreeNodes = 512;
 constexpr int kSms = 148;
 
 long long rows_of(const wm_pool_attn_args& a) { return static_cast<long long>(a.q_heads / a.kv_heads) * a.q_len; }
@@ -138,6 +137,8 @@ int validate(const wm_pool_attn_args& a, Plan& plan) {
     return fail(WM_EUNSUPPORTED, "%s: rows must be 16-byte aligned", who);
   for (const int64_t* strides : {a.k_strides, a.v_strides, a.k_scale_strides, a.v_scale_strides})
     if (strides[2] < 0 || strides[2] >= 1 << 24) return fail(WM_EUNSUPPORTED, "%s: pool rows must be less than 2^24 elements apart", who);
+  if (!aligned16(a.out) || !aligned16(a.out_strides, wide) || !aligned16(a.workspace)) return fail(WM_EUNSUPPORTED, "%s: output rows and workspace must be 16-byte aligned", who);
+  if (a.k_len > kMaxSlots) return fail(WM_EUNSUPPORTED, "%s: too many slots", who);
   if (!make_plan(a, plan)) return fail(WM_EUNSUPPORTED, "%s: too many query rows", who);
   return WM_OK;
 }
@@ -146,7 +147,7 @@ int validate(const wm_pool_attn_args& a, Plan& plan) {
 
 size_t pool_attn_workspace(const wm_pool_attn_args& a) {
   Plan plan;
-  if (a.batch < 1 || a.kv_heads < 1 || a.q_heads < a.kv_heads || a.q_len < 1 || a.k_len < 1 || !make_plan(a, plan)) return 0;
+  if (a.batch < 1 || a.kv_heads < 1 || a.q_heads < a.kv_heads || a.q_len < 1 || a.k_len < 1 || a.k_len > kMaxSlots || !make_plan(a, plan)) return 0;
   if (plan.cluster > 0) return 0;
   return static_cast<size_t>(plan.blocks) * (sizeof(Note) + 2 * plan.rows_per_block * (a.head_dim + 2) * sizeof(float));
 }

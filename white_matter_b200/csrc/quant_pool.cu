@@ -248,7 +248,6 @@ __global__ void __launch_bounds__(kThreads) pool_dequant_kernel(const wm_pool_de
 // Pointer doubling over bit sets: after r rounds a node knows its 2^r nearest ancestors and the one 2^r steps up, and
 // takes over that one's set in the next round.  One block per tree, one thread per node; a round reads its neighbours'
 // state, meets, and writes.  Chains that have not ended after the rounds a chain of `tokens` nodes takes are cycles.
-constexpr int kMaxTreeNodes = 512;
 constexpr int kTreeWords = kMaxTreeNodes / 32;
 constexpr int kRoot = -1, kDead = -2;
 
@@ -341,6 +340,7 @@ int pool_dequant_launch(const wm_pool_dequant_args& a, cudaStream_t stream) {
   if (a.head_dim % 16 || a.head_dim > 128) return fail(WM_EUNSUPPORTED, "%s: head_dim must be a multiple of 16 up to 128", who);
   const long long planes = static_cast<long long>(a.batch) * a.heads;
   if (planes > INT_MAX) return fail(WM_EUNSUPPORTED, "%s: too many (sequence, head) planes", who);
+  if (a.slots > kMaxSlots) return fail(WM_EUNSUPPORTED, "%s: too many slots", who);
   const int wide = a.dtype == WM_F32 ? 4 : 2;
   if (!aligned16(a.codes) || !aligned16(a.out) || !aligned16(a.code_strides, 1) || !aligned16(a.out_strides, wide))
     return fail(WM_EUNSUPPORTED, "%s: rows must be 16-byte aligned", who);

@@ -7,6 +7,9 @@
 
 namespace wm {
 
+constexpr int kMaxTreeNodes = 512;      // drafted tokens per tree
+constexpr int kMaxSlots = 0x7fffff00;  // of a pool: the kernels step a few rows past the last one in 32 bits
+
 int pool_commit_launch(const wm_pool_commit_args& a, cudaStream_t stream);
 int pool_dequant_launch(const wm_pool_dequant_args& a, cudaStream_t stream);
 int draft_tree_launch(const wm_draft_tree_args& a, cudaStream_t stream);

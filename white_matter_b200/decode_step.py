@@ -76,7 +76,7 @@ class KVPoolCache:
         Device-side: the write positions come from ``lengths`` on the GPU, so the call can be captured in a CUDA
         graph and replayed while the lengths grow.  Rows that would not fit the capacity are dropped.  ``index`` (B,m)
         commits rows ``index[b, i]`` of the new ones instead, ``counts`` (B,) only the first ``counts[b]``: the
-        accepted branch of a draft.
+        accepted branch of a draft (D a multiple of 16 up to 128).  The new rows must not be views of this pool.
         """
         if index is not None or counts is not None:
             if key.dtype != self.keys.dtype:
@@ -278,7 +278,7 @@ class DecodeStepGraph:
         if not cache.keys.is_cuda:
             raise ValueError("decode capture requires a CUDA pool")
         self.cache = cache
-        self._buffers = (cache.keys, cache.values, cache.lengths)
+        self._buffers = self._held()
         saved = cache.lengths.clone()
         stream = torch.cuda.Stream(device=cache.keys.device)
         stream.wait_stream(torch.cuda.current_stream())
@@ -292,8 +292,12 @@ class DecodeStepGraph:
             self.output = step()
         cache.lengths.copy_(saved)  # capture runs nothing, but the warm-up steps advanced and restored the lengths
 
+    def _held(self) -> tuple:
+        names = ("keys", "values", "lengths", "key_scales", "value_scales")
+        return tuple(getattr(self.cache, name) for name in names if hasattr(self.cache, name))
+
     def __call__(self) -> torch.Tensor:
-        if any(a is not b for a, b in zip(self._buffers, (self.cache.keys, self.cache.values, self.cache.lengths))):
+        if any(a is not b for a, b in zip(self._buffers, self._held())):
             raise ValueError("pool storage changed; capture the step again")
         self.graph.replay()
         return self.output

@@ -27,8 +27,8 @@ _QUANTISED = (torch.int8, torch.float8_e4m3fn)
 _ROWS = (torch.bfloat16, torch.float32)
 
 
-def _refuse_grad(what: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and True in [t.requires_grad for t in tensors]:
+def _refuse_grad(what: str, *tensors: torch.Tensor | None) -> None:
+    if torch.is_grad_enabled() and True in [t is not None and t.requires_grad for t in tensors]:
         raise ValueError(f"{what} has no gradients: call it under torch.no_grad()")
 
 
@@ -96,7 +96,7 @@ def pool_commit(
         raise ValueError("new rows must have the pool's dtype")
     if new_keys.get_device() != device or new_values.get_device() != device:
         raise ValueError("new rows must be on the pool's device")
-    _refuse_grad("a pool commit", new_keys, new_values)
+    _refuse_grad("a pool commit", keys, values, key_scales, value_scales, new_keys, new_values)
     lengths = _int_vector("lengths", lengths, batch, device)
     rows = source_rows = shape[2]
     if index is not None:
@@ -145,7 +145,7 @@ def quantized_pool_append(
     (one further with ``use_dummy_token``).  ``index`` (B,m) picks the rows instead: slot i gets row ``index[b,i]``;
     ``counts`` (B,) bounds the number of rows per sequence -- together they commit the accepted branch of a draft.
     Rows that would not fit the pool, and indices outside the new rows, are skipped: their slots keep what they held.
-    The lengths stay as they are.
+    The lengths stay as they are.  The new rows must not be views of the pool that the call writes.
     """
     if type(use_dummy_token) is not bool:
         raise ValueError("use_dummy_token must be boolean")
@@ -174,6 +174,7 @@ def dequantize_kv_rows(
     if dtype not in _ROWS:
         raise ValueError("rows are read back in bfloat16 or float32")
     (batch, heads, slots, dim), device, _, storage, strides, _, scale_strides, _, scale, _ = _check_pool(codes, codes, scales, scales)
+    _refuse_grad("a read back", scales)
     if lengths is not None:
         lengths = _int_vector("lengths", lengths, batch, device)
     out = torch.empty_like(codes, dtype=dtype, memory_format=torch.contiguous_format)
@@ -224,9 +225,9 @@ def pool_attention(
     if dim > 128 or dim * wide % 16 or (quantised and dim % 16):
         raise RuntimeError("sm100 pool attention needs rows of a multiple of 16 bytes and head_dim <= 128")
     if draft is None:
-        _refuse_grad("pool attention", query)
+        _refuse_grad("pool attention", query, keys, values, key_scales, value_scales)
     else:
-        _refuse_grad("pool attention", query, draft[0], draft[1])
+        _refuse_grad("pool attention", query, keys, values, key_scales, value_scales, draft[0], draft[1])
     out = query.new_empty((batch, length, heads, dim))
     if not (batch and length and heads and dim):
         return out
