@@ -495,7 +495,20 @@ __global__ void __launch_bounds__(kBlockThreads, 2) pool_attn_shared_kernel(cons
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + c.b * a.out_strides[0] + head * a.out_strides[1] + token * a.out_strides[2];
       float* partial = partial_row(a, plan, gridDim.x, blockIdx.x, c.tile == 0, r);
       if (!whole(c) && tid % kPerRow == 0) *reinterpret_cast<float2*>(partial) = make_float2(top, empty ? 0.f : l);
-      const bool poisoned = kTree && sm.poison[turn] != 0;
+      if (kTree && sm.poison[turn] != 0) {  // drafted values that are not finite, for the rows that see them
+        const int words = (a.q_len + 31) / 32;
+        for (int d = 2 * (tid % kPerRow); d < a.head_dim; d += 2 * kPerRow) {
+          for (int j = 0; j < a.q_len; ++j) {
+            if (!(a.ancestors[(tree + token) * words + (j >> 5)] >> (j & 31) & 1u)) continue;
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(a.draft_v) +
+                                                                  (c.b * a.draft_v_strides[0] + c.kv_head * a.draft_v_strides[1] + j * a.draft_v_strides[2] + d) * 2);
+            if ((x & 0x7f80u) == 0x7f80u) sm.acc[0][r][d] += __uint_as_float(x << 16);
+            if ((x & 0x7f800000u) == 0x7f800000u) sm.acc[0][r][d + 1] += __uint_as_float(x & 0xffff0000u);
+          }
+        }
+      }
+      const bool done = whole(c);
+#pragma unroll 4
       for (int d = 2 * (tid % kPerRow); d < a.head_dim; d += 2 * kPerRow) {
         float2 y = *reinterpret_cast<const float2*>(&sm.acc[0][r][d]);
         if (kSide > 1) {
@@ -503,18 +516,8 @@ __global__ void __launch_bounds__(kBlockThreads, 2) pool_attn_shared_kernel(cons
           y.x += z.x;
           y.y += z.y;
         }
-        if (poisoned) {  // drafted values that are not finite, for the rows that see them
-          const int words = (a.q_len + 31) / 32;
-          for (int j = 0; j < a.q_len; ++j) {
-            if (!(a.ancestors[(tree + token) * words + (j >> 5)] >> (j & 31) & 1u)) continue;
-            const uint32_t x = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(a.draft_v) +
-                                                                  (c.b * a.draft_v_strides[0] + c.kv_head * a.draft_v_strides[1] + j * a.draft_v_strides[2] + d) * 2);
-            if ((x & 0x7f80u) == 0x7f80u) y.x += __uint_as_float(x << 16);
-            if ((x & 0x7f800000u) == 0x7f800000u) y.y += __uint_as_float(x & 0xffff0000u);
-          }
-        }
         if (empty) y = make_float2(0.f, 0.f);
-        if (whole(c))
+        if (done)
           *reinterpret_cast<uint32_t*>(out + d) = empty ? 0u : pack_bf16(y.x * inverse, y.y * inverse);
         else
           *reinterpret_cast<float2*>(partial + 2 + d) = y;
