@@ -12,13 +12,16 @@
 // elements t*DP/4 .. of a key, lane g of eight holds elements g*DP/8 .. of a value row.
 //
 // Codes of 8-bit pools become bf16 in registers, which is exact; the key's scale multiplies the score in fp32, the
-// value's scale the weight before it is rounded to bf16 (2^-8 relative at most, like the weight of a bf16 pool).
+// value's scale the weight.  Weights over bf16 pools are rounded to bf16 (2^-8 of themselves at most), and the sum takes them as
+// rounded.  Over 8-bit pools they enter the product in two parts, rounded and rest, 16 bits together: with one part, reads of one
+// sequence were 1.2 to 1.5 times as far from the exact result as the output's rounding, with two 1.0, for 5 % of the time of
+// 64 sequences (115.6 -> 121 us) and none on one.  (Over bf16 pools an infinity's product with the rest would be NaN.)
 //
 // A row's weights are exponentials against a reference that moves only when a score exceeds it by 8 (in powers of two):
 // the sums are fp32 and the weights floating, so nothing is lost by weights up to 2^8, and the common step needs
 // one vote instead of a reduction over the lanes.
 //
-// 64 sequences of up to 8192 tokens, 16 heads of 64, one token: 115 us over int8 (4 960 GB/s), 116 us over e4m3, bound by the instructions that
+// 64 sequences of up to 8192 tokens, 16 heads of 64, one token: 121 us over int8 (4 710 GB/s), 121 us over e4m3, bound by the instructions that
 // make bf16 of codes; bf16 with 8 drafted tokens 163 us (6 600 GB/s), bound by HBM.  One sequence of 480 tokens: 5.6 us.
 #pragma once
 
@@ -67,7 +70,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return y;
 }
 // (a & b) | c as one instruction: written as operators with two constants it becomes two, and the conversion of int8 codes is
-// what the 8-bit read spends most of its instructions on (64 sequences of up to 8192 rows: 143 us against 112 us when this was changed, 115 us with the sum of rounded weights)
+// what the 8-bit read spends most of its instructions on (64 sequences of up to 8192 rows: 143 us against 112 us, before the weights were held in two parts)
 __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t y;
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(a), "r"(b), "r"(c));
@@ -223,9 +226,11 @@ struct Keys {
 __device__ __forceinline__ float usable_scale(float scale, bool seen) { return !seen ? 1.f : fabsf(scale) < 0x1p-110f ? 0x1p-110f : scale; }
 
 // Weights of U x 16 keys for every tile, as B operands of O^T += V^T P^T.  x holds the keys' products with the queries (keys
-// g: x[.][.][0], [1]; g + 8: [2], [3]; rows 2t, 2t + 1).
-template <int DP, int RT, int U, bool kScaled, bool kPerRow>
-__device__ __forceinline__ void weights(State<DP, RT>& st, float (&x)[U][RT][4], const Keys (&keys)[U], const uint32_t (&seen)[U][kPerRow ? RT : 1][2], uint32_t (&pb)[U][RT][2]) {
+// g: x[.][.][0], [1]; g + 8: [2], [3]; rows 2t, 2t + 1).  With kFine the weights come in two parts, rounded (pb) and what the
+// rounding left (rest).
+template <int DP, int RT, int U, bool kScaled, bool kPerRow, bool kFine = false>
+__device__ __forceinline__ void weights(State<DP, RT>& st, float (&x)[U][RT][4], const Keys (&keys)[U], const uint32_t (&seen)[U][kPerRow ? RT : 1][2], uint32_t (&pb)[U][RT][2],
+                                        uint32_t (*rest)[RT][2] = nullptr) {
   // x becomes the exponent against the row's reference; -infinity where the row does not see the key
   float over = -INFINITY;
 #pragma unroll
@@ -276,20 +281,26 @@ __device__ __forceinline__ void weights(State<DP, RT>& st, float (&x)[U][RT][4],
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const float inverse[2] = {kScaled ? reciprocal_approx(keys[u].scale[0]) : 1.f, kScaled ? reciprocal_approx(keys[u].scale[1]) : 1.f};
+    const float inverse[2] = {kScaled && !kFine ? reciprocal_approx(keys[u].scale[0]) : 1.f, kScaled && !kFine ? reciprocal_approx(keys[u].scale[1]) : 1.f};
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float(&y)[4] = x[u][rt];
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = exp2_approx(y[e]);
+      if (kFine) {
+        st.l[rt][0] += y[0] + y[2];
+        st.l[rt][1] += y[1] + y[3];
+      }
       if (kScaled) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] *= keys[u].scale[e >> 1];
       }
       const uint32_t b0 = pack_bf16(y[0], y[1]), b1 = pack_bf16(y[2], y[3]);
-      // the sum takes the weights as they are rounded, so that the result is an exact mean of value rows (with the sum of the
-      // unrounded ones a read of 8-bit rows was 1.45 times as far from the exact result as its own rounding to bf16)
-      if (kScaled) {
+      // in one part the sum takes the weights as they are rounded, so that the result is an exact mean of value rows
+      if (kFine) {
+        rest[u][rt][0] = transpose_8x8(pack_bf16(y[0] - __uint_as_float(b0 << 16), y[1] - __uint_as_float(b0 & 0xffff0000u)));
+        rest[u][rt][1] = transpose_8x8(pack_bf16(y[2] - __uint_as_float(b1 << 16), y[3] - __uint_as_float(b1 & 0xffff0000u)));
+      } else if (kScaled) {
         st.l[rt][0] = fmaf(__uint_as_float(b0 << 16), inverse[0], st.l[rt][0]);
         st.l[rt][1] = fmaf(__uint_as_float(b0 & 0xffff0000u), inverse[0], st.l[rt][1]);
         st.l[rt][0] = fmaf(__uint_as_float(b1 << 16), inverse[1], st.l[rt][0]);
@@ -313,7 +324,7 @@ __host__ __device__ constexpr int groups_per_step() {
 
 // This warp's rows of the tiles [tile, stop) that lie among the visible slots.  With kDense the rows of the pool are DP
 // elements and lie one behind the other (scales too): a lane then needs one address for all of its rows of a step.
-template <int kStorage, int DP, int RT, bool kDense>
+template <int kStorage, int DP, int RT, bool kDense, bool kFine>
 __device__ __forceinline__ void past_keys(const wm_pool_attn_args& a, const Piece& c, int tile, int stop, const Queries<DP, RT>& q, State<DP, RT>& st) {
   using R = Rows<kStorage, DP>;
   constexpr bool kScaled = kStorage != WM_BF16;
@@ -418,8 +429,8 @@ __device__ __forceinline__ void past_keys(const wm_pool_attn_args& a, const Piec
       }
       load_k(next);
     }
-    uint32_t pb[U][RT][2];
-    weights<DP, RT, U, kScaled, false>(st, x, keys, seen, pb);
+    uint32_t pb[U][RT][2], rest[U][RT][2];
+    weights<DP, RT, U, kScaled, false, kFine>(st, x, keys, seen, pb, rest);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (!keys[u].all) {  // what a masked slot holds must not meet its zero weight
@@ -435,7 +446,10 @@ __device__ __forceinline__ void past_keys(const wm_pool_attn_args& a, const Piec
         uint32_t va[4];
         R::value_fragment(va, vr[u], s);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) mma_16816(st.o[s][rt], va[0], va[1], va[2], va[3], pb[u][rt][0], pb[u][rt][1]);
+        for (int rt = 0; rt < RT; ++rt) {
+          mma_16816(st.o[s][rt], va[0], va[1], va[2], va[3], pb[u][rt][0], pb[u][rt][1]);
+          if (kFine) mma_16816(st.o[s][rt], va[0], va[1], va[2], va[3], rest[u][rt][0], rest[u][rt][1]);
+        }
       }
     }
     if (next >= end) break;
@@ -446,7 +460,7 @@ __device__ __forceinline__ void past_keys(const wm_pool_attn_args& a, const Piec
 }
 
 // ---------------------------------------------------------------- drafted tokens
-template <int kStorage, int DP, int RT>
+template <int kStorage, int DP, int RT, bool kFine>
 __device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Plan& plan, const Piece& c, int tile, int stop, const Queries<DP, RT>& q, State<DP, RT>& st) {
   using R = Rows<WM_BF16, DP>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -477,7 +491,7 @@ __device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Pla
     special = __any_sync(0xffffffffu, special);
     float x[1][RT][4];
     scores<WM_BF16, DP, RT, kStorage != WM_BF16>(kr, q, x[0]);
-    uint32_t pb[1][RT][2], sees[RT][2], seen[1][RT][2];
+    uint32_t pb[1][RT][2], rest[1][RT][2], sees[RT][2], seen[1][RT][2];
     const Keys keys[1] = {{{factor, factor}, {1.f, 1.f}, false}};
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -489,14 +503,17 @@ __device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Pla
         seen[0][rt][j] = (sees[rt][j] >> g & 1u) | (sees[rt][j] >> (g + 8) & 1u) << 1;
       }
     }
-    weights<DP, RT, 1, false, true>(st, x, keys, seen, pb);
+    weights<DP, RT, 1, false, true, kFine>(st, x, keys, seen, pb, rest);
     if (!special) {
 #pragma unroll
       for (int s = 0; s < DP / 16; ++s) {
         uint32_t va[4];
         R::value_fragment(va, vr, s);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) mma_16816(st.o[s][rt], va[0], va[1], va[2], va[3], pb[0][rt][0], pb[0][rt][1]);
+        for (int rt = 0; rt < RT; ++rt) {
+          mma_16816(st.o[s][rt], va[0], va[1], va[2], va[3], pb[0][rt][0], pb[0][rt][1]);
+          if (kFine) mma_16816(st.o[s][rt], va[0], va[1], va[2], va[3], rest[0][rt][0], rest[0][rt][1]);
+        }
       }
     } else {  // an infinity or NaN among the values reaches the rows that see it and no others: row by row
 #pragma unroll
@@ -581,6 +598,7 @@ __device__ __forceinline__ Piece cluster_piece(const wm_pool_attn_args& a, const
 template <int kStorage, int DP, int RT, bool kTree, Mode kMode>
 __global__ void __launch_bounds__(kThreads, resident_blocks(kStorage, RT, DP)) pool_attn_mma_kernel(const wm_pool_attn_args a, const Plan plan) {
   constexpr int kRows = RT * 8, kPitch = DP + 4;
+  constexpr bool kFine = kStorage != WM_BF16;
   __shared__ __align__(16) float sm_acc[kWarps][kRows][kPitch];
   __shared__ float sm_m[kWarps][kRows], sm_l[kWarps][kRows];
   __shared__ uint2 sm_q[Queries<DP, RT>::kShared ? RT * (DP / 16) * 32 : 1];
@@ -631,9 +649,9 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(kStorage, RT, DP)) p
     }
     if (Queries<DP, RT>::kShared) __syncthreads();
 
-    if (c.tile < c.past_tiles) past_keys<kStorage, DP, RT, kMode == kDenseShares>(a, c, c.tile, min(c.stop, c.past_tiles), q, st);
+    if (c.tile < c.past_tiles) past_keys<kStorage, DP, RT, kMode == kDenseShares, kFine>(a, c, c.tile, min(c.stop, c.past_tiles), q, st);
     if (kTree && c.stop > c.past_tiles && c.stop > c.tile)
-      draft_keys<kStorage, DP, RT>(a, plan, c, max(c.tile - c.past_tiles, 0), c.stop - c.past_tiles, q, st);
+      draft_keys<kStorage, DP, RT, kFine>(a, plan, c, max(c.tile - c.past_tiles, 0), c.stop - c.past_tiles, q, st);
 
     // join the warps: references, sums and accumulators side by side
 #pragma unroll
@@ -759,7 +777,7 @@ cudaError_t launch_mma(const wm_pool_attn_args& a, const Plan& plan, cudaStream_
     config.numAttrs = 1;
     return cudaLaunchKernelEx(&config, pool_attn_mma_kernel<kStorage, DP, RT, kTree, kCluster>, a, plan);
   }
-  if constexpr (DP % 64 == 0) {  // heads of 64 and 128, the usual pool: 115 us against 127 us on 64 sequences of up to 8192 int8 rows
+  if constexpr (DP % 64 == 0) {  // heads of 64 and 128, the usual pool: 115 us against 127 us on 64 sequences of up to 8192 int8 rows, before the weights were held in two parts
     const bool scaled = kStorage != WM_BF16;
     if (a.head_dim == DP && a.k_strides[2] == DP && a.v_strides[2] == DP && (!scaled || (a.k_scale_strides[2] == 1 && a.v_scale_strides[2] == 1))) {
       pool_attn_mma_kernel<kStorage, DP, RT, kTree, kDenseShares><<<plan.blocks, kThreads, 0, stream>>>(a, plan);
