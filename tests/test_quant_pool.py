@@ -555,3 +555,40 @@ def test_a_captured_step_notices_replaced_scales():
     pool.key_scales = pool.key_scales.clone()
     with pytest.raises(ValueError, match="capture the step again"):
         step()
+
+
+# ------------------------------------------------------------------ GPU: values of zero, codes that are no number
+
+
+def expanded(codes, scales, storage, batch):
+    """One sequence's rows as the pool of a whole batch, without copies: enough segments that a share holds a long run of keys."""
+    codes, scales = codes.to(STORAGE[storage]).cuda(), scales.cuda()
+    return codes.expand(batch, -1, -1, -1), scales.expand(batch, -1, -1)
+
+
+@pytest.mark.gpu
+@on_gpu
+@pytest.mark.parametrize("dim", [64, 128, 48])
+@pytest.mark.parametrize("tokens", [1, 9, 20, 40, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("storage", sorted(STORAGE))
+def test_keys_with_values_of_zero_stay_in_the_sum(storage, dtype, tokens, dim):
+    """One key leads 8 000 others by 11.2 (a weight of 2^-16.2 each, 0.11 together); the others' values are zeros, or so small that
+    their scale times such a weight is no normal fp32 number."""
+    batch, slots = (300, 8000) if dtype == torch.bfloat16 else (300, 2000)
+    gen = torch.Generator().manual_seed(21)
+    k, v = torch.zeros(1, 1, slots, dim), torch.zeros(1, 1, slots, dim)
+    k[..., 0], k[..., 1] = -5.5, 5.5  # exact in both storages
+    k[0, 0, 0, 0], k[0, 0, 0, 1] = 5.5, 0.0
+    v[0, 0, 0] = torch.randn(dim, generator=gen)
+    v[0, 0, 1::3] = 2.0**-98 * torch.randn(len(range(1, slots, 3)), dim, generator=gen).clamp(-2, 2)
+    (kc, ks), (vc, vs) = (oracle.quantise_rows(t, storage) for t in (k, v))
+    query = torch.zeros(1, 1, tokens, dim).to(dtype)
+    query[..., 0], query[..., 1] = 1.0, -0.04
+    (keys, key_scales), (values, value_scales) = expanded(kc, ks, storage, batch), expanded(vc, vs, storage, batch)
+    got = quantized_pool_attention(query.cuda().expand(batch, -1, -1, -1), keys, values, key_scales, value_scales, softmax_scale=1.0)
+    rows = [kc * ks[..., None].double(), vc * vs[..., None].double()]
+    out, mass, reach = oracle.attention(query[:, :, :1], *rows, None, 0, None, None, 1.0)
+    limit = oracle.bound(out, mass, reach, dtype, dim, slots)
+    worst = ((got.cpu().double() - out).abs() / limit).max().item()
+    assert worst <= 1, f"error {worst:.3g} times the bound"

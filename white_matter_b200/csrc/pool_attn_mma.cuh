@@ -221,9 +221,13 @@ struct Keys {
   bool all;
 };
 
-// The value scale of a key, as a number that has an inverse: a row of zeros has scale 0, which becomes 2^-110 (a commit writes no
-// other scale below 2^-108), a row that is not seen may have any, which becomes 1.
-__device__ __forceinline__ float usable_scale(float scale, bool seen) { return !seen ? 1.f : fabsf(scale) < 0x1p-110f ? 0x1p-110f : scale; }
+// The value scale of a key: a row that is not seen may have any, which becomes 1.
+__device__ __forceinline__ float usable_scale(float scale, bool seen) { return seen ? scale : 1.f; }
+
+// Below this scale a weight that counts in the sum may be lost in its product with the scale (products below 2^-126 are zero): such keys,
+// rows of zeros with scale 0 among them, enter the sum by the weight itself.  From it on, only weights below 2^-62 are lost.  (64
+// sequences with 32 drafted tokens over int8 rows of 64: 287 -> 294 us for looking; heads of 128: no difference.)
+constexpr float kTinyScale = 0x1p-64f;
 
 // Weights of U x 16 keys for every tile, as B operands of O^T += V^T P^T.  x holds the keys' products with the queries (keys
 // g: x[.][.][0], [1]; g + 8: [2], [3]; rows 2t, 2t + 1).  With kFine the weights come in two parts, rounded (pb) and what the
@@ -281,7 +285,16 @@ __device__ __forceinline__ void weights(State<DP, RT>& st, float (&x)[U][RT][4],
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const float inverse[2] = {kScaled && !kFine ? reciprocal_approx(keys[u].scale[0]) : 1.f, kScaled && !kFine ? reciprocal_approx(keys[u].scale[1]) : 1.f};
+    float inverse[2] = {1.f, 1.f};
+    bool tiny[2] = {false, false}, some_tiny = false;
+    if (kScaled && !kFine) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        tiny[h] = fabsf(keys[u].scale[h]) < kTinyScale;
+        inverse[h] = tiny[h] ? 0.f : reciprocal_approx(keys[u].scale[h]);
+      }
+      some_tiny = __any_sync(0xffffffffu, tiny[0] || tiny[1]);
+    }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float(&y)[4] = x[u][rt];
@@ -290,6 +303,10 @@ __device__ __forceinline__ void weights(State<DP, RT>& st, float (&x)[U][RT][4],
       if (kFine) {
         st.l[rt][0] += y[0] + y[2];
         st.l[rt][1] += y[1] + y[3];
+      }
+      if (some_tiny) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st.l[rt][e & 1] += tiny[e >> 1] ? y[e] : 0.f;
       }
       if (kScaled) {
 #pragma unroll
