@@ -12,6 +12,7 @@
  *   WM_E4M3  scale = the smallest power of two with a / scale <= 448, code = x / scale rounded to e4m3, halves to even.
  * A row with a < 2^-100 is held as zeros with scale 0; a row with an infinity or NaN gets codes 0 and scale NaN and
  * reads back as NaN throughout.
+ * In a pool that was quantised elsewhere e4m3's two NaN codes are NaN to the read back and to every query that sees them.
  */
 #ifndef WM_B200_SERVING_H
 #define WM_B200_SERVING_H

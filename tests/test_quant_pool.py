@@ -592,3 +592,50 @@ def test_keys_with_values_of_zero_stay_in_the_sum(storage, dtype, tokens, dim):
     limit = oracle.bound(out, mass, reach, dtype, dim, slots)
     worst = ((got.cpu().double() - out).abs() / limit).max().item()
     assert worst <= 1, f"error {worst:.3g} times the bound"
+
+
+@pytest.mark.gpu
+@on_gpu
+@pytest.mark.parametrize("dim", [16, 32, 48, 64, 80, 96, 128])
+@pytest.mark.parametrize("batch, slots, tokens", [(1, 300, 1), (2, 300, 5), (2, 300, 20), (2, 4400, 1), (2, 4400, 3), (2, 4400, 17), (2, 4400, 40)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_e4m3_codes_that_are_no_number(dtype, batch, slots, tokens, dim):
+    """A pool that was quantised elsewhere may hold the two NaN codes: in a visible key they reach everything of the queries that see
+    it, in a visible value their element alone, and nothing else."""
+    gen = torch.Generator().manual_seed(22)
+    heads, kv_heads = 4, 2
+    (kc, ks), (vc, vs) = (oracle.quantise_rows(torch.randn(batch, kv_heads, slots, dim, generator=gen), "e4m3") for _ in "kv")
+    query = torch.randn(batch, heads, tokens, dim, generator=gen).to(dtype)
+    mask = torch.rand(batch, slots, generator=gen) < 0.7
+    lengths = torch.tensor([slots - 3, slots // 2][:batch])
+    seen = torch.tensor([[7, slots - 9], [3, slots // 2 - 1]])
+    mask[torch.arange(2)[:batch, None], seen[:batch]] = True
+    mask[:, 5] = False
+    codes = [t.to(torch.float8_e4m3fn).view(torch.uint8) for t in (kc, vc)]
+    for which in codes:  # not seen: masked, or behind the last token
+        which[:, :, 5], which[:, :, int(lengths[0]) :] = 0x7F, 0xFF
+        for b in range(batch):
+            which[b, :, int(lengths[b]) :] = 0x7F
+    places = [(batch - 1, 1, int(seen[batch - 1, 0]), 0, 0x7F), (batch - 1, 1, int(seen[batch - 1, 1]), dim - 1, 0xFF), (batch - 1, 1, int(seen[batch - 1, 0]), dim // 2 + 1, 0xFF)]
+    clean = oracle.attention(query, kc * ks[..., None].double(), vc * vs[..., None].double(), lengths, 0, mask)
+    for kind in (0, 1):
+        spoilt = [c.clone() for c in codes]
+        want = torch.zeros(batch, tokens, heads, dim, dtype=torch.bool)
+        for b, h, slot, d, code in places[:1] if kind == 0 else places:
+            spoilt[kind][b, h, slot, d] = code
+            want[b, :, 2 * h : 2 * h + 2, slice(None) if kind == 0 else d] = True
+        got = quantized_pool_attention(
+            query.cuda(), *(s.view(torch.float8_e4m3fn).cuda() for s in spoilt), ks.cuda(), vs.cuda(), kv_lengths=lengths.cuda(), key_mask=mask.cuda(),
+        ).cpu()
+        assert torch.equal(torch.isnan(got), want), kind
+        out, mass, reach = clean
+        limit = oracle.bound(out, mass, reach, dtype, dim, slots)
+        # the element of the spoilt value counts elsewhere as the number it replaces: only columns without one are compared
+        worst = ((got.double() - out).abs() / limit)[~want].max().item()
+        assert worst <= 1, f"error {worst:.3g} times the bound"
+    # without a mask, every slot up to the last in sight
+    got = quantized_pool_attention(query.cuda(), *(s.view(torch.float8_e4m3fn).cuda() for s in spoilt), ks.cuda(), vs.cuda(), kv_lengths=torch.tensor([5] * batch).cuda())
+    want = torch.zeros(batch, tokens, heads, dim, dtype=torch.bool)
+    if batch == 2:
+        want[1, :, 2:4, 0] = want[1, :, 2:4, dim // 2 + 1] = True
+    assert torch.equal(torch.isnan(got.cpu()), want)

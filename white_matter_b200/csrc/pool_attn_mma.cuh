@@ -91,14 +91,29 @@ __device__ __forceinline__ void load_row(uint32_t* r, const char* p) {
 template <int kStorage>
 struct Codes {
   static constexpr int kBytes = kStorage == WM_BF16 ? 2 : 1;
-  // bytes 0, 2 (even) and 1, 3 (odd) of a word of codes as bf16 pairs
-  __device__ static uint32_t even(uint32_t w) {
-    if (kStorage == WM_INT8) return int8_pair(w);
-    return e4m3_pair(w << 4, w << 8);
+  // e4m3's two NaN codes come out of pairs() as +-480, which no other code is: `top`, the largest magnitude that it met, tells whether
+  // there were any.  Who finds some sees to what he made of them.  (64 sequences of up to 8192 rows of 64, one token: 123 -> 133 us.  NaN
+  // made in place, by zero times a product that overflows for 480 alone, took 142 us, a vote in every step 136 us.)
+  __device__ static bool some_nan(uint32_t top) { return kStorage == WM_E4M3 && ((top & 0xffffu) == 0x07f0u || top >> 16 == 0x07f0u); }
+  // bit 7 of every byte that is a NaN code
+  __device__ static uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+  // a pair with NaN for +-480
+  __device__ static uint32_t repaired(uint32_t pair) {
+    if ((pair & 0x7fffu) == 0x43f0u) pair |= 0x7fffu;
+    if ((pair & 0x7fff0000u) == 0x43f00000u) pair |= 0x7fff0000u;
+    return pair;
   }
-  __device__ static uint32_t odd(uint32_t w) {
-    if (kStorage == WM_INT8) return int8_pair(w >> 8);
-    return e4m3_pair(w >> 4, w);
+  // bytes 0, 2 (even) and 1, 3 (odd) of a word of codes as bf16 pairs
+  __device__ static void pairs(uint32_t w, uint32_t& even, uint32_t& odd, uint32_t& top) {
+    if (kStorage == WM_INT8) {
+      even = int8_pair(w);
+      odd = int8_pair(w >> 8);
+    } else {
+      const uint32_t e = w << 4 & 0x07f007f0u, o = w >> 4 & 0x07f007f0u;
+      top = __vimax3_u16x2(top, e, o);
+      even = e4m3_pair(e, w << 8);
+      odd = e4m3_pair(o, w);
+    }
   }
 
  private:
@@ -111,7 +126,7 @@ struct Codes {
   }
   // exponent and fraction in the places bf16 has them, which reads as 2^-120 of the number (subnormals too)
   __device__ static uint32_t e4m3_pair(uint32_t magnitude, uint32_t sign) {
-    const uint32_t x = and_or(sign, 0x80008000u, magnitude & 0x07f007f0u);
+    const uint32_t x = and_or(sign, 0x80008000u, magnitude);
     uint32_t y;
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x7b807b80u));
     return y;
@@ -145,7 +160,7 @@ struct Rows {
   // Fragment s (16 of head_dim) of K: elements 4s .. 4s + 3 of the piece.  8-bit pools take them in the order 0, 2, 1, 3,
   // which is how a word of codes comes apart; kPermute gives bf16 rows the same order.
   template <bool kPermute>
-  __device__ static void key_fragment(uint32_t (&a)[4], const uint32_t (&lo)[kKeyWords], const uint32_t (&hi)[kKeyWords], int s) {
+  __device__ static void key_fragment(uint32_t (&a)[4], const uint32_t (&lo)[kKeyWords], const uint32_t (&hi)[kKeyWords], int s, uint32_t& top) {
     if (kStorage == WM_BF16) {
       const uint32_t l0 = lo[2 * s < kKeyWords ? 2 * s : 0], l1 = lo[2 * s + 1 < kKeyWords ? 2 * s + 1 : 0];
       const uint32_t h0 = hi[2 * s < kKeyWords ? 2 * s : 0], h1 = hi[2 * s + 1 < kKeyWords ? 2 * s + 1 : 0];
@@ -154,14 +169,12 @@ struct Rows {
       a[2] = kPermute ? __byte_perm(l0, l1, 0x7632) : l1;
       a[3] = kPermute ? __byte_perm(h0, h1, 0x7632) : h1;
     } else {
-      a[0] = Codes<kStorage>::even(lo[s]);
-      a[1] = Codes<kStorage>::even(hi[s]);
-      a[2] = Codes<kStorage>::odd(lo[s]);
-      a[3] = Codes<kStorage>::odd(hi[s]);
+      Codes<kStorage>::pairs(lo[s], a[0], a[2], top);
+      Codes<kStorage>::pairs(hi[s], a[1], a[3], top);
     }
   }
   // Fragment s of V^T: elements 2s, 2s + 1 of the piece for the four keys.
-  __device__ static void value_fragment(uint32_t (&a)[4], const uint32_t (&v)[4][kValueWords], int s) {
+  __device__ static void value_fragment(uint32_t (&a)[4], const uint32_t (&v)[4][kValueWords], int s, uint32_t& top) {
     if (kStorage == WM_BF16) {
       const int w = s < kValueWords ? s : 0;
       a[0] = __byte_perm(v[0][w], v[1][w], 0x5410);
@@ -171,10 +184,8 @@ struct Rows {
     } else {
       const uint32_t pick = s & 1 ? 0x7632 : 0x5410;  // elements 2s, 2s + 1 of two keys: x0 x1 y0 y1
       const uint32_t first = __byte_perm(v[0][s / 2], v[1][s / 2], pick), second = __byte_perm(v[2][s / 2], v[3][s / 2], pick);
-      a[0] = Codes<kStorage>::even(first);
-      a[1] = Codes<kStorage>::odd(first);
-      a[2] = Codes<kStorage>::even(second);
-      a[3] = Codes<kStorage>::odd(second);
+      Codes<kStorage>::pairs(first, a[0], a[1], top);
+      Codes<kStorage>::pairs(second, a[2], a[3], top);
     }
   }
 };
@@ -198,11 +209,11 @@ struct Queries {
 
 // Products of 16 keys with the queries of every tile: S^T, keys g and g + 8 in the rows of x.
 template <int kStorage, int DP, int RT, bool kPermute>
-__device__ __forceinline__ void scores(const uint32_t (&kr)[2][Rows<kStorage, DP>::kKeyWords], const Queries<DP, RT>& q, float (&x)[RT][4]) {
+__device__ __forceinline__ void scores(const uint32_t (&kr)[2][Rows<kStorage, DP>::kKeyWords], const Queries<DP, RT>& q, float (&x)[RT][4], uint32_t& top) {
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) {
     uint32_t ka[4];
-    Rows<kStorage, DP>::template key_fragment<kPermute>(ka, kr[0], kr[1], s);
+    Rows<kStorage, DP>::template key_fragment<kPermute>(ka, kr[0], kr[1], s, top);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const uint2 b = q.get(rt, s);
@@ -339,6 +350,42 @@ __host__ __device__ constexpr int groups_per_step() {
   return DP * Codes<kStorage>::kBytes <= 64 ? 2 : 1;
 }
 
+// Called where a warp met NaN codes of e4m3 among the visible slots [begin, end), all of which every row sees: in a key they make the
+// whole row NaN, in a value their element, which is looked up in the pool once more.
+template <int DP, int RT>
+__device__ __forceinline__ uint32_t nan_elements(const wm_pool_attn_args& a, const Piece& c, int begin, int end, int w) {
+  using R = Rows<WM_E4M3, DP>;
+  const int lane = threadIdx.x & 31;
+  const uint8_t* mask = a.key_mask != nullptr ? a.key_mask + static_cast<long long>(c.b) * a.k_len : nullptr;
+  const char* v = static_cast<const char*>(a.v) + c.b * a.v_strides[0] + c.kv_head * a.v_strides[1] + R::value_piece(lane >> 2, a.head_dim) + 4 * w;
+  uint32_t codes = 0;
+#pragma unroll 1
+  for (int j = begin + (lane & 3); j < end; j += 4)
+    if (mask == nullptr || mask[j] != 0) codes |= Codes<WM_E4M3>::nan_codes(*reinterpret_cast<const uint32_t*>(v + j * a.v_strides[2]));
+  codes |= __shfl_xor_sync(0xffffffffu, codes, 1);
+  return codes | __shfl_xor_sync(0xffffffffu, codes, 2);
+}
+template <int DP, int RT>
+__device__ __forceinline__ void nan_keys(const wm_pool_attn_args& a, const Piece& c, int begin, int end, bool in_key, State<DP, RT>& st) {
+  const float nan = __uint_as_float(0x7fffffffu);
+  if (in_key) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) st.l[rt][0] = st.l[rt][1] = nan;
+  }
+#pragma unroll
+  for (int w = 0; w < Rows<WM_E4M3, DP>::kValueWords; ++w) {
+    const uint32_t codes = nan_elements<DP, RT>(a, c, begin, end, w);
+#pragma unroll
+    for (int n = 0; n < 4; ++n)  // element 4 w + n of the lane's piece
+      if (codes >> (8 * n + 7) & 1u) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) st.o[2 * w + (n >> 1)][rt][2 * (n & 1) + j] = nan;
+      }
+  }
+}
+
 // This warp's rows of the tiles [tile, stop) that lie among the visible slots.  With kDense the rows of the pool are DP
 // elements and lie one behind the other (scales too): a lane then needs one address for all of its rows of a step.
 template <int kStorage, int DP, int RT, bool kDense, bool kFine>
@@ -416,6 +463,7 @@ __device__ __forceinline__ void past_keys(const wm_pool_attn_args& a, const Piec
     }
   };
 
+  uint32_t top_key = 0, top_value = 0;
   load_k(j0);
   load_v(j0);
   for (;;) {
@@ -435,9 +483,19 @@ __device__ __forceinline__ void past_keys(const wm_pool_attn_args& a, const Piec
         keys[u].scale[h] = kScaled ? usable_scale(vscale[u][h], keys[u].all || (seen[u][0][0] >> h & 1u)) : 1.f;
       }
     }
+    if (kStorage == WM_E4M3 && word != kFull) {  // a masked slot may hold NaN codes
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (!(seen[u][0][0] >> h & 1u)) {
+#pragma unroll
+            for (int w = 0; w < R::kKeyWords; ++w) kr[u][h][w] = 0;
+          }
+    }
     float x[U][RT][4];
 #pragma unroll
-    for (int u = 0; u < U; ++u) scores<kStorage, DP, RT, false>(kr[u], q, x[u]);
+    for (int u = 0; u < U; ++u) scores<kStorage, DP, RT, false>(kr[u], q, x[u], top_key);
     if (next < end) {
       k += kStepKeys * k_row;
       if (kScaled) {
@@ -461,7 +519,7 @@ __device__ __forceinline__ void past_keys(const wm_pool_attn_args& a, const Piec
 #pragma unroll
       for (int s = 0; s < DP / 16; ++s) {
         uint32_t va[4];
-        R::value_fragment(va, vr[u], s);
+        R::value_fragment(va, vr[u], s, top_value);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
           mma_16816(st.o[s][rt], va[0], va[1], va[2], va[3], pb[u][rt][0], pb[u][rt][1]);
@@ -474,6 +532,8 @@ __device__ __forceinline__ void past_keys(const wm_pool_attn_args& a, const Piec
     load_v(next);
     j0 = next;
   }
+  if (kStorage == WM_E4M3 && __any_sync(0xffffffffu, Codes<kStorage>::some_nan(__vmaxu2(top_key, top_value))))
+    nan_keys<DP, RT>(a, c, tile * kTileKeys, end, __any_sync(0xffffffffu, Codes<kStorage>::some_nan(top_key)), st);
 }
 
 // ---------------------------------------------------------------- drafted tokens
@@ -507,7 +567,8 @@ __device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Pla
       }
     special = __any_sync(0xffffffffu, special);
     float x[1][RT][4];
-    scores<WM_BF16, DP, RT, kStorage != WM_BF16>(kr, q, x[0]);
+    uint32_t none = 0;
+    scores<WM_BF16, DP, RT, kStorage != WM_BF16>(kr, q, x[0], none);
     uint32_t pb[1][RT][2], rest[1][RT][2], sees[RT][2], seen[1][RT][2];
     const Keys keys[1] = {{{factor, factor}, {1.f, 1.f}, false}};
 #pragma unroll
@@ -525,7 +586,7 @@ __device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Pla
 #pragma unroll
       for (int s = 0; s < DP / 16; ++s) {
         uint32_t va[4];
-        R::value_fragment(va, vr, s);
+        R::value_fragment(va, vr, s, none);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
           mma_16816(st.o[s][rt], va[0], va[1], va[2], va[3], pb[0][rt][0], pb[0][rt][1]);
@@ -547,7 +608,7 @@ __device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Pla
             uint32_t va[4], one[4][R::kValueWords];
 #pragma unroll
             for (int h = 0; h < 4; ++h) one[h][s] = vr[h][s] & keep[h];
-            R::value_fragment(va, one, s);
+            R::value_fragment(va, one, s, none);
             float x[4] = {0.f, 0.f, 0.f, 0.f};
             mma_16816(x, va[0], va[1], va[2], va[3], b0, b1);
             // the other columns hold 0 * infinity: only this row's is taken

@@ -80,6 +80,11 @@ __device__ __forceinline__ void cp_async_wait() {
 __device__ __forceinline__ void st_shared_16(uint32_t dst, const uint4& x) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
 }
+__device__ __forceinline__ uint4 ld_shared_16(uint32_t src) {
+  uint4 x;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(src) : "memory");
+  return x;
+}
 __device__ __forceinline__ uint4 load_16(const char* p) {
   uint4 x;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(p));
@@ -170,13 +175,32 @@ struct Stager {
     const int row0 = threadIdx.x / C::kChunks, part = threadIdx.x % C::kChunks;
     const uint32_t to = ptx::smem_u32(sm.tile[i % C::kStages][0]);
     const uint32_t first = to + RowLayout<DP>::piece(row0, 2 * part), second = to + RowLayout<DP>::piece(row0, 2 * part + 1);
+    uint32_t top = 0;
 #pragma unroll
     for (int n = 0; n < 2 * C::kPasses; ++n) {
       const uint4 x = sm.raw[kStorage == WM_BF16 ? 0 : n][kStorage == WM_BF16 ? 0 : threadIdx.x];
       const int at = n % C::kPasses * C::kPassRows * C::kRowBytes + n / C::kPasses * C::kTileBytes;
-      st_shared_16(first + at, make_uint4(Codes<kStorage>::even(x.x), Codes<kStorage>::odd(x.x), Codes<kStorage>::even(x.y), Codes<kStorage>::odd(x.y)));
-      st_shared_16(second + at, make_uint4(Codes<kStorage>::even(x.z), Codes<kStorage>::odd(x.z), Codes<kStorage>::even(x.w), Codes<kStorage>::odd(x.w)));
+      uint32_t y[8];
+      Codes<kStorage>::pairs(x.x, y[0], y[1], top);
+      Codes<kStorage>::pairs(x.y, y[2], y[3], top);
+      Codes<kStorage>::pairs(x.z, y[4], y[5], top);
+      Codes<kStorage>::pairs(x.w, y[6], y[7], top);
+      st_shared_16(first + at, make_uint4(y[0], y[1], y[2], y[3]));
+      st_shared_16(second + at, make_uint4(y[4], y[5], y[6], y[7]));
     }
+    if (Codes<kStorage>::some_nan(top)) {  // all rows of a block see the same slots, so a NaN may go through the products
+#pragma unroll 1
+      for (int n = 0; n < 2 * C::kPasses; ++n) {
+        const int at = n % C::kPasses * C::kPassRows * C::kRowBytes + n / C::kPasses * C::kTileBytes;
+        repair(first + at);
+        repair(second + at);
+      }
+    }
+  }
+  __device__ static void repair(uint32_t at) {
+    uint4 y = ld_shared_16(at);
+    y = make_uint4(Codes<kStorage>::repaired(y.x), Codes<kStorage>::repaired(y.y), Codes<kStorage>::repaired(y.z), Codes<kStorage>::repaired(y.w));
+    st_shared_16(at, y);
   }
 
   // A step of drafted tokens from node n0 on, by plain loads, eight in flight per thread.  Values that are not finite become

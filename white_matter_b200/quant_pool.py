@@ -10,7 +10,8 @@ With ``a`` the row's largest magnitude:
   ``x / scale`` rounded to e4m3, halves to even.  An element is off by at most 2^-4 of itself, or 2^-10 of the scale.
 
 A row whose largest magnitude is below 2^-100 is held as zeros with scale 0.  A row with an infinity or NaN gets scale
-NaN: it reads back as NaN throughout, and a query that sees it returns NaN.  The upstream project keeps its pool in
+NaN: it reads back as NaN throughout, and a query that sees it returns NaN.  A pool that was quantised elsewhere may hold
+e4m3's NaN codes: a query that sees one among the keys returns NaN, one among the values makes its element NaN.  The upstream project keeps its pool in
 bf16 (models/cache.py:43-60); these operators have no counterpart there.  All of them are for inference.
 """
 
