@@ -33,7 +33,7 @@ extern "C" {
  * indices outside the source are skipped: such a slot keeps what it held.  Pool tensors are (batch, heads, slots,
  * head_dim), scales (batch, heads, slots), sources (batch, heads, source_rows, head_dim), with element strides for
  * (batch, head, token).  head_dim is a multiple of 16 up to 128; pool rows and source rows are 16-byte aligned.
- * The pool must not overlap the source. */
+ * The pool must not overlap the source.  More than 2^31 - 65536 sequences are refused. */
 typedef struct wm_pool_commit_args {
   void* keys;
   void* values;
@@ -59,7 +59,8 @@ typedef struct wm_pool_commit_args {
 
 /* The rows an 8-bit pool stands for: out = code * scale in `dtype`; rows at or behind lengths[b] + lead are written as
  * zeros and not read (lengths NULL: every row is live).  codes (batch, heads, slots, head_dim), scales (batch, heads,
- * slots), out like codes, element strides for (batch, head, token), 16-byte aligned rows. */
+ * slots), out like codes, element strides for (batch, head, token), 16-byte aligned rows.  More than 2^31 - 65536 (sequence,
+ * head) pairs are refused. */
 typedef struct wm_pool_dequant_args {
   const void* codes;
   const float* scales;

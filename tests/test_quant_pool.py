@@ -142,6 +142,25 @@ def test_commit_refusals(change, status, text):
     assert text in lib.wm_last_error()
 
 
+@pytest.mark.parametrize("many", [2**31 - 1, 2**31 - 65535])
+def test_more_sequences_than_32_bits_count_a_grid_at_a_time_are_refused(many):
+    commit = _native.PoolCommitArgs()
+    for name in ("keys", "values", "key_scales", "value_scales", "new_keys", "new_values", "lengths"):
+        setattr(commit, name, 1 << 20)
+    for name in ("key_strides", "value_strides", "new_key_strides", "new_value_strides"):
+        setattr(commit, name, _native._Strides(4096, 1024, 64))
+    commit.storage, commit.dtype = _native.WM_INT8, _native.WM_BF16
+    commit.batch, commit.heads, commit.slots, commit.rows, commit.source_rows, commit.head_dim = many, 1, 8, 2, 2, 64
+    lib = _native.load_library()
+    assert lib.wm_pool_commit(ctypes.byref(commit), None) == -2 and b"too many sequences" in lib.wm_last_error()
+    back = _native.PoolDequantArgs()
+    for name in ("codes", "scales", "out"):
+        setattr(back, name, 1 << 20)
+    back.code_strides = back.out_strides = _native._Strides(4096, 1024, 64)
+    back.storage, back.dtype, back.batch, back.heads, back.slots, back.head_dim = _native.WM_INT8, _native.WM_BF16, many, 1, 8, 64
+    assert lib.wm_pool_dequant(ctypes.byref(back), None) == -2 and b"planes" in lib.wm_last_error()
+
+
 def test_python_refusals():
     codes, rows = torch.zeros(1, 2, 8, 64, dtype=torch.int8), torch.zeros(1, 2, 1, 64)
     scales, lengths = torch.zeros(1, 2, 8), torch.zeros(1, dtype=torch.int32)

@@ -7,6 +7,8 @@ namespace wm {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMaxGridY = 65535;
+constexpr int kMaxPlanes = INT_MAX - kMaxGridY;  // sequences of a commit, (sequence, head) planes of a read back: counted in 32 bits, a grid at a time
 
 // ---------------------------------------------------------------- commit
 // 16 bytes of a source row: its values in fp32, and the bits of the largest magnitude as fp32 bits (as integers these order
@@ -169,7 +171,7 @@ int commit_storage(const wm_pool_commit_args& a, cudaStream_t stream) {
   const bool tokens = a.rows >= kRows && a.new_key_strides[1] < a.new_key_strides[2];
   const long long rows = static_cast<long long>(a.heads) * (tokens ? (a.rows + kRows - 1) / kRows * kRows : a.rows);
   const long long per_block = kRows * kThreads / LPR;
-  const dim3 grid(static_cast<unsigned>((rows + per_block - 1) / per_block), static_cast<unsigned>(a.batch < 65535 ? a.batch : 65535), 2);
+  const dim3 grid(static_cast<unsigned>((rows + per_block - 1) / per_block), static_cast<unsigned>(a.batch < kMaxGridY ? a.batch : kMaxGridY), 2);
   if (tokens)
     pool_commit_kernel<T, LPR, kStorage, true><<<grid, kThreads, 0, stream>>>(a);
   else
@@ -322,6 +324,7 @@ int pool_commit_launch(const wm_pool_commit_args& a, cudaStream_t stream) {
   if (a.index == nullptr && a.source_rows < a.rows) return fail(WM_EINVAL, "%s: more rows than the source has", who);
   if (a.lead != 0 && a.lead != 1) return fail(WM_EINVAL, "%s: lead must be 0 or 1", who);
   if (a.head_dim % 16 || a.head_dim > 128) return fail(WM_EUNSUPPORTED, "%s: head_dim must be a multiple of 16 up to 128", who);
+  if (a.batch > kMaxPlanes) return fail(WM_EUNSUPPORTED, "%s: too many sequences", who);
   if (static_cast<long long>(a.heads) * a.rows > INT_MAX - kRows * kThreads) return fail(WM_EUNSUPPORTED, "%s: too many rows per sequence", who);
   const int wide = a.dtype == WM_F32 ? 4 : 2, held = quantised ? 1 : wide;
   if (!aligned16(a.keys) || !aligned16(a.values) || !aligned16(a.new_keys) || !aligned16(a.new_values) || !aligned16(a.key_strides, held) ||
@@ -339,13 +342,13 @@ int pool_dequant_launch(const wm_pool_dequant_args& a, cudaStream_t stream) {
   if (a.lead != 0 && a.lead != 1) return fail(WM_EINVAL, "%s: lead must be 0 or 1", who);
   if (a.head_dim % 16 || a.head_dim > 128) return fail(WM_EUNSUPPORTED, "%s: head_dim must be a multiple of 16 up to 128", who);
   const long long planes = static_cast<long long>(a.batch) * a.heads;
-  if (planes > INT_MAX) return fail(WM_EUNSUPPORTED, "%s: too many (sequence, head) planes", who);
+  if (planes > kMaxPlanes) return fail(WM_EUNSUPPORTED, "%s: too many (sequence, head) planes", who);
   if (a.slots > kMaxSlots) return fail(WM_EUNSUPPORTED, "%s: too many slots", who);
   const int wide = a.dtype == WM_F32 ? 4 : 2;
   if (!aligned16(a.codes) || !aligned16(a.out) || !aligned16(a.code_strides, 1) || !aligned16(a.out_strides, wide))
     return fail(WM_EUNSUPPORTED, "%s: rows must be 16-byte aligned", who);
   const int per_block = kUnits * (kThreads / (a.head_dim / 16));
-  const dim3 grid(static_cast<unsigned>((static_cast<long long>(a.slots) + per_block - 1) / per_block), static_cast<unsigned>(planes < 65535 ? planes : 65535));
+  const dim3 grid(static_cast<unsigned>((static_cast<long long>(a.slots) + per_block - 1) / per_block), static_cast<unsigned>(planes < kMaxGridY ? planes : kMaxGridY));
   if (a.dtype == WM_F32)
     pool_dequant_kernel<float><<<grid, kThreads, 0, stream>>>(a);
   else
