@@ -658,3 +658,25 @@ def test_e4m3_codes_that_are_no_number(dtype, batch, slots, tokens, dim):
     if batch == 2:
         want[1, :, 2:4, 0] = want[1, :, 2:4, dim // 2 + 1] = True
     assert torch.equal(torch.isnan(got.cpu()), want)
+
+
+@pytest.mark.gpu
+@on_gpu
+@pytest.mark.parametrize("kind", ["plain", "int8"])
+def test_lengths_stop_at_the_first_index_outside_the_new_rows(kind):
+    """A padded branch: slots that the commit skipped must not come into sight."""
+    make = lambda: KVPoolCache(5, 1, 2, 12, 64) if kind == "plain" else QuantKVPoolCache(5, 1, 2, 12, 64)
+    rows = torch.randn(5, 2, 4, 64, device="cuda").bfloat16()
+    index = torch.tensor([[0, 2, -1, -1], [3, 4, 0, 1], [-1, -1, -1, -1], [0, 1, 2, 3], [2, 2, 1, 9]], device="cuda")
+    for counts, want in ((None, [2, 1, 0, 4, 3]), ([1, 4, 2, 3, -7], [1, 1, 0, 3, 0])):
+        for index_dtype in (torch.int64, torch.int32):
+            pool = make()
+            start = torch.tensor([0, 3, 5, 10, 12], dtype=torch.int32)
+            pool.lengths.copy_(start)
+            pool.append(rows, rows, index=index.to(index_dtype), counts=None if counts is None else torch.tensor(counts, device="cuda"))
+            assert pool.lengths.tolist() == [min(12, int(s) + n) for s, n in zip(start, want)]
+    pool = make()
+    pool.append(rows[:, :, :0], rows[:, :, :0], index=index)
+    assert not pool.lengths.any()
+    pool.append(rows, rows, index=index[:, :0])
+    assert not pool.lengths.any()

@@ -76,14 +76,15 @@ class KVPoolCache:
         Device-side: the write positions come from ``lengths`` on the GPU, so the call can be captured in a CUDA
         graph and replayed while the lengths grow.  Rows that would not fit the capacity are dropped.  ``index`` (B,m)
         commits rows ``index[b, i]`` of the new ones instead, ``counts`` (B,) only the first ``counts[b]``: the
-        accepted branch of a draft (D a multiple of 16 up to 128).  The new rows must not be views of this pool.
+        accepted branch of a draft (D a multiple of 16 up to 128).  An index outside the new rows (-1, to pad a branch)
+        commits nothing, and the length ends before the first of them.  The new rows must not be views of this pool.
         """
         if index is not None or counts is not None:
             if key.dtype != self.keys.dtype:
                 raise ValueError("new rows must have the pool's dtype and device")
             rows = pool_commit(self.keys, self.values, None, None, self.lengths, key, value, int(self.use_dummy_token), index, counts)
             if advance:
-                _advance(self, rows, counts)
+                _advance(self, rows, index, counts, key.shape[2])
             return
         if key.shape != value.shape or key.ndim != 4 or key.shape[:2] != self.keys.shape[:2] or key.shape[3] != self.keys.shape[3]:
             raise ValueError("new rows must be (B, channels*kv_heads, n, D) for both K and V")
@@ -143,8 +144,16 @@ class KVPoolCache:
         )
 
 
-def _advance(cache, rows: int, counts: torch.Tensor | None) -> None:
-    cache.lengths.add_(rows if counts is None else counts.clamp(0, rows)).clamp_(max=cache.capacity)
+def _advance(cache, rows: int, index: torch.Tensor | None, counts: torch.Tensor | None, source_rows: int) -> None:
+    """Lengths over the rows that a commit wrote, on the device: up to the first index outside the new rows, whose slot kept what it held."""
+    if not (rows and source_rows):
+        return
+    if counts is not None:
+        counts = counts.clamp(0, rows)
+    if index is not None:
+        written = (index.clamp(0, source_rows - 1) == index).cumprod(1).sum(1)
+        counts = written if counts is None else torch.minimum(counts, written)
+    cache.lengths.add_(rows if counts is None else counts).clamp_(max=cache.capacity)
 
 
 class QuantKVPoolCache:
@@ -210,7 +219,7 @@ class QuantKVPoolCache:
             self.keys, self.values, self.key_scales, self.value_scales, self.lengths, key, value, int(self.use_dummy_token), index, counts
         )
         if advance:
-            _advance(self, rows, counts)
+            _advance(self, rows, index, counts, key.shape[2])
 
     def read(
         self,
