@@ -680,3 +680,25 @@ def test_lengths_stop_at_the_first_index_outside_the_new_rows(kind):
     assert not pool.lengths.any()
     pool.append(rows, rows, index=index[:, :0])
     assert not pool.lengths.any()
+
+
+@pytest.mark.gpu
+@on_gpu
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as forward_ad
+
+    pool = QuantKVPoolCache(1, 1, 2, 16, 64)
+    rows = torch.randn(1, 2, 3, 64, device="cuda").bfloat16()
+    pool.append(rows, rows)
+    query = torch.randn(1, 2, 1, 64, device="cuda").bfloat16()
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(query, torch.ones_like(query))
+        for mode in (torch.no_grad, torch.enable_grad):
+            with mode(), pytest.raises(ValueError, match="derivatives"):
+                pool.read(dual, 0)
+        dual_rows = forward_ad.make_dual(rows, torch.ones_like(rows))
+        with pytest.raises(ValueError, match="derivatives"):
+            pool.append(dual_rows, rows)
+        with pytest.raises(ValueError, match="derivatives"):
+            dequantize_kv_rows(pool.keys, forward_ad.make_dual(pool.key_scales, torch.ones_like(pool.key_scales)))
+        pool.read(query, 0)  # nothing in it has a tangent

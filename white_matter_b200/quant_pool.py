@@ -20,6 +20,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 
@@ -31,6 +32,9 @@ _ROWS = (torch.bfloat16, torch.float32)
 def _refuse_grad(what: str, *tensors: torch.Tensor | None) -> None:
     if torch.is_grad_enabled() and True in [t is not None and t.requires_grad for t in tensors]:
         raise ValueError(f"{what} has no gradients: call it under torch.no_grad()")
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # inside a dual level: tangents are not switched off by torch.no_grad()
+        if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise ValueError(f"{what} has no forward-mode derivatives: unpack the dual tensors first")
 
 
 def _int_vector(name: str, t: torch.Tensor, batch: int, index: int) -> torch.Tensor:
