@@ -131,6 +131,11 @@ typedef struct wm_pool_attn_args {
 WM_API size_t wm_pool_attn_workspace_bytes(const wm_pool_attn_args* args);
 
 WM_API int wm_pool_commit(const wm_pool_commit_args* args, void* stream);
+
+/* The lengths behind a commit, in place: lengths[b] grows by the rows that were written, to `capacity` at most.  Those are rows, with
+ * counts counts[b] of them at most, with index (batch, rows) those before the first index outside the source's source_rows. */
+WM_API int wm_pool_advance(void* lengths, int32_t lengths_is64, const int32_t* index, const int32_t* counts, int32_t batch,
+                           int32_t rows, int32_t source_rows, int32_t capacity, void* stream);
 WM_API int wm_pool_dequant(const wm_pool_dequant_args* args, void* stream);
 WM_API int wm_draft_tree(const wm_draft_tree_args* args, void* stream);
 WM_API int wm_pool_attn(const wm_pool_attn_args* args, void* stream);

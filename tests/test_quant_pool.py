@@ -161,6 +161,13 @@ def test_more_sequences_than_32_bits_count_a_grid_at_a_time_are_refused(many):
     assert lib.wm_pool_dequant(ctypes.byref(back), None) == -2 and b"planes" in lib.wm_last_error()
 
 
+@pytest.mark.parametrize("change, status", [(dict(lengths=None), -1), (dict(batch=0), -1), (dict(rows=0), -1), (dict(source=0), -1), (dict(capacity=0), -1), (dict(rows=2**31 - 1), -2)])
+def test_advance_refusals(change, status):
+    a = dict(lengths=1 << 20, batch=1, rows=4, source=4, capacity=9)
+    a.update(change)
+    assert _native.load_library().wm_pool_advance(a["lengths"], 0, None, None, a["batch"], a["rows"], a["source"], a["capacity"], None) == status
+
+
 def test_python_refusals():
     codes, rows = torch.zeros(1, 2, 8, 64, dtype=torch.int8), torch.zeros(1, 2, 1, 64)
     scales, lengths = torch.zeros(1, 2, 8), torch.zeros(1, dtype=torch.int32)
@@ -702,3 +709,27 @@ def test_forward_mode_tangents_are_refused():
         with pytest.raises(ValueError, match="derivatives"):
             dequantize_kv_rows(pool.keys, forward_ad.make_dual(pool.key_scales, torch.ones_like(pool.key_scales)))
         pool.read(query, 0)  # nothing in it has a tangent
+
+
+@pytest.mark.gpu
+@on_gpu
+@pytest.mark.parametrize("rows", [1, 31, 32, 33, 100])
+def test_long_branches_and_strided_lengths_advance_alike(rows):
+    gen = torch.Generator().manual_seed(rows)
+    batch, capacity = 70, 90
+    index = torch.randint(0, rows + 1, (batch, rows), generator=gen)  # `rows` is the first number outside
+    index[:10] = index[:10].clamp(max=rows - 1)
+    counts = torch.randint(-2, rows + 3, (batch,), generator=gen)
+    new = torch.randn(batch, 1, rows, 64, device="cuda").bfloat16()
+    for dtype in (torch.int32, torch.int64):
+        pool = QuantKVPoolCache(batch, 1, 1, capacity, 64)
+        start = torch.randint(0, capacity, (batch,), generator=gen)
+        pool.lengths = torch.stack((start, start), 1).to(dtype).cuda()[:, 0]  # stride 2
+        pool.append(new, new, index=index.cuda(), counts=counts.cuda())
+        want = []
+        for b in range(batch):
+            n = 0
+            while n < min(rows, int(counts[b])) and index[b, n] < rows:
+                n += 1
+            want.append(min(capacity, int(start[b]) + n))
+        assert pool.lengths.tolist() == want

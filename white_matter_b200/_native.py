@@ -413,6 +413,8 @@ def load_library() -> ctypes.CDLL:
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]  # a structure by reference, or its packed record
             fn.restype = ctypes.c_int
+        lib.wm_pool_advance.argtypes = [ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, *[ctypes.c_int32] * 4, ctypes.c_void_p]
+        lib.wm_pool_advance.restype = ctypes.c_int
         lib.wm_pool_attn_workspace_bytes.argtypes = [ctypes.c_void_p]
         lib.wm_pool_attn_workspace_bytes.restype = ctypes.c_size_t
         lib.wm_mix_workspace_bytes.argtypes = [ctypes.POINTER(MixArgs)]
@@ -463,14 +465,14 @@ pack_draft_tree = _packer(DraftTreeArgs)
 pack_pool_attn = _packer(PoolAttnArgs)
 
 
-def call_record(name: str, record: bytes, index: int) -> None:
-    """``call`` for a packed record and the index of the tensors' device."""
+def call_record(name: str, index: int, *record) -> None:
+    """``call`` for a packed record (or plain arguments) and the index of the tensors' device."""
     lib = _library or load_library()
     if index == torch.cuda.current_device():
-        status = getattr(lib, name)(record, current_stream_of(index))
+        status = getattr(lib, name)(*record, current_stream_of(index))
     else:
         with torch.cuda.device(index):
-            status = getattr(lib, name)(record, current_stream_of(index))
+            status = getattr(lib, name)(*record, current_stream_of(index))
     if status != 0:
         message = lib.wm_last_error().decode(errors="replace")
         raise RuntimeError(f"{name} failed ({status}): {message}")

@@ -193,6 +193,28 @@ int commit_rows(const wm_pool_commit_args& a, cudaStream_t stream) {
   return lanes <= 8 ? commit<__nv_bfloat16, 8>(a, stream) : commit<__nv_bfloat16, 16>(a, stream);
 }
 
+// The lengths behind a commit, a warp per sequence: a launch and two dependent loads, 2 us.
+__global__ void __launch_bounds__(kThreads) pool_advance_kernel(void* lengths, int lengths_is64, const int32_t* index, const int32_t* counts, int batch, int rows,
+                                                                int source_rows, int capacity) {
+  const int lane = threadIdx.x & 31;
+  const long long b = static_cast<long long>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  if (b >= batch) return;
+  int written = counts != nullptr ? min(max(counts[b], 0), rows) : rows;
+  if (index != nullptr) {
+    for (int base = 0; base < written; base += 32) {
+      const int i = base + lane, from = i < written ? index[b * rows + i] : 0;
+      const uint32_t outside = __ballot_sync(0xffffffffu, from < 0 || from >= source_rows);
+      if (outside != 0) written = min(written, base + __ffs(outside) - 1);
+    }
+  }
+  if (lane != 0) return;
+  const long long before = load_index(lengths, lengths_is64, static_cast<int>(b)), after = min(before + written, static_cast<long long>(capacity));
+  if (lengths_is64)
+    static_cast<long long*>(lengths)[b] = after;
+  else
+    static_cast<int*>(lengths)[b] = static_cast<int>(after);
+}
+
 // ---------------------------------------------------------------- read back
 // Bound by HBM, two thirds of it writes.  A plane is one (b, head).  A thread turns 16 codes of kUnits rows, all in flight
 // together; the threads of a block that do not fill a row are idle.  A pool of 16 x 128 heads x 2049 rows of 64, e4m3 to bf16
@@ -333,6 +355,17 @@ int pool_commit_launch(const wm_pool_commit_args& a, cudaStream_t stream) {
   return commit_rows(a, stream);
 }
 
+int pool_advance_launch(void* lengths, int lengths_is64, const int32_t* index, const int32_t* counts, int batch, int rows, int source_rows, int capacity, cudaStream_t stream) {
+  const char* who = "wm_pool_advance";
+  if (lengths == nullptr) return fail(WM_EINVAL, "%s: lengths are required", who);
+  if (batch < 1 || rows < 1 || source_rows < 1 || capacity < 1) return fail(WM_EINVAL, "%s: sizes must be positive", who);
+  if (rows > INT_MAX - 32) return fail(WM_EUNSUPPORTED, "%s: too many rows per sequence", who);
+  pool_advance_kernel<<<static_cast<unsigned>((static_cast<long long>(batch) + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, stream>>>(
+      lengths, lengths_is64, index, counts, batch, rows, source_rows, capacity);
+  count_launch();
+  return cuda_check(cudaGetLastError(), "pool_advance_kernel");
+}
+
 int pool_dequant_launch(const wm_pool_dequant_args& a, cudaStream_t stream) {
   const char* who = "wm_pool_dequant";
   if (a.codes == nullptr || a.scales == nullptr || a.out == nullptr) return fail(WM_EINVAL, "%s: codes, scales and out are required", who);
@@ -377,6 +410,11 @@ extern "C" {
 int wm_pool_commit(const wm_pool_commit_args* a, void* stream) {
   if (a == nullptr) return wm::fail(WM_EINVAL, "wm_pool_commit: null arguments");
   return wm::pool_commit_launch(*a, static_cast<cudaStream_t>(stream));
+}
+
+int wm_pool_advance(void* lengths, int32_t lengths_is64, const int32_t* index, const int32_t* counts, int32_t batch, int32_t rows, int32_t source_rows,
+                    int32_t capacity, void* stream) {
+  return wm::pool_advance_launch(lengths, lengths_is64, index, counts, batch, rows, source_rows, capacity, static_cast<cudaStream_t>(stream));
 }
 
 int wm_pool_dequant(const wm_pool_dequant_args* a, void* stream) {

@@ -11,6 +11,7 @@ constexpr int kMaxTreeNodes = 512;      // drafted tokens per tree
 constexpr int kMaxSlots = 0x7fffff00;  // of a pool: the kernels step a few rows past the last one in 32 bits
 
 int pool_commit_launch(const wm_pool_commit_args& a, cudaStream_t stream);
+int pool_advance_launch(void* lengths, int lengths_is64, const int32_t* index, const int32_t* counts, int batch, int rows, int source_rows, int capacity, cudaStream_t stream);
 int pool_dequant_launch(const wm_pool_dequant_args& a, cudaStream_t stream);
 int draft_tree_launch(const wm_draft_tree_args& a, cudaStream_t stream);
 int pool_attn_launch(const wm_pool_attn_args& a, cudaStream_t stream);

@@ -82,9 +82,10 @@ class KVPoolCache:
         if index is not None or counts is not None:
             if key.dtype != self.keys.dtype:
                 raise ValueError("new rows must have the pool's dtype and device")
-            rows = pool_commit(self.keys, self.values, None, None, self.lengths, key, value, int(self.use_dummy_token), index, counts)
-            if advance:
-                _advance(self, rows, index, counts, key.shape[2])
+            pool_commit(
+                self.keys, self.values, None, None, self.lengths, key, value, int(self.use_dummy_token), index, counts,
+                advance_to=self.capacity if advance else None,
+            )
             return
         if key.shape != value.shape or key.ndim != 4 or key.shape[:2] != self.keys.shape[:2] or key.shape[3] != self.keys.shape[3]:
             raise ValueError("new rows must be (B, channels*kv_heads, n, D) for both K and V")
@@ -142,18 +143,6 @@ class KVPoolCache:
             query, key, value, draft_key, draft_value, tree, kv_lengths=self.lengths, use_dummy_token=self.use_dummy_token,
             key_mask=key_mask, softmax_scale=softmax_scale,
         )
-
-
-def _advance(cache, rows: int, index: torch.Tensor | None, counts: torch.Tensor | None, source_rows: int) -> None:
-    """Lengths over the rows that a commit wrote, on the device: up to the first index outside the new rows, whose slot kept what it held."""
-    if not (rows and source_rows):
-        return
-    if counts is not None:
-        counts = counts.clamp(0, rows)
-    if index is not None:
-        written = (index.clamp(0, source_rows - 1) == index).cumprod(1).sum(1)
-        counts = written if counts is None else torch.minimum(counts, written)
-    cache.lengths.add_(rows if counts is None else counts).clamp_(max=cache.capacity)
 
 
 class QuantKVPoolCache:
@@ -215,11 +204,10 @@ class QuantKVPoolCache:
     ) -> None:
         """Quantise ``(B, channels*kv_heads, n, D)`` new rows (bf16 or fp32) behind each sequence's committed tokens;
         ``index`` and ``counts`` as in ``KVPoolCache.append``."""
-        rows = pool_commit(
-            self.keys, self.values, self.key_scales, self.value_scales, self.lengths, key, value, int(self.use_dummy_token), index, counts
+        pool_commit(
+            self.keys, self.values, self.key_scales, self.value_scales, self.lengths, key, value, int(self.use_dummy_token), index, counts,
+            advance_to=self.capacity if advance else None,
         )
-        if advance:
-            _advance(self, rows, index, counts, key.shape[2])
 
     def read(
         self,

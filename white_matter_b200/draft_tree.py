@@ -58,7 +58,7 @@ def prepare_draft_tree(parents: torch.Tensor, *, include_self: bool = False) -> 
     depths = torch.empty_like(parents)
     if batch and tokens:
         record = _native.pack_draft_tree(parents.data_ptr(), ancestors.data_ptr(), depths.data_ptr(), batch, tokens, include_self)
-        _native.call_record("wm_draft_tree", record, parents.get_device())
+        _native.call_record("wm_draft_tree", parents.get_device(), record)
     return DraftTree(ancestors, depths)
 
 

@@ -86,9 +86,10 @@ def _check_pool(keys: torch.Tensor, values: torch.Tensor, key_scales, value_scal
 
 def pool_commit(
     keys: torch.Tensor, values: torch.Tensor, key_scales, value_scales, lengths: torch.Tensor, new_keys: torch.Tensor,
-    new_values: torch.Tensor, lead: int, index: torch.Tensor | None, counts: torch.Tensor | None,
-) -> int:
-    """Checks and the launch behind every commit that quantises or picks rows; returns how many rows a sequence can get."""
+    new_values: torch.Tensor, lead: int, index: torch.Tensor | None, counts: torch.Tensor | None, *, advance_to: int | None = None,
+) -> None:
+    """Checks and the launch behind every commit that quantises or picks rows.  With ``advance_to``, a capacity, the lengths then move
+    over the rows that were written: with an index, those before the first one outside the new rows."""
     (batch, heads, slots, dim), device, quantised, storage, k_strides, v_strides, ks_strides, vs_strides, ks, vs = _check_pool(
         keys, values, key_scales, value_scales
     )
@@ -102,7 +103,7 @@ def pool_commit(
     if new_keys.get_device() != device or new_values.get_device() != device:
         raise ValueError("new rows must be on the pool's device")
     _refuse_grad("a pool commit", keys, values, key_scales, value_scales, new_keys, new_values)
-    lengths = _int_vector("lengths", lengths, batch, device)
+    held, lengths = lengths, _int_vector("lengths", lengths, batch, device)
     rows = source_rows = shape[2]
     if index is not None:
         if index.ndim != 2 or index.shape[0] != batch or index.dtype not in (torch.int32, torch.int64) or index.get_device() != device:
@@ -116,18 +117,21 @@ def pool_commit(
         if counts.dtype != torch.int32:
             counts = counts.clamp(0, rows).to(torch.int32)
     if not (batch and heads and slots and dim and rows and source_rows):
-        return rows
+        return
     new_keys, nk, nk_strides = _aligned(new_keys)
     new_values, nv, nv_strides = _aligned(new_values)
+    at, at_index, at_counts = lengths.data_ptr(), 0 if index is None else index.data_ptr(), 0 if counts is None else counts.data_ptr()
     record = _native.pack_pool_commit(
-        keys.data_ptr(), values.data_ptr(), ks, vs, nk, nv, lengths.data_ptr(), 0 if index is None else index.data_ptr(),
-        0 if counts is None else counts.data_ptr(),
+        keys.data_ptr(), values.data_ptr(), ks, vs, nk, nv, at, at_index, at_counts,
         *k_strides, *v_strides, *ks_strides, *vs_strides, *nk_strides, *nv_strides,
         storage, _native.WM_F32 if dtype == torch.float32 else _native.WM_BF16, batch, heads, slots, rows, source_rows, dim, lead,
         lengths.dtype == torch.int64,
     )
-    _native.call_record("wm_pool_commit", record, device)
-    return rows
+    _native.call_record("wm_pool_commit", device, record)
+    if advance_to is not None:
+        _native.call_record("wm_pool_advance", device, at, lengths.dtype == torch.int64, at_index, at_counts, batch, rows, source_rows, advance_to)
+        if held is not lengths:
+            held.copy_(lengths)
 
 
 def quantized_pool_append(
@@ -191,7 +195,7 @@ def dequantize_kv_rows(
         storage, _native.WM_F32 if dtype == torch.float32 else _native.WM_BF16, batch, heads, slots, dim, int(use_dummy_token),
         lengths is not None and lengths.dtype == torch.int64,
     )
-    _native.call_record("wm_pool_dequant", record, device)
+    _native.call_record("wm_pool_dequant", device, record)
     return out
 
 
@@ -261,7 +265,7 @@ def pool_attention(
         code, storage, batch, heads, kv_heads, length, slots, dim, lead, lengths64, shared,
         dim**-0.5 if softmax_scale is None else float(softmax_scale),
     )
-    _native.call_record("wm_pool_attn", record, device)
+    _native.call_record("wm_pool_attn", device, record)
     return out
 
 
