@@ -286,3 +286,31 @@ def test_draft_verify_commit_loop_replayed_from_a_graph(storage):
                     codes, scales = oracle.quantise_rows(picked, storage)
                     assert torch.equal(now[b, :, at : at + n], codes * scales[..., None])
         check_attention(got[channels * size :].view(batch, 1, heads, dim), queries[0, :, :, :1].cpu(), [r[:, :kv_heads] for r in after], cache.lengths.cpu(), 1, None)
+
+
+@pytest.mark.gpu
+@on_gpu
+@pytest.mark.parametrize("storage", sorted(STORAGE))
+def test_an_infinite_drafted_value_takes_no_bits_from_the_rows_that_do_not_see_it(storage):
+    """Up to 16 rows over an 8-bit pool take the weights in two bf16 parts, 16 bits: also next to a drafted value that is infinite and
+    that they do not see.  Values of alternating sign cancel, so the weights' error shows beside a small result: two parts leave
+    2^-16 of the mass, one part 2^-9 (both twice, for the sum that divides them)."""
+    tokens, dim = 12, 64
+    gen = torch.Generator().manual_seed(44)
+    query = torch.randn(1, 1, tokens, dim, generator=gen).bfloat16()
+    (kc, ks), (vc, vs) = (oracle.quantise_rows(torch.randn(1, 1, 4, dim, generator=gen), storage) for _ in "kv")
+    draft = [torch.randn(1, 1, tokens, dim, generator=gen).bfloat16() for _ in "kv"]
+    draft[1] = torch.where(torch.arange(tokens)[:, None] % 2 == 0, 1.0, -1.0).expand(1, 1, tokens, dim).bfloat16().clone()
+    parents = torch.cat((torch.arange(-1, tokens - 2), torch.tensor([-1])))[None]  # a chain, and one node beside it
+    visible, depths = oracle.tree_tables(parents, True)
+    out, mass, reach = oracle.attention(query, kc * ks[..., None].double(), vc * vs[..., None].double(), [0], 0, None, (*draft, visible, depths))
+    draft[1][0, 0, tokens - 1] = float("inf")
+    got = draft_tree_attention(
+        query.cuda(), kc.to(STORAGE[storage]).cuda(), vc.to(STORAGE[storage]).cuda(), *(d.cuda() for d in draft),
+        prepare_draft_tree(parents.cuda(), include_self=True), kv_lengths=torch.tensor([0]).cuda(), key_scales=ks.cuda(), value_scales=vs.cuda(),
+    ).cpu().double()
+    assert torch.isinf(got[0, -1]).all()
+    # rounding of the result, weights in two parts, scores and exponentials in fp32 as in oracle.bound
+    limit = 1.01 * (2.0**-8 * out.abs() + (2 * 2.0**-16 + 2.1 * ((dim + 8) * 2.0**-24 * reach + 2.0**-21)) * mass)
+    worst = ((got - out).abs() / limit)[0, :-1].max().item()
+    assert worst <= 1, f"error {worst:.3g} times the bound"

@@ -610,6 +610,12 @@ __device__ __forceinline__ void draft_keys(const wm_pool_attn_args& a, const Pla
             for (int h = 0; h < 4; ++h) one[h][s] = vr[h][s] & keep[h];
             R::value_fragment(va, one, s, none);
             float x[4] = {0.f, 0.f, 0.f, 0.f};
+            if (kFine) {
+              mma_16816(x, va[0], va[1], va[2], va[3], g == r ? rest[0][rt][0] : 0u, g == r ? rest[0][rt][1] : 0u);
+              // an infinity's weight may have nothing left for its second part, or have it with the other sign: the first part decides
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[e] = fabsf(x[e]) < INFINITY ? x[e] : 0.f;
+            }
             mma_16816(x, va[0], va[1], va[2], va[3], b0, b1);
             // the other columns hold 0 * infinity: only this row's is taken
 #pragma unroll
