@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oracle import serving_oracle as oracle
-from test_quant_pool import check_attention, on_gpu, quantised_problem
+from test_quant_pool import LONG_MASKED, check_attention, long_masked_problem, on_gpu, quantised_problem
 from white_matter_b200 import DraftTree, KVPoolCache, QuantKVPoolCache, draft_tree_attention, prepare_draft_tree
 from white_matter_b200.quant_pool import STORAGE
 
@@ -314,3 +314,46 @@ def test_an_infinite_drafted_value_takes_no_bits_from_the_rows_that_do_not_see_i
     limit = 1.01 * (2.0**-8 * out.abs() + (2 * 2.0**-16 + 2.1 * ((dim + 8) * 2.0**-24 * reach + 2.0**-21)) * mass)
     worst = ((got - out).abs() / limit)[0, :-1].max().item()
     assert worst <= 1, f"error {worst:.3g} times the bound"
+
+
+@pytest.mark.gpu
+@on_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("storage", ["plain", *sorted(STORAGE)])
+@pytest.mark.parametrize("shape", LONG_MASKED, ids=str)
+def test_masks_over_long_sequences_of_a_tree(shape, storage, dtype):
+    batch, heads, kv_heads, tokens, slots, dim, lead, lengths, blank = shape
+    query, pools, rows, mask = long_masked_problem(41, "int8" if storage == "plain" else storage, dtype, *shape)
+    if storage == "plain":
+        rows = [r.to(dtype) for r in rows]
+        pools = [(torch.where(torch.isnan(s)[..., None], torch.full_like(r, float("nan")), r), None) for r, (_, s) in zip(rows, pools)]
+    gen = torch.Generator().manual_seed(42)
+    parents = random_parents(gen, batch, tokens)
+    draft = [torch.randn(batch, kv_heads, tokens, dim, generator=gen).to(dtype) for _ in "kv"]
+    (k, ks), (v, vs) = pools
+    kind = STORAGE.get(storage, dtype)
+    got = draft_tree_attention(
+        query.cuda(), k.to(kind).cuda(), v.to(kind).cuda(), *(d.cuda() for d in draft), prepare_draft_tree(parents.cuda()), kv_lengths=torch.tensor(lengths).cuda(),
+        use_dummy_token=bool(lead), key_mask=mask.cuda(), key_scales=None if ks is None else ks.cuda(), value_scales=None if vs is None else vs.cuda(),
+    )
+    assert got[0].abs().amax(-1).min() > 0
+    check_attention(got, query, rows, lengths, lead, mask, (*draft, *oracle.tree_tables(parents, False)))
+
+
+@pytest.mark.gpu
+@on_gpu
+@pytest.mark.parametrize("tokens", [3, 30])
+@pytest.mark.parametrize("dim, dtype", [(8, torch.bfloat16), (40, torch.bfloat16), (72, torch.bfloat16), (120, torch.bfloat16), (4, torch.float32), (20, torch.float32), (100, torch.float32)])
+def test_head_sizes_that_fill_no_tile_over_long_sequences(dim, dtype, tokens):
+    """The same head sizes where a sequence has many steps, with and without a mask."""
+    batch, heads, kv_heads, slots, lengths = 2, 4, 2, 1100, [1090, 700]
+    gen = torch.Generator().manual_seed(43)
+    query, k, v = (torch.randn(batch, n, t, dim, generator=gen).to(dtype) for n, t in ((heads, tokens), (kv_heads, slots), (kv_heads, slots)))
+    draft = [torch.randn(batch, kv_heads, tokens, dim, generator=gen).to(dtype) for _ in "kv"]
+    parents = random_parents(gen, batch, tokens)
+    for mask in (None, torch.rand(batch, slots, generator=gen) < 0.6):
+        got = draft_tree_attention(
+            query.cuda(), k.cuda(), v.cuda(), *(d.cuda() for d in draft), prepare_draft_tree(parents.cuda()), kv_lengths=torch.tensor(lengths).cuda(),
+            key_mask=None if mask is None else mask.cuda(),
+        )
+        check_attention(got, query, [k, v], lengths, 0, mask, (*draft, *oracle.tree_tables(parents, False)))

@@ -733,3 +733,71 @@ def test_long_branches_and_strided_lengths_advance_alike(rows):
                 n += 1
             want.append(min(capacity, int(start[b]) + n))
         assert pool.lengths.tolist() == want
+
+
+# ------------------------------------------------------------------ GPU: masks over long sequences
+
+
+def long_masked_problem(seed, storage, dtype, batch, heads, kv_heads, tokens, slots, dim, lead, lengths, blank):
+    """A problem whose long sequences keep three slots of five, in runs that end inside tiles, while sequence `blank` (a short one,
+    or none) sees nothing; every slot that is not seen is poisoned."""
+    query, pools, rows, _ = quantised_problem(seed, storage, dtype, batch, heads, kv_heads, tokens, slots, dim, lead, False, lengths)
+    gen = torch.Generator().manual_seed(seed + 2)
+    mask = torch.rand(batch, slots, generator=gen) < 0.6
+    mask[:, 200:330] = False  # a whole tile that nothing is left of
+    mask[:, 1000:1300] = True  # and two that keep everything
+    if blank is not None:
+        mask[blank] = False
+    for codes, scales in pools:
+        for b in range(batch):
+            scales[b][:, ~mask[b]] = float("nan")
+            codes[b][:, ~mask[b]] = 100.0 if storage == "int8" else float("nan")
+    return query, pools, rows, mask
+
+
+LONG_MASKED = [  # batch, heads, kv_heads, tokens, slots, dim, lead, lengths, blank sequence
+    (3, 2, 1, 3, 4300, 128, 1, [4299, 4100, 77], 2),  # up to 16 rows per KV head, shares
+    (2, 4, 2, 1, 4300, 64, 0, [4300, 50], 1),
+    (2, 2, 1, 7, 4200, 80, 0, [4150, 30], 1),
+    (1, 3, 1, 2, 1900, 112, 0, [1890], None),  # a cluster per segment
+    (2, 4, 2, 5, 1800, 96, 1, [1799, 20], 1),
+    (3, 8, 1, 9, 4300, 64, 0, [4300, 4000, 60], 2),  # more rows: 32, 64 and 128 per block
+    (2, 2, 1, 16, 4300, 128, 1, [4200, 40], 1),
+    (1, 3, 1, 40, 1000, 112, 0, [990], None),
+    (2, 4, 1, 15, 2100, 48, 1, [2000, 9], 1),
+]
+
+
+@pytest.mark.gpu
+@on_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("storage", sorted(STORAGE))
+@pytest.mark.parametrize("shape", LONG_MASKED, ids=str)
+def test_masks_over_long_sequences(shape, storage, dtype):
+    batch, heads, kv_heads, tokens, slots, dim, lead, lengths, blank = shape
+    query, pools, rows, mask = long_masked_problem(31, storage, dtype, *shape)
+    (k, ks), (v, vs) = pools
+    got = quantized_pool_attention(
+        query.cuda(), k.to(STORAGE[storage]).cuda(), v.to(STORAGE[storage]).cuda(), ks.cuda(), vs.cuda(), kv_lengths=torch.tensor(lengths).cuda(),
+        use_dummy_token=bool(lead), key_mask=mask.cuda(),
+    )
+    assert got[0].abs().amax(-1).min() > 0 and (blank is None or not got[blank].any())
+    check_attention(got, query, rows, lengths, lead, mask)
+
+
+@pytest.mark.gpu
+@on_gpu
+@pytest.mark.parametrize("tokens", [1, 3, 20, 100])
+@pytest.mark.parametrize("storage", sorted(STORAGE))
+def test_a_call_repeats_itself_bit_for_bit(storage, tokens):
+    """The shares, and so the order of every sum, follow from the sizes and lengths alone."""
+    torch.manual_seed(23)
+    pool = QuantKVPoolCache(9, 1, 3, 3000, 64, storage=storage)
+    for _ in range(3):
+        pool.append(torch.randn(9, 3, 1000, 64, device="cuda"), torch.randn(9, 3, 1000, 64, device="cuda"))
+    pool.lengths.copy_(torch.arange(9) * 333 + 1)
+    for dtype in (torch.bfloat16, torch.float32):
+        query = torch.randn(9, 6, tokens, 64, device="cuda").to(dtype)
+        first = pool.read(query, 0)
+        for _ in range(5):
+            assert torch.equal(pool.read(query, 0), first)
