@@ -433,15 +433,6 @@ def dtype_code(dtype: torch.dtype) -> int:
     raise ValueError(f"sm100 kernels support float32 and bfloat16, got {dtype}")
 
 
-def storage_code(dtype: torch.dtype) -> int:
-    """Element type of a pool: the operator types, or one of the 8-bit forms."""
-    if dtype == torch.int8:
-        return WM_INT8
-    if dtype == torch.float8_e4m3fn:
-        return WM_E4M3
-    return dtype_code(dtype)
-
-
 def strides3(t: torch.Tensor) -> _Strides:
     """(batch, head, token) element strides of a (B,H,T,D) view."""
     return _Strides(t.stride(0), t.stride(1), t.stride(2))
