@@ -98,8 +98,10 @@ int cluster_size(const wm_pool_attn_args& a, const Plan& p) {
 bool make_plan(const wm_pool_attn_args& a, Plan& p) {
   const long long rows = rows_of(a);
   p.rows_per_block = rows_per_block(a);
-  // measured with 1, 2, 4: 241, 227, 197 us on 64 sequences with 32 drafted tokens (shared memory, heads of 64); 113, 118, 126 us on
-  // 8 sequences with 41 and 4 heads per group (heads of 128); 143, 143, 147 us on 64 sequences with one token
+  // measured with 1, 2, 4, 8.  Shared memory, heads of 64: 64 sequences with 32 drafted tokens over bf16 243, 223, 197, 201 us, over int8 328, 309,
+  // 294, 304 us; small calls differ less (8 sequences with 41 tokens, 4 heads per KV head, int8: 60, 61, 65, 73 us; 24 sequences with 7, e4m3: 52, 47,
+  // 49, 56 us).  Heads of 128, the same four: 223, 224, 229, 238; 274, 276, 282, 294; 106, 112, 117, 132; 76, 77, 83, 94 us.  Few rows: one token,
+  // 64 sequences, int8 rows of 64 125, 125, 128, 132 us, rows of 128 with 4 heads per KV head 128, 130, 135, 145 us; fp32, 8 tokens 85, 86, 92, 99 us
   p.segment_cost = in_shared(a) ? (a.head_dim <= 64 ? 4 : 1) : 2;
   const long long blocks = (rows + p.rows_per_block - 1) / p.rows_per_block;
   p.draft_tiles = a.ancestors != nullptr ? (a.q_len + kTileKeys - 1) / kTileKeys : 0;

@@ -17,12 +17,14 @@
 // sequence were 1.2 to 1.5 times as far from the exact result as the output's rounding, with two 1.0, for 5 % of the time of
 // 64 sequences (115.6 -> 121 us) and none on one.  (Over bf16 pools an infinity's product with the rest would be NaN.)
 //
-// A row's weights are exponentials against a reference that moves only when a score exceeds it by 8 (in powers of two):
-// the sums are fp32 and the weights floating, so nothing is lost by weights up to 2^8, and the common step needs
-// one vote instead of a reduction over the lanes.
+// A row's weights are exponentials against a reference that moves only when a score exceeds it by 8 (in powers of two), so the
+// common step needs one vote instead of a reduction over the lanes.  Weights up to 2^8 lose no precision (the sums are fp32), but range:
+// values above 2^118 in magnitude may overflow sums whose mean does not, and weights below 2^-118 of a row's largest are lost.
 //
-// 64 sequences of up to 8192 tokens, 16 heads of 64, one token: 121 us over int8 (4 710 GB/s), 121 us over e4m3, bound by the instructions that
-// make bf16 of codes; bf16 with 8 drafted tokens 163 us (6 600 GB/s), bound by HBM.  One sequence of 480 tokens: 5.6 us.
+// 64 sequences of up to 8192 tokens, 16 heads of 64, one token: 122 us over int8 (4 690 GB/s), 133 us over e4m3.  No unit is full there (2.2
+// instructions per cycle and SM of 4, ALU pipe 55 %, tensor pipe 21 %, DRAM 72 % of the copy bandwidth): what is left is latency, of memory before all, that 16
+// warps per SM do not cover, and every instruction more shows.  Heads of 128, 4 per KV head: 130 and 141 us for 3 % fewer bytes.  bf16
+// with 8 drafted tokens 163 to 174 us (6 600 to 6 190 GB/s), bound by HBM.  One sequence of 480 tokens: 5.6 us.
 #pragma once
 
 #include <math.h>
@@ -70,7 +72,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return y;
 }
 // (a & b) | c as one instruction: written as operators with two constants it becomes two, and the conversion of int8 codes is
-// what the 8-bit read spends most of its instructions on (64 sequences of up to 8192 rows: 143 us against 112 us, before the weights were held in two parts)
+// what the 8-bit read spends most of its instructions on (64 sequences of up to 8192 rows: 152 us against 122 us)
 __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t y;
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(a), "r"(b), "r"(c));
@@ -861,7 +863,9 @@ cudaError_t launch_mma(const wm_pool_attn_args& a, const Plan& plan, cudaStream_
     config.numAttrs = 1;
     return cudaLaunchKernelEx(&config, pool_attn_mma_kernel<kStorage, DP, RT, kTree, kCluster>, a, plan);
   }
-  if constexpr (DP % 64 == 0) {  // heads of 64 and 128, the usual pool: 115 us against 127 us on 64 sequences of up to 8192 int8 rows, before the weights were held in two parts
+  // heads of 64 and 128, the usual pool: 122 us against 133 us on 64 sequences of up to 8192 int8 rows of 64, 130 us against 135 us on rows of
+  // 128; rows of 96 take 139 us this way and 113 us without, rows of 32 would gain (87 against 98 us)
+  if constexpr (DP % 64 == 0) {
     const bool scaled = kStorage != WM_BF16;
     if (a.head_dim == DP && a.k_strides[2] == DP && a.v_strides[2] == DP && (!scaled || (a.k_scale_strides[2] == 1 && a.v_scale_strides[2] == 1))) {
       pool_attn_mma_kernel<kStorage, DP, RT, kTree, kDenseShares><<<plan.blocks, kThreads, 0, stream>>>(a, plan);

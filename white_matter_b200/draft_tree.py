@@ -84,7 +84,8 @@ def draft_tree_attention(
     ``key_scales`` / ``value_scales`` as in ``quantized_pool_attention``; the rules for ``kv_lengths``,
     ``use_dummy_token`` and ``key_mask`` are the same.  Node i also sees the drafted tokens that ``tree`` names.
     Padding nodes, and nodes that see nothing, return zero; the K/V of padding nodes, and of slots that are not seen, may
-    hold anything.  Returns (B,T,H,D).
+    hold anything.  Precision and range are those of ``quantized_pool_attention``; over bf16 pools the weights are one bf16
+    part for any number of rows.  Returns (B,T,H,D).
     """
     if query.ndim != 4:
         raise ValueError("query must be (B,H,T,D)")

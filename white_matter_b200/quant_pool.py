@@ -7,12 +7,14 @@ With ``a`` the row's largest magnitude:
 * ``"int8"`` (``torch.int8``): ``scale = a / 127``, ``code = round(x * (127 / a))``, quotients and product rounded to
   fp32, halves to even.  An element is off by at most half a step, ``a / 254`` (and a few fp32 roundings).
 * ``"e4m3"`` (``torch.float8_e4m3fn``): ``scale`` is the smallest power of two with ``a / scale <= 448``, ``code`` is
-  ``x / scale`` rounded to e4m3, halves to even.  An element is off by at most 2^-4 of itself, or 2^-10 of the scale.
+  ``x / scale`` rounded to e4m3, halves to even.  An element is off by at most 2^-4 of itself, or 2^-10 of the scale; one of
+  248 * 2^120 or more rounds to 2^128, which reads back as infinity.
 
 A row whose largest magnitude is below 2^-100 is held as zeros with scale 0.  A row with an infinity or NaN gets scale
 NaN: it reads back as NaN throughout, and a query that sees it returns NaN.  A pool that was quantised elsewhere may hold
 e4m3's NaN codes: a query that sees one among the keys returns NaN, one among the values makes its element NaN.  The upstream project keeps its pool in
-bf16 (models/cache.py:43-60); these operators have no counterpart there.  All of them are for inference.
+bf16 (models/cache.py:43-60); these operators have no counterpart there.  All of them are for inference, and not for tracing:
+they pass addresses to the library, which ends a ``torch.compile`` graph (``fullgraph=True`` raises); CUDA graphs capture them.
 """
 
 from __future__ import annotations
@@ -298,6 +300,11 @@ def quantized_pool_attention(
     s < ``kv_lengths[b]`` (all of them without lengths) and, with ``use_dummy_token``, slot 0, as far as ``key_mask``
     (B,N) keeps them; slots that are not seen may hold anything.  Rows without a visible slot return zero.  The
     lengths stay on the device, so the call can be captured in a CUDA graph.  Returns (B,T,H,D).
+
+    Sums and soft-max statistics are fp32.  With bf16 queries the weights, times the values' scales, enter the product as two bf16 parts
+    (16 bits) for up to 16 rows (tokens times heads) per KV head and as one for more.  Values above 2^118 in magnitude may
+    overflow the sums although their mean does not; weights below 2^-118 of a row's largest, and products of a weight and a scale
+    below 2^-126, count as nothing.
     """
     if key.dtype not in _QUANTISED:
         raise ValueError("the pool must be int8 or float8_e4m3fn")
