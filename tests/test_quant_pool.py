@@ -1,6 +1,7 @@
 """The 8-bit KV pool: refusals and layouts on the CPU; commit, read back and read against the CPU oracle on the GPU."""
 
 import ctypes
+import functools
 import re
 from pathlib import Path
 
@@ -586,6 +587,18 @@ def test_a_captured_step_notices_replaced_scales():
 # ------------------------------------------------------------------ GPU: values of zero, codes that are no number
 
 
+@functools.lru_cache
+def leading_key_rows(storage, slots, dim):
+    """Codes and scales of the keys and values of the test below."""
+    gen = torch.Generator().manual_seed(21)
+    k, v = torch.zeros(1, 1, slots, dim), torch.zeros(1, 1, slots, dim)
+    k[..., 0], k[..., 1] = -5.5, 5.5  # exact in both storages
+    k[0, 0, 0, 0], k[0, 0, 0, 1] = 5.5, 0.0
+    v[0, 0, 0] = torch.randn(dim, generator=gen)
+    v[0, 0, 1::3] = 2.0**-98 * torch.randn(len(range(1, slots, 3)), dim, generator=gen).clamp(-2, 2)
+    return tuple(oracle.quantise_rows(t, storage) for t in (k, v))
+
+
 def expanded(codes, scales, storage, batch):
     """One sequence's rows as the pool of a whole batch, without copies: enough segments that a share holds a long run of keys."""
     codes, scales = codes.to(STORAGE[storage]).cuda(), scales.cuda()
@@ -602,13 +615,7 @@ def test_keys_with_values_of_zero_stay_in_the_sum(storage, dtype, tokens, dim):
     """One key leads 8 000 others by 11.2 (a weight of 2^-16.2 each, 0.11 together); the others' values are zeros, or so small that
     their scale times such a weight is no normal fp32 number."""
     batch, slots = (300, 8000) if dtype == torch.bfloat16 else (300, 2000)
-    gen = torch.Generator().manual_seed(21)
-    k, v = torch.zeros(1, 1, slots, dim), torch.zeros(1, 1, slots, dim)
-    k[..., 0], k[..., 1] = -5.5, 5.5  # exact in both storages
-    k[0, 0, 0, 0], k[0, 0, 0, 1] = 5.5, 0.0
-    v[0, 0, 0] = torch.randn(dim, generator=gen)
-    v[0, 0, 1::3] = 2.0**-98 * torch.randn(len(range(1, slots, 3)), dim, generator=gen).clamp(-2, 2)
-    (kc, ks), (vc, vs) = (oracle.quantise_rows(t, storage) for t in (k, v))
+    (kc, ks), (vc, vs) = leading_key_rows(storage, slots, dim)
     query = torch.zeros(1, 1, tokens, dim).to(dtype)
     query[..., 0], query[..., 1] = 1.0, -0.04
     (keys, key_scales), (values, value_scales) = expanded(kc, ks, storage, batch), expanded(vc, vs, storage, batch)
@@ -630,7 +637,8 @@ def test_e4m3_codes_that_are_no_number(dtype, batch, slots, tokens, dim):
     it, in a visible value their element alone, and nothing else."""
     gen = torch.Generator().manual_seed(22)
     heads, kv_heads = 4, 2
-    (kc, ks), (vc, vs) = (oracle.quantise_rows(torch.randn(batch, kv_heads, slots, dim, generator=gen), "e4m3") for _ in "kv")
+    kc, vc = (torch.randn(batch, kv_heads, slots, dim, generator=gen).mul(64).to(torch.float8_e4m3fn).float() for _ in "kv")
+    ks, vs = (torch.exp(0.3 * torch.randn(batch, kv_heads, slots, generator=gen)) / 64 for _ in "kv")
     query = torch.randn(batch, heads, tokens, dim, generator=gen).to(dtype)
     mask = torch.rand(batch, slots, generator=gen) < 0.7
     lengths = torch.tensor([slots - 3, slots // 2][:batch])
