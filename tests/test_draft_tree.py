@@ -357,3 +357,30 @@ def test_head_sizes_that_fill_no_tile_over_long_sequences(dim, dtype, tokens):
             key_mask=None if mask is None else mask.cuda(),
         )
         check_attention(got, query, [k, v], lengths, 0, mask, (*draft, *oracle.tree_tables(parents, False)))
+
+
+@pytest.mark.gpu
+@on_gpu
+@pytest.mark.parametrize("slots", [200, 4400])
+@pytest.mark.parametrize("tokens", [4, 12, 30])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_e4m3_codes_that_are_no_number_reach_the_nodes_and_no_padding(dtype, tokens, slots):
+    gen = torch.Generator().manual_seed(45)
+    batch, heads, kv_heads, dim = 2, 2, 1, 64
+    codes = [torch.randn(batch, kv_heads, slots, dim, generator=gen).mul(64).to(torch.float8_e4m3fn).view(torch.uint8) for _ in "kv"]
+    scales = torch.full((batch, kv_heads, slots), 1 / 64)
+    query, *draft = (torch.randn(batch, n, tokens, dim, generator=gen).to(dtype) for n in (heads, kv_heads, kv_heads))
+    parents = random_parents(gen, batch, tokens)
+    parents[:, 2] = -2
+    live = oracle.tree_tables(parents, True)[1] >= 0
+    for kind in (0, 1):
+        spoilt = [c.clone() for c in codes]
+        spoilt[kind][1, 0, slots - 7, 9] = 0xFF
+        got = draft_tree_attention(
+            query.cuda(), *(s.view(torch.float8_e4m3fn).cuda() for s in spoilt), *(d.cuda() for d in draft), prepare_draft_tree(parents.cuda(), include_self=True),
+            key_scales=scales.cuda(), value_scales=scales.cuda(),
+        ).cpu()
+        want = torch.zeros(batch, tokens, heads, dim, dtype=torch.bool)
+        want[1, :, :, slice(None) if kind == 0 else 9] = live[1, :, None] if kind == 1 else live[1, :, None, None]
+        assert torch.equal(torch.isnan(got), want)
+        assert not got[~live].any()
